@@ -185,6 +185,73 @@ int prana_attention_decode_splitk_noalloc(const float *q, const uint16_t *const 
 /* attention (prefill, attention.rs:236-284): causal over f32 K/V. */
 int prana_attention_prefill(const float *q, const float *k, const float *v, size_t seq, size_t n_heads,
                             size_t n_kv_heads, size_t head_dim, float *out, prana_stream_t stream);
+/* ---- serving: packed prompts, 8-bit caches, trees of drafted tokens
+ * No counterpart in the reference, which serves one sequence at a time, drafts
+ * a chain and keeps its cache in f16. These entry points take the rows of many
+ * sequences packed behind one another, with the sequences' sizes and caches in
+ * host arrays that are read before the call returns. They are asynchronous on
+ * `stream` (NULL = the library's), allocate nothing and keep nothing between
+ * calls, so they may be captured into a HIP graph; a replay repeats the call
+ * with the sizes and pointers it was captured with. Results are f32-accurate
+ * (not the scalar tier's bits). Device pointers lie on 16 bytes (scales on 4),
+ * row strides are multiples of 16 bytes and head_dim is a multiple of 8 up to
+ * 256; anything else is PRANA_ERR_INVALID. Outputs do not overlap inputs. */
+
+/* Causal attention of whole prompts: sequence s is the next seq_lens[s] rows
+ * (0 allowed) of q, k, v and out, and its row i attends to its rows 0..=i. q
+ * and out are `type` (PRANA_F32 or PRANA_F16), RoPE applied, with row strides
+ * ld_q and ld_out in elements; k and v are f16 rows (prana_f32_to_f16, or a
+ * cache's) with row stride ld_kv. So q, k and v may lie in one buffer of fused
+ * projections. Any n_heads / n_kv_heads. */
+int prana_attention_packed(const void *q, const uint16_t *k, const uint16_t *v, int type, const size_t *seq_lens,
+                           size_t n_seq, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t ld_q,
+                           size_t ld_kv, size_t ld_out, void *out, prana_stream_t stream);
+
+/* One sequence's K and V cache: `rows` rows of n_kv_heads*head_dim values.
+ * PRANA_KV_F16: f16, the scales unused (what prana_kv_write_f16 fills).
+ * PRANA_KV_Q8: i8 with one f32 scale per row and KV head, [rows][n_kv_heads]:
+ * a value is its i8 times its scale. */
+enum prana_kv_type { PRANA_KV_F16 = 1, PRANA_KV_Q8 = 8 };
+typedef struct prana_kv {
+  void *k, *v;
+  float *k_scales, *v_scales;
+  size_t rows;
+} prana_kv;
+
+/* Quantizes K and V rows into the 8-bit caches of n_seq sequences: the next
+ * n_rows[s] rows (0 allowed) of k and v (f32, row stride ld) become rows
+ * first_rows[s].. of kv[s] (first_rows[s] + n_rows[s] <= kv[s].rows). Per row
+ * and KV head: scale = amax/127 (1 when all values are 0), i8 = x*127/amax
+ * rounded exactly, ties away from zero. A head that holds an infinity or NaN
+ * reads back as NaN. No two sequences of a call may share a cache row. */
+int prana_kv_write_q8(const float *k, const float *v, size_t ld, const prana_kv *kv, const size_t *first_rows,
+                      const size_t *n_rows, size_t n_seq, size_t n_kv_heads, size_t head_dim, prana_stream_t stream);
+/* The reverse: rows first_rows[s].. of the 8-bit caches as the next n_rows[s]
+ * rows of k and v, `type` PRANA_F32 or PRANA_F16 (rounded to nearest even),
+ * row stride ld. */
+int prana_kv_read_q8(const prana_kv *kv, const size_t *first_rows, const size_t *n_rows, size_t n_seq,
+                     size_t n_kv_heads, size_t head_dim, int type, void *k, void *v, size_t ld,
+                     prana_stream_t stream);
+
+/* Attention of drafted tokens over the caches of n_seq sequences, a tree per
+ * sequence: sequence s has n_tree[s] (0..64) drafted tokens whose K/V rows are
+ * already in its cache at rows past[s].. (past[s] + n_tree[s] <= kv[s].rows).
+ * Its drafted token i attends to rows 0..past[s]-1 and to drafted token j
+ * where bit j of its mask word is set (itself and its ancestors; bits from
+ * n_tree[s] on are ignored). mask: device, one word per drafted token; NULL =
+ * a chain (token i sees tokens 0..=i), so n_tree = 1 is a decode step and
+ * n_tree = k the verify batch of a chain draft. A token that sees no row gets
+ * zeros. q and out: device f32 [sum of n_tree][n_heads*head_dim], RoPE applied
+ * to q. What masked rows and rows past the drafted ones hold (infinities and
+ * NaN too) does not reach the result. workspace: device scratch of the size
+ * prana_attention_tree_workspace gives for the same sizes (it may be 0, then
+ * workspace may be NULL); calls that may run at the same time need one each. */
+int prana_attention_tree(const float *q, int kv_type, const prana_kv *kv, const size_t *past, const size_t *n_tree,
+                         size_t n_seq, const uint64_t *mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                         float *out, void *workspace, size_t workspace_bytes, prana_stream_t stream);
+int prana_attention_tree_workspace(const size_t *past, const size_t *n_tree, size_t n_seq, size_t n_heads,
+                                   size_t n_kv_heads, size_t head_dim, size_t *bytes);
+
 /* Greedy argmax (infer.rs:560-568 / sampler.rs:40-48) of each row. */
 int prana_argmax(const float *logits, size_t rows, size_t n, uint32_t *out_idx, prana_stream_t stream);
 /* f32_to_f16 / f16_to_f32 (lib.rs:57-113) elementwise. */

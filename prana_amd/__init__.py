@@ -13,9 +13,10 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import GenStats, PranaConfig, PranaError, check, check_synth, load, load_synth
+from ._lib import GenStats, PranaConfig, PranaError, PranaKv, check, check_synth, load, load_synth
 
 F32, F16, Q4_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 8, 12, 14
+KV_F16, KV_Q8 = 1, 8  # prana_kv_type
 GGML_NAMES = {F32: "F32", F16: "F16", Q4_0: "Q4_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q6_K: "Q6_K"}
 
 
@@ -336,6 +337,110 @@ def attention_prefill(q, k, v, seq, n_heads, n_kv_heads, head_dim):
     do = DeviceArray((seq, n_heads * head_dim), np.float32)
     check(load().prana_attention_prefill(dq.ptr, dk.ptr, dv.ptr, seq, n_heads, n_kv_heads, head_dim, do.ptr, None))
     return do.to_host()
+
+
+# ---------------------------------------------------------------- serving
+class KvF16:
+    """One sequence's f16 K/V cache on the device: [rows, n_kv_heads*head_dim]
+    halves (host arrays are copied; DeviceArrays are used in place)."""
+
+    kind = KV_F16
+
+    def __init__(self, k, v):
+        self.k, self.v = (c if isinstance(c, DeviceArray)
+                          else DeviceArray.from_host(np.ascontiguousarray(c).view(np.uint16)) for c in (k, v))
+        self.rows = self.k.shape[0]
+
+    def struct(self):
+        return PranaKv(self.k.ptr, self.v.ptr, None, None, self.rows)
+
+
+class KvQ8:
+    """One sequence's 8-bit K/V cache on the device: i8 rows and an f32 scale
+    per row and KV head. Filled by kv_write_q8."""
+
+    kind = KV_Q8
+
+    def __init__(self, rows, n_kv_heads, head_dim):
+        self.rows, self.n_kv_heads, self.head_dim = rows, n_kv_heads, head_dim
+        self.k, self.v = (DeviceArray.from_host(np.zeros((rows, n_kv_heads * head_dim), np.int8)) for _ in "kv")
+        self.k_scales, self.v_scales = (DeviceArray.from_host(np.ones((rows, n_kv_heads), np.float32)) for _ in "kv")
+
+    def struct(self):
+        return PranaKv(self.k.ptr, self.v.ptr, self.k_scales.ptr, self.v_scales.ptr, self.rows)
+
+
+def _sizes(values):
+    return (C.c_size_t * max(len(values), 1))(*[int(x) for x in values])
+
+
+def _kv_structs(caches):
+    return (PranaKv * max(len(caches), 1))(*[c.struct() for c in caches])
+
+
+def kv_write_q8(caches, k, v, first_rows, n_rows):
+    """Quantize the packed f32 rows of k and v into KvQ8 caches: the next
+    n_rows[s] rows become rows first_rows[s].. of caches[s]."""
+    dk, dv = DeviceArray.from_host(np.asarray(k, np.float32)), DeviceArray.from_host(np.asarray(v, np.float32))
+    check(load().prana_kv_write_q8(dk.ptr, dv.ptr, dk.shape[1], _kv_structs(caches), _sizes(first_rows),
+                                   _sizes(n_rows), len(caches), caches[0].n_kv_heads, caches[0].head_dim, None))
+    check(load().prana_synchronize())
+
+
+def kv_read_q8(caches, first_rows, n_rows, half=False):
+    """Rows of KvQ8 caches as values, packed: (k, v) in f32, or in f16."""
+    width = caches[0].n_kv_heads * caches[0].head_dim
+    dk, dv = (DeviceArray((int(sum(n_rows)), width), np.float16 if half else np.float32) for _ in "kv")
+    check(load().prana_kv_read_q8(_kv_structs(caches), _sizes(first_rows), _sizes(n_rows), len(caches),
+                                  caches[0].n_kv_heads, caches[0].head_dim, F16 if half else F32, dk.ptr, dv.ptr,
+                                  width, None))
+    return dk.to_host(), dv.to_host()
+
+
+def attention_packed(q, k, v, seq_lens, n_heads, n_kv_heads, head_dim):
+    """Causal attention of whole prompts packed behind one another: q [rows,
+    n_heads*head_dim] in f32 or f16 (the result has its type), k / v f16 rows."""
+    q = np.ascontiguousarray(q)
+    kind = {np.dtype(np.float32): F32, np.dtype(np.float16): F16}[q.dtype]
+    dq = DeviceArray.from_host(q)
+    dk, dv = (DeviceArray.from_host(np.ascontiguousarray(x).view(np.uint16)) for x in (k, v))
+    do = DeviceArray(q.shape, q.dtype)
+    check(load().prana_attention_packed(dq.ptr, dk.ptr, dv.ptr, kind, _sizes(seq_lens), len(seq_lens), n_heads,
+                                        n_kv_heads, head_dim, q.shape[1], dk.shape[1], q.shape[1], do.ptr, None))
+    return do.to_host()
+
+
+def attention_tree_workspace(past, n_tree, n_heads, n_kv_heads, head_dim):
+    """Bytes of device scratch attention_tree needs for these sizes."""
+    n = C.c_size_t()
+    check(load().prana_attention_tree_workspace(_sizes(past), _sizes(n_tree), len(past), n_heads, n_kv_heads,
+                                                head_dim, C.byref(n)))
+    return n.value
+
+
+def attention_tree(q, caches, past, n_tree, n_heads, n_kv_heads, head_dim, mask=None):
+    """Attention of drafted tokens, a tree per sequence, over KvF16 or KvQ8
+    caches: q [sum(n_tree), n_heads*head_dim] f32, mask one word per drafted
+    token (bit j: it sees drafted token j of its sequence; None = a chain)."""
+    dq = DeviceArray.from_host(np.asarray(q, np.float32))
+    dm = DeviceArray.from_host(np.asarray(mask, np.uint64)) if mask is not None else None
+    work = DeviceArray((attention_tree_workspace(past, n_tree, n_heads, n_kv_heads, head_dim),), np.uint8)
+    do = DeviceArray(dq.shape, np.float32)
+    check(load().prana_attention_tree(dq.ptr, caches[0].kind, _kv_structs(caches), _sizes(past), _sizes(n_tree),
+                                      len(caches), dm.ptr if dm else None, n_heads, n_kv_heads, head_dim, do.ptr,
+                                      work.ptr, work.nbytes, None))
+    return do.to_host()  # (waits for the library's stream)
+
+
+def tree_mask(parents):
+    """Mask words of one sequence's tree from each token's parent (an earlier
+    token of the tree, or -1): a token sees itself and its ancestors."""
+    words = []
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError("a token's parent is an earlier token or -1")
+        words.append((words[p] if p >= 0 else 0) | (1 << i))
+    return np.array(words, np.uint64)
 
 
 def argmax(logits):

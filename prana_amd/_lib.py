@@ -37,6 +37,12 @@ class GenStats(C.Structure):
     ]
 
 
+class PranaKv(C.Structure):
+    """prana_kv: one sequence's K and V cache (device pointers)."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p), ("rows", c_size)]
+
+
 class PranaError(RuntimeError):
     """A failed call: .code is the library's status (PRANA_ERR_*)."""
 
@@ -88,6 +94,17 @@ _SIGS = {
                                                       c_size, c_size, c_void_p, c_void_p]),
     "prana_attention_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_size, c_size, c_size, c_size, c_void_p,
                                         c_void_p]),
+    # serving
+    "prana_attention_packed": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size, c_size, c_size, c_size,
+                                       c_size, c_size, c_size, c_void_p, c_void_p]),
+    "prana_kv_write_q8": (c_int, [c_void_p, c_void_p, c_size, c_void_p, c_void_p, c_void_p, c_size, c_size, c_size,
+                                  c_void_p]),
+    "prana_kv_read_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_size, c_size, c_size, c_int, c_void_p, c_void_p,
+                                 c_size, c_void_p]),
+    "prana_attention_tree": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_size, c_void_p, c_size, c_size,
+                                     c_size, c_void_p, c_void_p, c_size, c_void_p]),
+    "prana_attention_tree_workspace": (c_int, [c_void_p, c_void_p, c_size, c_size, c_size, c_size,
+                                               C.POINTER(c_size)]),
     "prana_argmax": (c_int, [c_void_p, c_size, c_size, c_void_p, c_void_p]),
     "prana_f32_to_f16": (c_int, [c_void_p, c_size, c_void_p, c_void_p]),
     "prana_f16_to_f32": (c_int, [c_void_p, c_size, c_void_p, c_void_p]),

@@ -12,6 +12,7 @@
 #include "gguf.h"
 #include "graph.h"
 #include "model.h"
+#include "serving.h"
 #include "tokenizer.h"
 
 namespace prana {
@@ -450,6 +451,68 @@ int prana_attention_prefill(const float* q, const float* k, const float* v, size
                                   need ? sc.att.as<float>() : nullptr, s);
     if (rc) return rc;
     PRANA_HIP(hipStreamSynchronize(s));
+    return static_cast<int>(kOk);
+  });
+}
+
+// ------------------------------------------------------------------ serving
+// The checks come before the device is touched: a refused call needs no GPU.
+int prana_attention_packed(const void* q, const uint16_t* k, const uint16_t* v, int type, const size_t* seq_lens,
+                           size_t n_seq, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t ld_q,
+                           size_t ld_kv, size_t ld_out, void* out, prana_stream_t stream) {
+  return guard([&] {
+    if (int rc = check_attention_packed(q, k, v, type, seq_lens, n_seq, n_heads, n_kv_heads, head_dim, ld_q, ld_kv,
+                                        ld_out, out))
+      return rc;
+    INIT_OR_RETURN();
+    return launch_attention_packed(q, k, v, type == PRANA_F16, seq_lens, n_seq, n_heads, n_kv_heads, head_dim, ld_q,
+                                   ld_kv, ld_out, out, pick_stream(stream));
+  });
+}
+
+int prana_kv_write_q8(const float* k, const float* v, size_t ld, const prana_kv* kv, const size_t* first_rows,
+                      const size_t* n_rows, size_t n_seq, size_t n_kv_heads, size_t head_dim, prana_stream_t stream) {
+  return guard([&] {
+    if (int rc = check_kv_q8("kv_write_q8", kv, first_rows, n_rows, n_seq, n_kv_heads, head_dim, k, v, ld, 4))
+      return rc;
+    INIT_OR_RETURN();
+    return launch_kv_write_q8(k, v, ld, kv, first_rows, n_rows, n_seq, n_kv_heads, head_dim, pick_stream(stream));
+  });
+}
+
+int prana_kv_read_q8(const prana_kv* kv, const size_t* first_rows, const size_t* n_rows, size_t n_seq,
+                     size_t n_kv_heads, size_t head_dim, int type, void* k, void* v, size_t ld,
+                     prana_stream_t stream) {
+  return guard([&] {
+    PRANA_CHECK(type == PRANA_F32 || type == PRANA_F16, "kv_read_q8: type must be PRANA_F32 or PRANA_F16");
+    if (int rc = check_kv_q8("kv_read_q8", kv, first_rows, n_rows, n_seq, n_kv_heads, head_dim, k, v, ld,
+                             type == PRANA_F32 ? 4 : 2))
+      return rc;
+    INIT_OR_RETURN();
+    return launch_kv_read_q8(kv, first_rows, n_rows, n_seq, n_kv_heads, head_dim, type == PRANA_F16, k, v, ld,
+                             pick_stream(stream));
+  });
+}
+
+int prana_attention_tree(const float* q, int kv_type, const prana_kv* kv, const size_t* past, const size_t* n_tree,
+                         size_t n_seq, const uint64_t* mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                         float* out, void* workspace, size_t workspace_bytes, prana_stream_t stream) {
+  return guard([&] {
+    if (int rc = check_attention_tree(q, kv_type, kv, past, n_tree, n_seq, mask, n_heads, n_kv_heads, head_dim, out,
+                                      workspace, workspace_bytes))
+      return rc;
+    INIT_OR_RETURN();
+    return launch_attention_tree(q, kv_type == PRANA_KV_Q8, kv, past, n_tree, n_seq, mask, n_heads, n_kv_heads,
+                                 head_dim, out, static_cast<float*>(workspace), pick_stream(stream));
+  });
+}
+
+int prana_attention_tree_workspace(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads,
+                                   size_t n_kv_heads, size_t head_dim, size_t* bytes) {
+  return guard([&] {
+    PRANA_CHECK(bytes, "attention_tree_workspace: null argument");
+    if (int rc = check_tree_sizes(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim)) return rc;
+    *bytes = attention_tree_floats(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim) * sizeof(float);
     return static_cast<int>(kOk);
   });
 }

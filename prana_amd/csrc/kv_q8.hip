@@ -1,0 +1,277 @@
+// The 8-bit K/V cache: rows of K and V quantized as they are written
+// (prana_kv_write_q8) and read back (prana_kv_read_q8).
+//
+//   scale = amax / 127 over the values of one KV head in one row (1 when all
+//   are 0), i8 = round(x * 127 / amax), ties away from zero, value = i8 * scale.
+//
+// One scale per row and head, because that is what attention can take out of
+// its products: the scale of a K row multiplies its score, that of a V row its
+// probability, and the i8 values go to the matrix cores as they are.
+//
+// Both kernels move each byte once and are bound by memory. A lane holds 8
+// values of a head (two 16-byte loads of f32, one 8-byte store of i8), the
+// lanes of a head find its maximum among them, and a lane takes kItems heads
+// whose loads are in flight together.
+#include <algorithm>
+
+#include "common.h"
+#include "serving.h"
+
+namespace prana {
+
+namespace {
+
+constexpr int kKvNT = 256;
+constexpr int kKvSeqs = 64;  // sequences of one launch: 56 bytes each of kernel arguments
+constexpr int kItems = 4;    // heads of a lane group, loads in flight together
+
+struct KvSeq {
+  void *k, *v;
+  float *ks, *vs;
+  uint32_t src;     // first packed row
+  uint32_t rows;    // rows to move
+  uint32_t first;   // first cache row
+  uint32_t block0;  // first workgroup of the sequence
+};
+
+struct KvArgs {
+  const void* k;  // the packed side
+  const void* v;
+  size_t ld;
+  uint32_t n_seq, n_kv, hd;
+  KvSeq seq[kKvSeqs];
+};
+
+// The sequence that workgroup b belongs to: the last whose first workgroup is
+// not past it.
+__device__ __forceinline__ int find_seq(const KvArgs& a, uint32_t b) {
+  int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.seq[mid].block0 <= b)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// Largest of v over aligned groups of LPH lanes (a power of two).
+template <int LPH>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+#pragma unroll
+  for (int o = 1; o < LPH; o <<= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, 64)));
+  return v;
+}
+
+// round(|x| * 127 / amax) with ties up, exactly. In f32 the quotient is within
+// 127 * 3 * 2^-24 < 2.4e-5 of the real one, so a fraction further than 1e-4
+// from a half decides; otherwise (2 values in 10^4) it is taken in f64: |x| and
+// amax have 24 bits, so a quotient up to 127 that is not a tie is at least
+// 2^-33 from one, while the f64 evaluation is off by 2^-43 and the 2^-44 that
+// is added in relative terms (2^-37 at most) lifts exact ties over the half.
+__device__ __forceinline__ int quantize_exact(float x, float amax, float inv, bool fast) {
+  const float t = fabsf(x) * inv;
+  const float f = t - floorf(t);
+  float r = floorf(t + 0.5f);
+  if (!fast || fabsf(f - 0.5f) < 1e-4f) {
+    const double d = static_cast<double>(fabsf(x)) * 127.0 / static_cast<double>(amax);
+    r = static_cast<float>(floor(__fma_rn(d, 0x1p-44, d) + 0.5));
+  }
+  return static_cast<int>(copysignf(r, x));
+}
+
+template <int LPH>
+__global__ __launch_bounds__(kKvNT) void kv_write_kernel(KvArgs a) {
+  constexpr int kGroups = kKvNT / LPH;  // heads a workgroup takes at a time
+  const int si = find_seq(a, blockIdx.x);
+  const KvSeq& sq = a.seq[si];
+  const bool second = blockIdx.y != 0;
+  const float* src = static_cast<const float*>(second ? a.v : a.k);
+  int8_t* dst = static_cast<int8_t*>(second ? sq.v : sq.k);
+  float* scales = second ? sq.vs : sq.ks;
+  const int sub = threadIdx.x % LPH, grp = threadIdx.x / LPH;
+  const bool live = sub * 8u < a.hd;
+  const uint64_t n_items = static_cast<uint64_t>(sq.rows) * a.n_kv;
+  const uint64_t item0 = static_cast<uint64_t>(blockIdx.x - sq.block0) * (kGroups * kItems) + grp;
+  float x[kItems][8];
+#pragma unroll
+  for (int it = 0; it < kItems; it++) {
+    const uint64_t item = item0 + it * kGroups;
+    const uint32_t row = static_cast<uint32_t>(item / a.n_kv), head = static_cast<uint32_t>(item % a.n_kv);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[it][j] = 0.0f;
+    if (item < n_items && live) {
+      const float4* p = reinterpret_cast<const float4*>(src + (static_cast<size_t>(sq.src) + row) * a.ld +
+                                                        static_cast<size_t>(head) * a.hd + sub * 8);
+      const float4 u = p[0], w = p[1];
+      x[it][0] = u.x; x[it][1] = u.y; x[it][2] = u.z; x[it][3] = u.w;
+      x[it][4] = w.x; x[it][5] = w.y; x[it][6] = w.z; x[it][7] = w.w;
+    }
+  }
+#pragma unroll
+  for (int it = 0; it < kItems; it++) {
+    const uint64_t item = item0 + it * kGroups;
+    const uint32_t row = static_cast<uint32_t>(item / a.n_kv), head = static_cast<uint32_t>(item % a.n_kv);
+    // magnitudes as integers: a NaN is then larger than an infinity
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[it][j]) & 0x7fffffffu);
+    top = group_max<LPH>(top);
+    const bool finite = top < 0x7f800000u;
+    const float amax = __uint_as_float(top);
+    float scale = top ? amax / 127.0f : 1.0f;
+    const bool fast = amax > 0x1p-100f;  // scale and its inverse are normal numbers
+    const float inv = 1.0f / scale;
+    if (item >= n_items) continue;
+    uint32_t w[2] = {0, 0};
+    if (finite && top) {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        w[j / 4] |= static_cast<uint32_t>(quantize_exact(x[it][j], amax, inv, fast) & 0xff) << (8 * (j % 4));
+    }
+    if (!finite) scale = __uint_as_float(0x7fc00000u);  // reads back as NaN
+    const size_t r = static_cast<size_t>(sq.first) + row;
+    if (live)
+      *reinterpret_cast<uint2*>(dst + (r * a.n_kv + head) * a.hd + sub * 8) = make_uint2(w[0], w[1]);
+    if (sub == 0) scales[r * a.n_kv + head] = scale;
+  }
+}
+
+template <int LPH, bool HALF>
+__global__ __launch_bounds__(kKvNT) void kv_read_kernel(KvArgs a) {
+  constexpr int kGroups = kKvNT / LPH;
+  const int si = find_seq(a, blockIdx.x);
+  const KvSeq& sq = a.seq[si];
+  const bool second = blockIdx.y != 0;
+  const int8_t* src = static_cast<const int8_t*>(second ? sq.v : sq.k);
+  const float* scales = second ? sq.vs : sq.ks;
+  void* dst = const_cast<void*>(second ? a.v : a.k);
+  const int sub = threadIdx.x % LPH, grp = threadIdx.x / LPH;
+  if (sub * 8u >= a.hd) return;
+  const uint64_t n_items = static_cast<uint64_t>(sq.rows) * a.n_kv;
+  const uint64_t item0 = static_cast<uint64_t>(blockIdx.x - sq.block0) * (kGroups * kItems) + grp;
+  uint2 w[kItems];
+  float scale[kItems];
+#pragma unroll
+  for (int it = 0; it < kItems; it++) {
+    const uint64_t item = item0 + it * kGroups;
+    w[it] = make_uint2(0, 0);
+    scale[it] = 0.0f;
+    if (item < n_items) {
+      const size_t at = static_cast<size_t>(sq.first) * a.n_kv + item;  // (row, head) of the cache
+      w[it] = *reinterpret_cast<const uint2*>(src + at * a.hd + sub * 8);
+      scale[it] = scales[at];
+    }
+  }
+#pragma unroll
+  for (int it = 0; it < kItems; it++) {
+    const uint64_t item = item0 + it * kGroups;
+    if (item >= n_items) continue;
+    const uint32_t row = static_cast<uint32_t>(item / a.n_kv), head = static_cast<uint32_t>(item % a.n_kv);
+    const size_t at = (static_cast<size_t>(sq.src) + row) * a.ld + static_cast<size_t>(head) * a.hd + sub * 8;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t word = j < 4 ? w[it].x : w[it].y;
+      y[j] = static_cast<float>(static_cast<int8_t>(word >> (8 * (j % 4)))) * scale[it];
+    }
+    if constexpr (HALF) {
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        h[j] = static_cast<uint32_t>(f32_to_f16(y[2 * j])) | static_cast<uint32_t>(f32_to_f16(y[2 * j + 1])) << 16;
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst) + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    } else {
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(dst) + at);
+      o[0] = make_float4(y[0], y[1], y[2], y[3]);
+      o[1] = make_float4(y[4], y[5], y[6], y[7]);
+    }
+  }
+}
+
+// Lanes of a head: the power of two that holds its 8-value pieces.
+int lanes_per_head(size_t hd) {
+  int n = 1;
+  while (n * 8 < static_cast<int>(hd)) n *= 2;
+  return n;
+}
+
+enum class Move { kWrite, kRead32, kRead16 };
+
+template <int LPH>
+void launch_move(Move m, const KvArgs& a, uint32_t blocks, hipStream_t s) {
+  const dim3 grid(blocks, 2), nt(kKvNT);
+  if (m == Move::kWrite)
+    hipLaunchKernelGGL((kv_write_kernel<LPH>), grid, nt, 0, s, a);
+  else if (m == Move::kRead32)
+    hipLaunchKernelGGL((kv_read_kernel<LPH, false>), grid, nt, 0, s, a);
+  else
+    hipLaunchKernelGGL((kv_read_kernel<LPH, true>), grid, nt, 0, s, a);
+}
+
+int launch_moves(Move m, const void* k, const void* v, size_t ld, const prana_kv* kv, const size_t* first_rows,
+                 const size_t* n_rows, size_t n_seq, size_t n_kv, size_t hd, hipStream_t s) {
+  const int lph = lanes_per_head(hd);
+  const size_t per_block = static_cast<size_t>(kKvNT / lph) * kItems;
+  KvArgs a{};
+  a.k = k;
+  a.v = v;
+  a.ld = ld;
+  a.n_kv = static_cast<uint32_t>(n_kv);
+  a.hd = static_cast<uint32_t>(hd);
+  size_t src = 0, blocks = 0;
+  auto flush = [&]() -> int {
+    if (blocks == 0) return kOk;
+    const uint32_t b = static_cast<uint32_t>(blocks);
+    switch (lph) {
+      case 1: launch_move<1>(m, a, b, s); break;
+      case 2: launch_move<2>(m, a, b, s); break;
+      case 4: launch_move<4>(m, a, b, s); break;
+      case 8: launch_move<8>(m, a, b, s); break;
+      case 16: launch_move<16>(m, a, b, s); break;
+      default: launch_move<32>(m, a, b, s); break;
+    }
+    PRANA_LAUNCH_CHECK();
+    a.n_seq = 0;
+    blocks = 0;
+    return kOk;
+  };
+  for (size_t i = 0; i < n_seq; i++) {
+    // a launch's grid stays far from 2^31 workgroups: long sequences go in parts
+    constexpr size_t kPartBlocks = size_t{1} << 24;
+    const size_t part = std::max<size_t>(1, kPartBlocks * per_block / n_kv);
+    for (size_t r = 0; r < n_rows[i]; r += part) {
+      const size_t rows = std::min(part, n_rows[i] - r);
+      if (a.n_seq == kKvSeqs || blocks > kPartBlocks)
+        if (int rc = flush()) return rc;
+      KvSeq& q = a.seq[a.n_seq++];
+      q.k = kv[i].k;
+      q.v = kv[i].v;
+      q.ks = kv[i].k_scales;
+      q.vs = kv[i].v_scales;
+      q.src = static_cast<uint32_t>(src + r);
+      q.rows = static_cast<uint32_t>(rows);
+      q.first = static_cast<uint32_t>(first_rows[i] + r);
+      q.block0 = static_cast<uint32_t>(blocks);
+      blocks += (rows * n_kv + per_block - 1) / per_block;
+    }
+    src += n_rows[i];
+  }
+  return flush();
+}
+
+}  // namespace
+
+int launch_kv_write_q8(const float* k, const float* v, size_t ld, const prana_kv* kv, const size_t* first_rows,
+                       const size_t* n_rows, size_t n_seq, size_t n_kv_heads, size_t head_dim, hipStream_t s) {
+  return launch_moves(Move::kWrite, k, v, ld, kv, first_rows, n_rows, n_seq, n_kv_heads, head_dim, s);
+}
+
+int launch_kv_read_q8(const prana_kv* kv, const size_t* first_rows, const size_t* n_rows, size_t n_seq,
+                      size_t n_kv_heads, size_t head_dim, bool half, void* k, void* v, size_t ld, hipStream_t s) {
+  return launch_moves(half ? Move::kRead16 : Move::kRead32, k, v, ld, kv, first_rows, n_rows, n_seq, n_kv_heads,
+                      head_dim, s);
+}
+
+}  // namespace prana
