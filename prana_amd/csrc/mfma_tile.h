@@ -1,0 +1,74 @@
+// Pieces the matrix-core attention kernels share: operand types, the
+// transposing LDS read, conversions to halves.
+//
+// Operands of v_mfma_f32_32x32x16_f16, lane l, h = l / 32: A (m = l % 32) and
+// B (n = l % 32) hold k = 8h .. 8h+7; C holds n = l % 32 and, in register i,
+// m = 8 (i / 4) + 4h + i % 4. Of v_mfma_f32_16x16x32_f16, g = l / 16: A and B
+// hold k = 8g .. 8g+7 of row or column l % 16; C holds n = l % 16 and, in
+// register i, m = 4g + i. Both take f16 subnormals as they are.
+#pragma once
+
+#include "common.h"
+
+namespace prana {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Transposing LDS read of halves: the 16 lanes of a group read 4 rows of 16
+// (lane l the four at row l / 4, column 4 (l % 4)), and lane l gets column l,
+// rows 0..3.
+__device__ __forceinline__ half4 lds_read_tr(const uint16_t* p) {
+  typedef __attribute__((address_space(3))) short4v* lds_ptr;
+  const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+  return __builtin_bit_cast(half4, v);
+}
+
+__device__ __forceinline__ half8 join(half4 a, half4 b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// 2^x as the hardware computes it (1 ulp; results under 2^-126 are 0).
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Whether one of the two halves in w is an infinity or NaN.
+__device__ __forceinline__ bool pair_not_finite(uint32_t w) {
+  return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+}
+__device__ __forceinline__ bool any_not_finite(const uint4& v) {
+  return pair_not_finite(v.x) || pair_not_finite(v.y) || pair_not_finite(v.z) || pair_not_finite(v.w);
+}
+// w with its halves that are not finite replaced by 0.
+__device__ __forceinline__ uint32_t pair_finite(uint32_t w) {
+  if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
+  if ((w & 0x7c000000u) == 0x7c000000u) w &= 0x0000ffffu;
+  return w;
+}
+__device__ __forceinline__ uint4 only_finite(const uint4& v) {
+  return make_uint4(pair_finite(v.x), pair_finite(v.y), pair_finite(v.z), pair_finite(v.w));
+}
+
+// An f32 as two halves, x = hi + lo to 22 bits (|x| under 65504; lo has steps
+// of at least 2^-24). x is opaque here: a product that feeds it would be fused
+// with the rounding to hi, but not with the one to lo, and the two would not
+// belong together where the product lies near a tie.
+__device__ __forceinline__ void split_half(float x, _Float16& hi, _Float16& lo) {
+  asm("" : "+v"(x));
+  hi = static_cast<_Float16>(x);
+  lo = static_cast<_Float16>(x - static_cast<float>(hi));
+}
+
+// The power of two that brings amax into [2^9, 2^10), where both halves of a
+// split are far from their limits; 1 where amax is 0 or not finite.
+__device__ __forceinline__ float row_factor(float amax) {
+  const uint32_t e = __float_as_uint(amax) >> 23;
+  if (e == 0u || e == 255u) return amax > 0.0f && e == 0u ? 0x1p126f : 1.0f;
+  const int k = 9 + 127 - static_cast<int>(e);
+  return __builtin_ldexpf(1.0f, k < -126 ? -126 : k > 126 ? 126 : k);
+}
+
+}  // namespace prana
