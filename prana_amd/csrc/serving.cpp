@@ -125,6 +125,7 @@ int check_attention_tree(const float* q, int kv_type, const prana_kv* kv, const 
   if (!aligned(q, 16) || !aligned(out, 16)) return refuse(what, "q and out must be 16-byte aligned");
   if (!aligned(mask, 8)) return refuse(what, "mask must be 8-byte aligned");
   const size_t need = attention_tree_floats(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim) * sizeof(float);
+  if (need > (size_t{1} << 42)) return refuse(what, "too many drafted tokens over too long caches");
   if (need && !workspace) return refuse(what, "null workspace");
   if (!aligned(workspace, 16)) return refuse(what, "workspace must be 16-byte aligned");
   if (workspace_bytes < need)

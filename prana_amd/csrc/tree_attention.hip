@@ -1,103 +1,910 @@
 // Attention of drafted tokens over the caches of several sequences
-// (prana_attention_tree). Drafted token i of a sequence with n rows in its
-// cache sees row t when t < n or bit t - n of its mask word is set.
-// One wave per drafted token and head.
+// (prana_attention_tree). Drafted token i of a sequence whose cache holds
+// `past` rows before the drafted ones sees row t when t < past or bit t - past
+// of its mask word is set:
+//   o_i = sum_t p_it v_t,  p_i = softmax over the seen t of q_i . k_t / sqrt(w).
+//
+// The rows of a sequence are its (drafted token, query head of the group)
+// pairs, so a KV head's cache is read once for all of them. The cache rows are
+// split over workgroups; each leaves its rows' maximum, sum and weighted sum,
+// which a second launch joins (a sequence that one part holds needs none).
+// All products run on the f16 matrix cores: q * log2(e)/sqrt(w), normalised
+// per row by a power of two, and the probabilities go in as two halves each
+// (22 bits); f16 and i8 cache values are halves exactly. An 8-bit row's K scale
+// multiplies its scores, its V scale its probabilities.
+//
+// Two kernels, by the rows of a sequence and KV head:
+//   narrow (up to 32 rows): bound by reading the cache. The four waves of a
+//     workgroup share the rows and take different keys, 32 at a time: K goes
+//     from memory straight into the operand's registers, V through a corner of
+//     LDS that only its wave uses, so no wave waits for another until the end.
+//   wide (more rows): bound by the products. Four waves of 32 rows share tiles
+//     of 64 keys in LDS.
+// In both S^T = K Q^T leaves a row's scores in the lanes of one column, whose
+// registers are, as halves, the operand of O^T += V^T P^T; V comes out of LDS
+// transposed to match. The kept maximum lags the scores by up to 2^8 before
+// the sums are rescaled.
 #include <algorithm>
+#include <cmath>
+#include <vector>
 
 #include "common.h"
+#include "mfma_tile.h"
 #include "serving.h"
 
 namespace prana {
 
 namespace {
 
-constexpr int kTrSeqs = 64;
+constexpr int kTrSeqs = 64;  // sequences of one launch
+constexpr int kTrNT = 256;
+constexpr float kLag = 8.0f;
+constexpr float kPShift = 7.0f;  // probabilities are kept times 2^7, at most 2^15
 
 struct TreeSeq {
   const void *k, *v;
   const float *ks, *vs;
-  uint32_t past, tok0, tokens;
+  uint32_t past, tokens;
+  uint32_t tok0;    // first drafted token in q, mask and out
+  uint32_t item0;   // first work item of the sequence
+  uint32_t splits;  // parts of the cache rows
+  uint32_t part0;   // first partial state, in rows (a sequence holds tokens * n_heads * splits)
 };
 
 struct TreeArgs {
   const float* q;
   const uint64_t* mask;
   float* out;
-  uint32_t n_heads, n_kv, group, hd;
-  float scale;
+  float* part;  // [partial row][hd] weighted sums, then [partial row][2] maximum and sum
+  size_t part_rows;
+  uint32_t n_seq, n_heads, n_kv, group, hd;
+  uint32_t rows_per_split;
+  float scale;  // log2(e) / sqrt(hd)
   TreeSeq seq[kTrSeqs];
 };
 
+__device__ __forceinline__ int find_seq(const TreeArgs& a, uint32_t item) {
+  int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.seq[mid].item0 <= item)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// The mask word of drafted token i, cut to the sequence's tokens.
+__device__ __forceinline__ uint64_t mask_word(const TreeArgs& a, const TreeSeq& sq, uint32_t i) {
+  const uint64_t own = sq.tokens >= 64 ? ~0ull : (1ull << sq.tokens) - 1;
+  return (a.mask ? a.mask[sq.tok0 + i] : (2ull << i) - 1) & own;
+}
+
+// Bit j: key first + j is seen (first - past keys lie before the drafted ones).
+__device__ __forceinline__ uint64_t seen_from(uint64_t word, int first_minus_past) {
+  if (first_minus_past >= 64) return 0;
+  if (first_minus_past >= 0) return word >> first_minus_past;
+  if (first_minus_past <= -64) return ~0ull;
+  return word << -first_minus_past | ((1ull << -first_minus_past) - 1);
+}
+
+// Eight i8 values as halves: u = v + 128 in the low bits of 0x6400 is the half
+// 1024 + u, and 1152 off that is v.
+__device__ __forceinline__ uint4 i8_to_halves(uint2 w) {
+  const uint32_t u[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t b = u[j / 2];
+    const uint32_t pair = __builtin_amdgcn_perm(0x64646464u, b, j % 2 ? 0x04030402u : 0x04010400u);
+    const half2v x = __builtin_bit_cast(half2v, pair) - half2v{1152.0f16, 1152.0f16};
+    o[j] = __builtin_bit_cast(uint32_t, x);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Eight values of a cache row as loaded, and as halves.
 template <bool Q8>
-__global__ __launch_bounds__(64) void tree_kernel(TreeArgs a) {
-  const TreeSeq& sq = a.seq[blockIdx.z];
-  const uint32_t i = blockIdx.x, lane = threadIdx.x;
-  if (i >= sq.tokens) return;
-  const uint32_t head = blockIdx.y, kvh = head / a.group;
-  const bool live = lane * 4 < a.hd;
-  const size_t at = ((static_cast<size_t>(sq.tok0) + i) * a.n_heads + head) * a.hd + lane * 4;
-  const uint64_t own = sq.tokens == 64 ? ~0ull : (1ull << sq.tokens) - 1;
-  const uint64_t bits = (a.mask ? a.mask[sq.tok0 + i] : (2ull << i) - 1) & own;
-  float q[4] = {}, acc[4] = {}, m = -INFINITY, l = 0.0f;
-  if (live)
-    for (int j = 0; j < 4; j++) q[j] = a.q[at + j];
-  for (uint32_t t = 0; t < sq.past + sq.tokens; t++) {
-    if (t >= sq.past && !((bits >> (t - sq.past)) & 1)) continue;
-    const size_t row = static_cast<size_t>(t) * a.n_kv + kvh, kt = row * a.hd + lane * 4;
-    float s = 0.0f, v[4] = {};
-    if (live)
-      for (int j = 0; j < 4; j++) {
-        if constexpr (Q8) {
-          s = fmaf(q[j], static_cast<float>(static_cast<const int8_t*>(sq.k)[kt + j]), s);
-          v[j] = static_cast<float>(static_cast<const int8_t*>(sq.v)[kt + j]) * sq.vs[row];
-        } else {
-          s = fmaf(q[j], f16_operand(static_cast<const uint16_t*>(sq.k)[kt + j]), s);
-          v[j] = f16_operand(static_cast<const uint16_t*>(sq.v)[kt + j]);
+struct Piece {
+  uint4 w;
+  __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const void* base, size_t at) {
+    w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
+  }
+  __device__ __forceinline__ uint4 halves() const { return w; }
+};
+template <>
+struct Piece<true> {
+  uint2 w;
+  __device__ __forceinline__ void zero() { w = make_uint2(0, 0); }
+  __device__ __forceinline__ void load(const void* base, size_t at) {
+    w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(base) + at);
+  }
+  __device__ __forceinline__ uint4 halves() const { return i8_to_halves(w); }
+};
+
+// A row's q as the score product's operand: PIECES pieces of 8 dims, piece s
+// at dim s * STEP + d0, as two halves, normalised. Returns the factor that
+// brings the scores back (a power of two). LANES: lanes (a power of two apart)
+// that hold one row.
+template <int PIECES, int STEP, int LANES>
+__device__ __forceinline__ float load_q(const float* qp, uint32_t d0, uint32_t hd, float scale, half8* qh, half8* ql) {
+  float amax = 0.0f;
+  float x[PIECES][8];
+#pragma unroll
+  for (int s = 0; s < PIECES; s++) {
+    const uint32_t d = s * STEP + d0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[s][j] = 0.0f;
+    if (d < hd) {
+      const float4 u = *reinterpret_cast<const float4*>(qp + d), w = *reinterpret_cast<const float4*>(qp + d + 4);
+      x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
+      x[s][4] = w.x; x[s][5] = w.y; x[s][6] = w.z; x[s][7] = w.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[s][j]));
+  }
+#pragma unroll
+  for (int o = 64 / LANES; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+  const float f = row_factor(amax);
+#pragma unroll
+  for (int s = 0; s < PIECES; s++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      _Float16 xh, xl;
+      split_half(x[s][j] * f * scale, xh, xl);
+      qh[s][j] = xh;
+      ql[s][j] = xl;
+    }
+  return 1.0f / f;
+}
+
+// V scales of 8-bit caches are taken relative to a power of two no smaller
+// than any scale met so far, so that a probability times its scale stays below
+// 2^15 as the probability does.
+struct ScaleTop {
+  float top = 0x1p-100f, inv = 0x1p100f;
+  // v: this lane's scales of the tile. The factor for what was summed before.
+  __device__ __forceinline__ float raise(float v) {
+    float big = fabsf(v) < INFINITY ? fabsf(v) : 0.0f;
+    big = wave_max_f32(big);
+    if (!(big > top)) return 1.0f;
+    const uint32_t e = min((__float_as_uint(big) >> 23) + 1, 253u);
+    const float nt = __uint_as_float(e << 23), f = top / nt;
+    top = nt;
+    inv = 1.0f / nt;
+    return f;
+  }
+};
+
+// ------------------------------------------------------------ narrow: up to 16 RB rows
+template <int HDP>
+struct NarrowShape {
+  static constexpr int kSteps = HDP / 32, kDimBlocks = HDP / 16, kPieces = HDP / 16;
+  // V rows an odd multiple of 32 bytes apart: the 32-byte pieces of 8 rows
+  // that a transposing read takes at a time fall on different banks
+  static constexpr int kLdV = HDP + 16;
+  static constexpr int kWaveHalves = 32 * kLdV;
+  static constexpr int kLdO = HDP + 4;  // joining the waves: floats per row
+  static constexpr int kBytes = std::max(4 * kWaveHalves * 2, 4 * 16 * kLdO * 4);
+};
+
+template <int HDP, int RB, bool Q8>
+__global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
+  using S = NarrowShape<HDP>;
+  __shared__ __attribute__((aligned(16))) unsigned char s_mem[S::kBytes];
+  __shared__ __attribute__((aligned(16))) float s_scale[4][64];  // per wave: K scales of 32 keys, V scales
+  __shared__ float s_m[4][16 * RB], s_l[4][16 * RB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = lane & 15, g = lane >> 4;
+  uint16_t* s_v = reinterpret_cast<uint16_t*>(s_mem) + wave * S::kWaveHalves;
+  const uint32_t kvh = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
+  const TreeSeq& sq = a.seq[find_seq(a, item)];
+  const uint32_t split = item - sq.item0, hd = a.hd;
+  const uint32_t rows = sq.tokens * a.group, total = sq.past + sq.tokens;
+  const uint32_t kbeg = split * a.rows_per_split, kend = min(total, kbeg + a.rows_per_split);
+
+  half8 qh[RB][S::kSteps], ql[RB][S::kSteps];
+  float c[RB], m[RB], l[RB];
+  uint64_t word[RB];
+  f32x4 o[RB][S::kDimBlocks];
+#pragma unroll
+  for (int r = 0; r < RB; r++) {
+    const uint32_t row = min(r * 16u + n, rows - 1), i = row / a.group;
+    const size_t at = (static_cast<size_t>(sq.tok0) + i) * a.n_heads + kvh * a.group + row % a.group;
+    c[r] = load_q<S::kSteps, 32, 4>(a.q + at * hd, g * 8, hd, a.scale, qh[r], ql[r]);
+    word[r] = mask_word(a, sq, i);
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[r][mb][j] = 0.0f;
+  }
+  ScaleTop top;
+
+  const size_t ld = static_cast<size_t>(a.n_kv) * hd, head = static_cast<size_t>(kvh) * hd;
+  Piece<Q8> kr[2][S::kSteps], vr[S::kPieces];
+  float sc = 0.0f;  // lanes 0-31: K scale of key lane; 32-63: V scale of key lane - 32
+  auto fetch = [&](uint32_t k0) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const uint32_t t = min(k0 + b * 16 + n, kend - 1);  // (keys past the end repeat the last and are masked)
+#pragma unroll
+      for (int s = 0; s < S::kSteps; s++) {
+        const uint32_t d = s * 32 + g * 8;
+        kr[b][s].zero();
+        if (d < hd) kr[b][s].load(sq.k, t * ld + head + d);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < S::kPieces; p++) {
+      const int e = p * 64 + lane;
+      const uint32_t t = k0 + e / (HDP / 8), d = (e % (HDP / 8)) * 8;
+      vr[p].zero();
+      if (t < kend && d < hd) vr[p].load(sq.v, t * ld + head + d);
+    }
+    if constexpr (Q8) {
+      const uint32_t t = k0 + (lane & 31);
+      sc = 0.0f;
+      if (t < kend) sc = (lane < 32 ? sq.ks : sq.vs)[static_cast<size_t>(t) * a.n_kv + kvh];
+    }
+  };
+  uint32_t k0 = kbeg + wave * 32;
+  if (k0 < kend) fetch(k0);
+  for (; k0 < kend; k0 += 128) {
+    const bool edge = k0 + 32 > min(sq.past, kend);  // not every row sees every key
+    bool odd = false;
+    if constexpr (!Q8) {
+      // a V value that is not finite must not meet the zero probability of a
+      // row that does not see it: it is left out and added below
+      if (edge) {
+#pragma unroll
+        for (int p = 0; p < S::kPieces; p++) odd = odd || any_not_finite(vr[p].w);
+        odd = __any(odd);
+        if (odd) {
+#pragma unroll
+          for (int p = 0; p < S::kPieces; p++) vr[p].w = only_finite(vr[p].w);
         }
       }
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    s *= a.scale;
-    if constexpr (Q8) s *= sq.ks[row];
-    const float mn = fmaxf(m, s), al = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
-    l = fmaf(l, al, p);
-    for (int j = 0; j < 4; j++) acc[j] = fmaf(acc[j], al, p * v[j]);
-    m = mn;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the reads of the keys before come first)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int p = 0; p < S::kPieces; p++) {
+      const int e = p * 64 + lane;
+      *reinterpret_cast<uint4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vr[p].halves();
+    }
+    if constexpr (Q8) {
+      s_scale[wave][lane] = sc;
+      const float v = lane < 32 ? 0.0f : sc;
+      if (__any(fabsf(v) > top.top)) {
+        const float f = top.raise(v);
+#pragma unroll
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+          for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[r][mb][j] *= f;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+
+    f32x4 s[RB][2];
+#pragma unroll
+    for (int r = 0; r < RB; r++)
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[r][b][j] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int t = 0; t < S::kSteps; t++) {
+        const half8 kf = __builtin_bit_cast(half8, kr[b][t].halves());
+#pragma unroll
+        for (int r = 0; r < RB; r++) {
+          s[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[r][t], s[r][b], 0, 0, 0);
+          s[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[r][t], s[r][b], 0, 0, 0);
+        }
+      }
+    const uint32_t kcur = k0;
+    if (k0 + 128 < kend) fetch(k0 + 128);
+
+    float ks[2][4], vs[2][4];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const float4 x = *reinterpret_cast<const float4*>(&s_scale[wave][b * 16 + 4 * g]);
+        const float4 y = *reinterpret_cast<const float4*>(&s_scale[wave][32 + b * 16 + 4 * g]);
+        ks[b][0] = x.x; ks[b][1] = x.y; ks[b][2] = x.z; ks[b][3] = x.w;
+        vs[b][0] = y.x; vs[b][1] = y.y; vs[b][2] = y.z; vs[b][3] = y.w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) vs[b][j] *= top.inv;
+      }
+    }
+    half8 ph[RB], pl[RB];
+#pragma unroll
+    for (int r = 0; r < RB; r++) {
+      if constexpr (Q8) {
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[r][b][j] *= ks[b][j];
+      }
+      uint32_t seen = ~0u;  // bit 16 b + j: this row sees key b * 16 + 4g + j
+      if (edge) {
+        const int first = static_cast<int>(kcur + 4 * g);
+        seen = static_cast<uint32_t>(seen_from(word[r], first - static_cast<int>(sq.past)));
+        const int left = static_cast<int>(kend) - first;  // keys before the end of this part
+        seen &= left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (!(seen >> (b * 16 + j) & 1)) s[r][b][j] = -INFINITY;
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
+                       fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c[r];
+      if (__any(mx > m[r] + kLag)) {
+        const float mn = fmaxf(m[r], mx);
+        const float al = mn == -INFINITY ? 1.0f : exp2_hw(m[r] - mn);  // (a row that has seen nothing yet)
+        m[r] = mn;
+        l[r] *= al;
+#pragma unroll
+        for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) o[r][mb][j] *= al;
+      }
+      const float ms = m[r] == -INFINITY ? 0.0f : m[r] - kPShift;
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          float p = exp2_hw(fmaf(s[r][b][j], c[r], -ms));
+          l[r] += p;
+          if constexpr (Q8) {
+            p *= vs[b][j];
+            if (edge && !(seen >> (b * 16 + j) & 1)) p = 0.0f;  // (its scale may be NaN)
+          }
+          _Float16 xh, xl;
+          split_half(p, xh, xl);
+          ph[r][b * 4 + j] = xh;
+          pl[r][b * 4 + j] = xl;
+        }
+    }
+    const uint16_t* vp = s_v + (4 * g + (n >> 2)) * S::kLdV + (n & 3) * 4;
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++) {
+      const half8 vf = join(lds_read_tr(vp + mb * 16), lds_read_tr(vp + 16 * S::kLdV + mb * 16));
+#pragma unroll
+      for (int r = 0; r < RB; r++) {
+        o[r][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[r], o[r][mb], 0, 0, 0);
+        o[r][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[r], o[r][mb], 0, 0, 0);
+      }
+    }
+    if (odd) {  // rare
+      for (uint32_t t = kcur; t < min(kcur + 32, kend); t++)
+#pragma unroll
+        for (int mb = 0; mb < S::kDimBlocks; mb++) {
+          const uint32_t d = mb * 16 + 4 * g;
+          if (d >= hd) continue;
+          const half4 x = *reinterpret_cast<const half4*>(static_cast<const uint16_t*>(sq.v) + t * ld + head + d);
+#pragma unroll
+          for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float v = static_cast<float>(x[j]);
+              if (!(fabsf(v) < INFINITY) && (seen_from(word[r], static_cast<int>(t) - static_cast<int>(sq.past)) & 1))
+                o[r][mb][j] += v;
+            }
+        }
+    }
   }
-  if (live)
-    for (int j = 0; j < 4; j++) a.out[at + j] = l == 0.0f ? 0.0f : acc[j] / l;
+
+  // join the waves
+#pragma unroll
+  for (int r = 0; r < RB; r++) {
+    l[r] += __shfl_xor(l[r], 16, 64);
+    l[r] += __shfl_xor(l[r], 32, 64);
+    if (g == 0) {
+      s_m[wave][r * 16 + n] = m[r];
+      s_l[wave][r * 16 + n] = l[r];
+    }
+  }
+  __syncthreads();  // (and every wave is done with its part of s_mem)
+  float* s_o = reinterpret_cast<float*>(s_mem);
+#pragma unroll
+  for (int r = 0; r < RB; r++) {
+    if (r) __syncthreads();
+    const int i = r * 16 + n;
+    const float M = fmaxf(fmaxf(s_m[0][i], s_m[1][i]), fmaxf(s_m[2][i], s_m[3][i]));
+    float f = m[r] == -INFINITY ? 0.0f : exp2_hw(m[r] - M);
+    if constexpr (Q8) f *= top.top;
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++) {
+      // a wave that saw nothing of this row holds zeros
+      *reinterpret_cast<float4*>(s_o + (wave * 16 + n) * S::kLdO + mb * 16 + 4 * g) =
+          make_float4(o[r][mb][0] * f, o[r][mb][1] * f, o[r][mb][2] * f, o[r][mb][3] * f);
+    }
+    __syncthreads();
+    for (int e = tid; e < 16 * (HDP / 4); e += kTrNT) {
+      const int rr = e / (HDP / 4);
+      const uint32_t d = (e % (HDP / 4)) * 4, row = r * 16 + rr;
+      if (row >= rows || d >= hd) continue;
+      float4 y = make_float4(0, 0, 0, 0);
+      const int ri = r * 16 + rr;
+      const float top_m = fmaxf(fmaxf(s_m[0][ri], s_m[1][ri]), fmaxf(s_m[2][ri], s_m[3][ri]));
+      float L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 16 + rr) * S::kLdO + d);
+        y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+        if (s_m[w][ri] != -INFINITY) L = fmaf(s_l[w][ri], exp2_hw(s_m[w][ri] - top_m), L);
+      }
+      const size_t qrow = static_cast<size_t>(row / a.group) * a.n_heads + kvh * a.group + row % a.group;
+      if (sq.splits == 1) {
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // (L is 0 where the row sees nothing)
+        *reinterpret_cast<float4*>(a.out + (static_cast<size_t>(sq.tok0) * a.n_heads + qrow) * hd + d) =
+            make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+      } else {
+        const size_t pr = sq.part0 + qrow * sq.splits + split;
+        *reinterpret_cast<float4*>(a.part + pr * hd + d) = y;
+        if (d == 0) {
+          float* ml = a.part + a.part_rows * hd + pr * 2;
+          ml[0] = top_m;
+          ml[1] = L;
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ wide: 128 rows a workgroup
+constexpr int kWideRows = 128;
+
+template <int HDP, int BN>
+struct WideShape {
+  static constexpr int kStepsQK = HDP / 16, kDimBlocks = HDP / 32, kKeyBlocks = BN / 32;
+  static constexpr int kChunks = HDP / 8;
+  static constexpr int kLdK = HDP + 8;                             // as in the packed prompts' kernel
+  static constexpr int kLdV = HDP % 128 == 96 ? HDP : HDP + 32;
+  static constexpr int kLoads = BN * kChunks / kTrNT;
+};
+
+template <int HDP, int BN, bool Q8>
+__global__ __launch_bounds__(kTrNT, HDP <= 96 ? 2 : 1) void tree_wide_kernel(TreeArgs a) {
+  using S = WideShape<HDP, BN>;
+  static_assert(BN * S::kChunks % kTrNT == 0, "a tile is a whole number of pieces per lane");
+  __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[BN * S::kLdV];
+  __shared__ __attribute__((aligned(16))) float s_scale[2][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = lane & 31, h = lane >> 5;
+  const uint32_t kvh = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
+  const TreeSeq& sq = a.seq[find_seq(a, item)];
+  const uint32_t hd = a.hd, rows = sq.tokens * a.group, total = sq.past + sq.tokens;
+  const uint32_t row_tiles = (rows + kWideRows - 1) / kWideRows;
+  const uint32_t split = (item - sq.item0) / row_tiles, row0 = (item - sq.item0) % row_tiles * kWideRows;
+  const uint32_t kbeg = split * a.rows_per_split, kend = min(total, kbeg + a.rows_per_split);
+  const bool idle = row0 + wave * 32 >= rows;  // the wave has no rows: it only stages
+  const uint32_t row = min(row0 + wave * 32 + n, rows - 1), i = row / a.group;
+  const size_t qrow = static_cast<size_t>(i) * a.n_heads + kvh * a.group + row % a.group;
+  const uint64_t word = mask_word(a, sq, i);
+
+  half8 qh[S::kStepsQK], ql[S::kStepsQK];
+  const float c = load_q<S::kStepsQK, 16, 2>(a.q + (static_cast<size_t>(sq.tok0) * a.n_heads + qrow) * hd, h * 8, hd,
+                                             a.scale, qh, ql);
+  f32x16 o[S::kDimBlocks];
+#pragma unroll
+  for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+    for (int j = 0; j < 16; j++) o[mb][j] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  ScaleTop top;
+
+  const size_t ld = static_cast<size_t>(a.n_kv) * hd, head = static_cast<size_t>(kvh) * hd;
+  Piece<Q8> kr[S::kLoads], vr[S::kLoads];
+  float sc = 0.0f;  // lanes 0..BN-1: K scale of key lane; BN..2BN-1: V scales
+  auto fetch = [&](uint32_t k0) {
+#pragma unroll
+    for (int p = 0; p < S::kLoads; p++) {
+      const int e = p * kTrNT + tid;
+      const uint32_t t = k0 + e / S::kChunks, d = (e % S::kChunks) * 8;
+      kr[p].zero();
+      vr[p].zero();
+      if (t < kend && d < hd) {
+        kr[p].load(sq.k, t * ld + head + d);
+        vr[p].load(sq.v, t * ld + head + d);
+      }
+    }
+    if constexpr (Q8) {
+      const uint32_t t = k0 + tid % BN;
+      sc = 0.0f;
+      if (tid < 2 * BN && t < kend) sc = (tid < BN ? sq.ks : sq.vs)[static_cast<size_t>(t) * a.n_kv + kvh];
+    }
+  };
+  fetch(kbeg);
+  for (uint32_t k0 = kbeg; k0 < kend; k0 += BN) {
+    const bool edge = k0 + BN > min(sq.past, kend);
+    bool odd = false;
+    if (!Q8 && edge) {
+      if constexpr (!Q8) {
+#pragma unroll
+        for (int p = 0; p < S::kLoads; p++) odd = odd || any_not_finite(vr[p].w);
+        odd = __syncthreads_or(odd);
+        if (odd) {
+#pragma unroll
+          for (int p = 0; p < S::kLoads; p++) vr[p].w = only_finite(vr[p].w);
+        }
+      }
+    } else {
+      __syncthreads();
+    }
+#pragma unroll
+    for (int p = 0; p < S::kLoads; p++) {
+      const int e = p * kTrNT + tid;
+      const int r = e / S::kChunks, d = (e % S::kChunks) * 8;
+      *reinterpret_cast<uint4*>(s_k + r * S::kLdK + d) = kr[p].halves();
+      *reinterpret_cast<uint4*>(s_v + r * S::kLdV + d) = vr[p].halves();
+    }
+    if constexpr (Q8) {
+      if (tid < 2 * BN) s_scale[tid / BN][tid % BN] = sc;
+    }
+    __syncthreads();
+    if (k0 + BN < kend) fetch(k0 + BN);
+    if (idle) continue;
+
+    f32x16 s[S::kKeyBlocks];
+#pragma unroll
+    for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) s[b][j] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < S::kStepsQK; t++)
+#pragma unroll
+      for (int b = 0; b < S::kKeyBlocks; b++) {
+        const half8 kf = *reinterpret_cast<const half8*>(s_k + (b * 32 + n) * S::kLdK + t * 16 + h * 8);
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[t], s[b], 0, 0, 0);
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[t], s[b], 0, 0, 0);
+      }
+    if constexpr (Q8) {
+      const float v = lane < BN ? s_scale[1][lane] : 0.0f;
+      if (__any(fabsf(v) > top.top)) {
+        const float f = top.raise(v);
+#pragma unroll
+        for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+          for (int j = 0; j < 16; j++) o[mb][j] *= f;
+      }
+#pragma unroll
+      for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const float4 x = *reinterpret_cast<const float4*>(&s_scale[0][b * 32 + 8 * g + 4 * h]);
+          s[b][4 * g] *= x.x;
+          s[b][4 * g + 1] *= x.y;
+          s[b][4 * g + 2] *= x.z;
+          s[b][4 * g + 3] *= x.w;
+        }
+    }
+    uint64_t seen = ~0ull;  // bit j: this row sees key k0 + 4h + j
+    if (edge) {
+      const int first = static_cast<int>(k0 + 4 * h);
+      seen = seen_from(word, first - static_cast<int>(sq.past));
+      const int left = static_cast<int>(kend) - first;
+      seen &= left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+#pragma unroll
+      for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+          if (!(seen >> (b * 32 + 8 * (j / 4) + j % 4) & 1)) s[b][j] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+    if (__any(mx > m + kLag)) {
+      const float mn = fmaxf(m, mx);
+      const float al = mn == -INFINITY ? 1.0f : exp2_hw(m - mn);
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) o[mb][j] *= al;
+    }
+    const float ms = m == -INFINITY ? 0.0f : m - kPShift;
+#pragma unroll
+    for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        half8 ph, pl;
+#pragma unroll
+        for (int gg = 0; gg < 2; gg++) {
+          float4 vs = make_float4(1, 1, 1, 1);
+          if constexpr (Q8) vs = *reinterpret_cast<const float4*>(&s_scale[1][b * 32 + 16 * t + 8 * gg + 4 * h]);
+          const float v4[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int reg = t * 8 + gg * 4 + j;
+            float p = exp2_hw(fmaf(s[b][reg], c, -ms));
+            l += p;
+            if constexpr (Q8) {
+              p *= v4[j] * top.inv;
+              if (edge && !(seen >> (b * 32 + 8 * (reg / 4) + reg % 4) & 1)) p = 0.0f;
+            }
+            _Float16 xh, xl;
+            split_half(p, xh, xl);
+            ph[gg * 4 + j] = xh;
+            pl[gg * 4 + j] = xl;
+          }
+        }
+        const uint16_t* vp = s_v + (b * 32 + t * 16 + 4 * h + ((lane & 15) >> 2)) * S::kLdV +
+                             ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+        for (int mb = 0; mb < S::kDimBlocks; mb++) {
+          const half8 vf = join(lds_read_tr(vp + mb * 32), lds_read_tr(vp + 8 * S::kLdV + mb * 32));
+          o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, o[mb], 0, 0, 0);
+          o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[mb], 0, 0, 0);
+        }
+      }
+    if (odd) {  // rare
+      for (uint32_t t = k0; t < min(k0 + BN, kend); t++) {
+        if (!(seen_from(word, static_cast<int>(t) - static_cast<int>(sq.past)) & 1)) continue;
+#pragma unroll
+        for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const uint32_t d = mb * 32 + 8 * g + 4 * h;
+            if (d >= hd) continue;
+            const half4 x = *reinterpret_cast<const half4*>(static_cast<const uint16_t*>(sq.v) + t * ld + head + d);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float v = static_cast<float>(x[j]);
+              if (!(fabsf(v) < INFINITY)) o[mb][4 * g + j] += v;
+            }
+          }
+      }
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (row0 + wave * 32 + n >= rows) return;
+  float f = 1.0f;
+  float* dst;
+  if (sq.splits == 1) {
+    f = l == 0.0f ? 0.0f : 1.0f / l;
+    dst = a.out + (static_cast<size_t>(sq.tok0) * a.n_heads + qrow) * hd;
+  } else {
+    const size_t pr = sq.part0 + qrow * sq.splits + split;
+    dst = a.part + pr * hd;
+    if (h == 0) {
+      float* ml = a.part + a.part_rows * hd + pr * 2;
+      ml[0] = m;
+      ml[1] = l;
+    }
+  }
+  if constexpr (Q8) f *= top.top;
+#pragma unroll
+  for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const uint32_t d = mb * 32 + 8 * g + 4 * h;
+      if (d < hd)
+        *reinterpret_cast<float4*>(dst + d) =
+            make_float4(o[mb][4 * g] * f, o[mb][4 * g + 1] * f, o[mb][4 * g + 2] * f, o[mb][4 * g + 3] * f);
+    }
+}
+
+// ------------------------------------------------------------ joining the parts
+struct JoinSeq {
+  uint32_t row0;    // first (token, head) row of the sequence in this launch
+  uint32_t out0;    // its first row of out
+  uint32_t splits, part0;
+};
+struct JoinArgs {
+  const float* part;
+  size_t part_rows;
+  float* out;
+  uint32_t n_seq, n_rows, hd;
+  JoinSeq seq[kTrSeqs];
+};
+
+// One wave per row: M = max m_s, out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).
+// Lanes 16 bytes of the row apart; with narrow rows several parts at a time.
+__global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
+  const uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= a.n_rows) return;
+  int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.seq[mid].row0 <= r)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const JoinSeq& sq = a.seq[lo];
+  const uint32_t row = r - sq.row0, ns = sq.splits;
+  const size_t p0 = sq.part0 + static_cast<size_t>(row) * ns;
+  const float* ml = a.part + a.part_rows * a.hd + p0 * 2;
+  float M = -INFINITY;
+  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, ml[2 * s]);
+  M = wave_max_f32(M);
+  float L = 0.0f;
+  for (uint32_t s = lane; s < ns; s += 64)
+    if (ml[2 * s] != -INFINITY) L = fmaf(ml[2 * s + 1], exp2_hw(ml[2 * s] - M), L);
+  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+  const uint32_t lanes = a.hd <= 64 ? 16 : a.hd <= 128 ? 32 : 64;  // lanes of a part
+  const uint32_t d = (lane % lanes) * 4;
+  float4 y = make_float4(0, 0, 0, 0);
+  if (d < a.hd)
+    for (uint32_t s = lane / lanes; s < ns; s += 64 / lanes) {
+      const float m = ml[2 * s];
+      if (m == -INFINITY) continue;  // (it saw nothing)
+      const float f = exp2_hw(m - M);
+      const float4 x = *reinterpret_cast<const float4*>(a.part + (p0 + s) * a.hd + d);
+      y.x = fmaf(x.x, f, y.x);
+      y.y = fmaf(x.y, f, y.y);
+      y.z = fmaf(x.z, f, y.z);
+      y.w = fmaf(x.w, f, y.w);
+    }
+  for (uint32_t o = lanes; o < 64; o <<= 1) {
+    y.x += __shfl_xor(y.x, o, 64);
+    y.y += __shfl_xor(y.y, o, 64);
+    y.z += __shfl_xor(y.z, o, 64);
+    y.w += __shfl_xor(y.w, o, 64);
+  }
+  if (lane < lanes && d < a.hd) {
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    *reinterpret_cast<float4*>(a.out + (static_cast<size_t>(sq.out0) + row) * a.hd + d) =
+        make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+  }
+}
+
+// ------------------------------------------------------------ plan
+// Kernel of a sequence, by its rows per KV head.
+enum Width { kNarrow16, kNarrow32, kWide, kWidths };
+// (32 narrow rows of heads wider than 128 would not fit the registers.)
+Width width_of(size_t rows, size_t hd) {
+  return rows <= 16 ? kNarrow16 : rows <= 32 && hd <= 128 ? kNarrow32 : kWide;
+}
+
+struct Plan {
+  size_t rows_per_split[kWidths];
+  size_t part_rows;
+  size_t floats;
+};
+
+// Cache rows of a part: as many workgroups as keep the card busy (kParts of
+// them), in whole tiles, but no part shorter than kLeast rows.
+Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd) {
+  constexpr size_t kParts = 1024, kLeast = 256;
+  const size_t group = n_heads / n_kv;
+  size_t work[kWidths] = {};  // cache rows times row tiles
+  for (size_t i = 0; i < n_seq; i++) {
+    if (!n_tree[i]) continue;
+    const size_t rows = n_tree[i] * group;
+    const Width w = width_of(rows, hd);
+    work[w] += (past[i] + n_tree[i]) * (w == kWide ? (rows + kWideRows - 1) / kWideRows : 1);
+  }
+  Plan p{};
+  for (int w = 0; w < kWidths; w++) {
+    const size_t unit = w == kWide ? 64 : 128;
+    const size_t r = std::max(kLeast, work[w] * n_kv / kParts);
+    p.rows_per_split[w] = (r + unit - 1) / unit * unit;
+  }
+  for (size_t i = 0; i < n_seq; i++) {
+    if (!n_tree[i]) continue;
+    const size_t rps = p.rows_per_split[width_of(n_tree[i] * group, hd)];
+    const size_t splits = (past[i] + n_tree[i] + rps - 1) / rps;
+    if (splits > 1) p.part_rows += n_tree[i] * n_heads * splits;
+  }
+  p.floats = p.part_rows * (hd + 2);
+  return p;
+}
+
+template <int HDP, int BN>
+void launch_width(const TreeArgs& a, Width w, bool q8, uint32_t items, hipStream_t s) {
+  const dim3 grid(items * a.n_kv), nt(kTrNT);
+  if (w == kNarrow16) {
+    if (q8)
+      hipLaunchKernelGGL((tree_narrow_kernel<HDP, 1, true>), grid, nt, 0, s, a);
+    else
+      hipLaunchKernelGGL((tree_narrow_kernel<HDP, 1, false>), grid, nt, 0, s, a);
+  } else if (w == kNarrow32) {
+    if constexpr (HDP <= 128) {
+      if (q8)
+        hipLaunchKernelGGL((tree_narrow_kernel<HDP, 2, true>), grid, nt, 0, s, a);
+      else
+        hipLaunchKernelGGL((tree_narrow_kernel<HDP, 2, false>), grid, nt, 0, s, a);
+    }
+  } else {
+    if (q8)
+      hipLaunchKernelGGL((tree_wide_kernel<HDP, BN, true>), grid, nt, 0, s, a);
+    else
+      hipLaunchKernelGGL((tree_wide_kernel<HDP, BN, false>), grid, nt, 0, s, a);
+  }
 }
 
 }  // namespace
 
-size_t attention_tree_floats(const size_t*, const size_t*, size_t, size_t, size_t, size_t) { return 0; }
+size_t attention_tree_floats(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads,
+                             size_t n_kv_heads, size_t head_dim) {
+  return make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim).floats;
+}
 
 int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const size_t* past, const size_t* n_tree,
                           size_t n_seq, const uint64_t* mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
-                          float* out, float*, hipStream_t s) {
-  TreeArgs a{q, mask, out, static_cast<uint32_t>(n_heads), static_cast<uint32_t>(n_kv_heads),
-             static_cast<uint32_t>(n_heads / n_kv_heads), static_cast<uint32_t>(head_dim),
-             1.0f / sqrtf(static_cast<float>(head_dim))};
-  size_t tok = 0, n = 0;
-  uint32_t most = 0;
-  for (size_t i = 0; i <= n_seq; i++) {
-    if (i == n_seq || n == kTrSeqs) {
-      if (n) {
-        const dim3 grid(most, static_cast<uint32_t>(n_heads), static_cast<uint32_t>(n));
-        if (q8)
-          hipLaunchKernelGGL(tree_kernel<true>, grid, dim3(64), 0, s, a);
+                          float* out, float* workspace, hipStream_t s) {
+  const Plan plan = make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim);
+  TreeArgs a{};
+  a.q = q;
+  a.mask = mask;
+  a.out = out;
+  a.part = workspace;
+  a.part_rows = plan.part_rows;
+  a.n_heads = static_cast<uint32_t>(n_heads);
+  a.n_kv = static_cast<uint32_t>(n_kv_heads);
+  a.group = static_cast<uint32_t>(n_heads / n_kv_heads);
+  a.hd = static_cast<uint32_t>(head_dim);
+  a.scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_dim)));
+  JoinArgs j{};
+  j.part = workspace;
+  j.part_rows = plan.part_rows;
+  j.out = out;
+  j.hd = a.hd;
+  size_t part0 = 0;
+  for (int w = 0; w < kWidths; w++) {
+    a.rows_per_split = static_cast<uint32_t>(std::min<size_t>(plan.rows_per_split[w], 0x7fffffff));
+    size_t tok0 = 0, items = 0;
+    auto flush = [&]() -> int {
+      if (a.n_seq) {
+        const uint32_t it = static_cast<uint32_t>(items);
+        if (head_dim <= 64)
+          launch_width<64, 64>(a, static_cast<Width>(w), q8, it, s);
+        else if (head_dim <= 96)
+          launch_width<96, 64>(a, static_cast<Width>(w), q8, it, s);
+        else if (head_dim <= 128)
+          launch_width<128, 64>(a, static_cast<Width>(w), q8, it, s);
+        else if (head_dim <= 192)
+          launch_width<192, 64>(a, static_cast<Width>(w), q8, it, s);
         else
-          hipLaunchKernelGGL(tree_kernel<false>, grid, dim3(64), 0, s, a);
+          launch_width<256, 32>(a, static_cast<Width>(w), q8, it, s);
         PRANA_LAUNCH_CHECK();
       }
-      n = 0;
-      most = 0;
-      if (i == n_seq) break;
+      if (j.n_seq) {
+        hipLaunchKernelGGL(tree_join_kernel, dim3((j.n_rows + 3) / 4), dim3(256), 0, s, j);
+        PRANA_LAUNCH_CHECK();
+      }
+      a.n_seq = j.n_seq = j.n_rows = 0;
+      items = 0;
+      return kOk;
+    };
+    for (size_t i = 0; i < n_seq; tok0 += n_tree[i], i++) {
+      if (!n_tree[i]) continue;
+      const size_t rows = n_tree[i] * a.group;
+      if (width_of(rows, head_dim) != w) continue;
+      const size_t splits = (past[i] + n_tree[i] + plan.rows_per_split[w] - 1) / plan.rows_per_split[w];
+      if (a.n_seq == kTrSeqs)
+        if (int rc = flush()) return rc;
+      TreeSeq& t = a.seq[a.n_seq++];
+      t = TreeSeq{kv[i].k, kv[i].v, kv[i].k_scales, kv[i].v_scales, static_cast<uint32_t>(past[i]),
+                  static_cast<uint32_t>(n_tree[i]), static_cast<uint32_t>(tok0), static_cast<uint32_t>(items),
+                  static_cast<uint32_t>(splits), static_cast<uint32_t>(part0)};
+      items += splits * (w == kWide ? (rows + kWideRows - 1) / kWideRows : 1);
+      if (splits > 1) {
+        j.seq[j.n_seq++] = JoinSeq{j.n_rows, static_cast<uint32_t>(tok0 * n_heads), t.splits, t.part0};
+        j.n_rows += static_cast<uint32_t>(n_tree[i] * n_heads);
+        part0 += n_tree[i] * n_heads * splits;
+      }
     }
-    if (!n_tree[i]) continue;
-    a.seq[n++] = TreeSeq{kv[i].k, kv[i].v, kv[i].k_scales, kv[i].v_scales, static_cast<uint32_t>(past[i]),
-                         static_cast<uint32_t>(tok), static_cast<uint32_t>(n_tree[i])};
-    most = std::max(most, static_cast<uint32_t>(n_tree[i]));
-    tok += n_tree[i];
+    if (int rc = flush()) return rc;
   }
   return kOk;
 }
