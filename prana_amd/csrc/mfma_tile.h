@@ -16,6 +16,8 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef short short4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -35,21 +37,19 @@ __device__ __forceinline__ half8 join(half4 a, half4 b) {
 // 2^x as the hardware computes it (1 ulp; results under 2^-126 are 0).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Whether one of the two halves in w is an infinity or NaN.
-__device__ __forceinline__ bool pair_not_finite(uint32_t w) {
-  return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+// Bit 15 of each half of the result: that half of w is an infinity or NaN
+// (its exponent, all ones, carries into the sign's place).
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; }
+__device__ __forceinline__ uint32_t odd_halves(u32x4 v) {
+  return odd_halves(v.x) | odd_halves(v.y) | odd_halves(v.z) | odd_halves(v.w);
 }
-__device__ __forceinline__ bool any_not_finite(const uint4& v) {
-  return pair_not_finite(v.x) || pair_not_finite(v.y) || pair_not_finite(v.z) || pair_not_finite(v.w);
-}
+constexpr uint32_t kOddBits = 0x80008000u;
 // w with its halves that are not finite replaced by 0.
-__device__ __forceinline__ uint32_t pair_finite(uint32_t w) {
-  if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
-  if ((w & 0x7c000000u) == 0x7c000000u) w &= 0x0000ffffu;
-  return w;
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) {
+  return w & ~(((odd_halves(w) & kOddBits) >> 15) * 0xffffu);
 }
-__device__ __forceinline__ uint4 only_finite(const uint4& v) {
-  return make_uint4(pair_finite(v.x), pair_finite(v.y), pair_finite(v.z), pair_finite(v.w));
+__device__ __forceinline__ u32x4 only_finite(u32x4 v) {
+  return u32x4{only_finite(v.x), only_finite(v.y), only_finite(v.z), only_finite(v.w)};
 }
 
 // An f32 as two halves, x = hi + lo to 22 bits (|x| under 65504; lo has steps
@@ -59,7 +59,7 @@ __device__ __forceinline__ uint4 only_finite(const uint4& v) {
 __device__ __forceinline__ void split_half(float x, _Float16& hi, _Float16& lo) {
   asm("" : "+v"(x));
   hi = static_cast<_Float16>(x);
-  lo = static_cast<_Float16>(x - static_cast<float>(hi));
+  lo = static_cast<_Float16>(fmaf(static_cast<float>(hi), -1.0f, x));  // one instruction with its rounding
 }
 
 // The power of two that brings amax into [2^9, 2^10), where both halves of a

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
   static_assert(BN * S::kChunks % kPkNT == 0, "a tile is a whole number of pieces per lane");
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
   __shared__ __attribute__((aligned(16))) uint16_t s_v[BN * S::kLdV];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
   const uint32_t kvh = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv;
   int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
@@ -94,6 +94,33 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
   const uint32_t tok_last = min(row_w + 31, rows - 1) / a.group;
   const uint32_t hd = a.hd;
 
+  // Addresses: a uniform base per tile and a lane's 32-bit offset. Pieces past
+  // the head's width repeat its last one (q is 0 there for K, and V columns
+  // there are never stored).
+  const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
+  const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
+  u32x4 kr[S::kLoads], vr[S::kLoads];
+  auto fetch = [&](uint32_t k0) {
+    const unsigned char* kp = reinterpret_cast<const unsigned char*>(kb + k0 * a.ld_kv);
+    const unsigned char* vp = reinterpret_cast<const unsigned char*>(vb + k0 * a.ld_kv);
+    const bool whole = k0 + BN <= len;
+    const uint32_t last = whole ? BN - 1 : len - 1 - k0;
+#pragma unroll
+    for (int i = 0; i < S::kLoads; i++) {
+      const uint32_t e = i * kPkNT + tid;
+      const uint64_t off = (static_cast<uint64_t>(min(e / S::kChunks, last)) * a.ld_kv +
+                            min(e % S::kChunks * 8, hd - 8)) * 2;
+      kr[i] = *reinterpret_cast<const u32x4*>(kp + off);
+      vr[i] = *reinterpret_cast<const u32x4*>(vp + off);
+    }
+    if (!whole) {  // keys past the end: K repeats the last (and is masked), V is 0
+#pragma unroll
+      for (int i = 0; i < S::kLoads; i++)
+        if ((i * kPkNT + tid) / S::kChunks > last) vr[i] = u32x4{0, 0, 0, 0};
+    }
+  };
+  fetch(0);  // (on its way while q is read)
+
   // this row's q: operand B of the score product
   half8 qh[S::kStepsQK], ql[HALF ? 1 : S::kStepsQK];
   float c = a.scale;  // scores times c are in log2 units
@@ -102,8 +129,8 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
 #pragma unroll
     for (int s = 0; s < S::kStepsQK; s++) {
       const uint32_t d = s * 16 + h * 8;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (d < hd) w = *reinterpret_cast<const uint4*>(qp + d);
+      u32x4 w = {0, 0, 0, 0};
+      if (d < hd) w = *reinterpret_cast<const u32x4*>(qp + d);
       qh[s] = __builtin_bit_cast(half8, w);
     }
   } else {
@@ -147,22 +174,6 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
     for (int i = 0; i < 16; i++) o[mb][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;  // kept maximum (log2 units) and this lane's share of the sum
 
-  const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
-  const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
-  uint4 kr[S::kLoads], vr[S::kLoads];
-  auto fetch = [&](uint32_t k0) {
-#pragma unroll
-    for (int i = 0; i < S::kLoads; i++) {
-      const int e = i * kPkNT + tid;
-      const uint32_t r = k0 + e / S::kChunks, d = (e % S::kChunks) * 8;
-      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-      if (r < len && d < hd) {
-        kr[i] = *reinterpret_cast<const uint4*>(kb + r * a.ld_kv + d);
-        vr[i] = *reinterpret_cast<const uint4*>(vb + r * a.ld_kv + d);
-      }
-    }
-  };
-  fetch(0);
   for (uint32_t k0 = 0; k0 <= tok_last_wg; k0 += BN) {
     // Where the tile reaches past some row's token, a V value that is not
     // finite must not meet that row's zero probability: such values stay out
@@ -170,9 +181,10 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
     const bool diagonal = k0 + BN - 1 > tok_first_wg;
     bool odd = false;
     if (diagonal) {
+      uint32_t bits = 0;
 #pragma unroll
-      for (int i = 0; i < S::kLoads; i++) odd = odd || any_not_finite(vr[i]);
-      odd = __syncthreads_or(odd);  // (also: every wave is done with the tile before)
+      for (int i = 0; i < S::kLoads; i++) bits |= odd_halves(vr[i]);
+      odd = __syncthreads_or((bits & kOddBits) != 0);  // (also: every wave is done with the tile before)
       if (odd) {
 #pragma unroll
         for (int i = 0; i < S::kLoads; i++) vr[i] = only_finite(vr[i]);
@@ -184,8 +196,8 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
     for (int i = 0; i < S::kLoads; i++) {
       const int e = i * kPkNT + tid;
       const int r = e / S::kChunks, d = (e % S::kChunks) * 8;
-      *reinterpret_cast<uint4*>(s_k + r * S::kLdK + d) = kr[i];
-      *reinterpret_cast<uint4*>(s_v + r * S::kLdV + d) = vr[i];
+      *reinterpret_cast<u32x4*>(s_k + r * S::kLdK + d) = kr[i];
+      *reinterpret_cast<u32x4*>(s_v + r * S::kLdV + d) = vr[i];
     }
     __syncthreads();
     if (k0 + BN <= tok_last_wg) fetch(k0 + BN);
@@ -263,17 +275,22 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
         }
       }
     if (odd) {  // rare: the values left out, for the rows that see them (any weight gives the same result)
-      for (uint32_t r = k0; r < min(k0 + BN, len); r++)
+      for (uint32_t r = k0; r < min(k0 + BN, len); r++) {
+        if (r > tok) break;
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const uint32_t d = mb * 32 + 8 * (i / 4) + 4 * h + i % 4;
-            if (d < hd && r <= tok) {
-              const uint16_t w = vb[r * a.ld_kv + d];
-              if ((w & 0x7c00u) == 0x7c00u) o[mb][i] += f16_operand(w);
+          for (int g = 0; g < 4; g++) {
+            const uint32_t d = mb * 32 + 8 * g + 4 * h;
+            if (d >= hd) continue;
+            const half4 x = *reinterpret_cast<const half4*>(vb + r * a.ld_kv + d);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const float v = static_cast<float>(x[j]);
+              o[mb][4 * g + j] += fabsf(v) < INFINITY ? 0.0f : v;
             }
           }
+      }
     }
   }
   l += __shfl_xor(l, 32, 64);

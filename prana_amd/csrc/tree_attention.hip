@@ -91,7 +91,7 @@ __device__ __forceinline__ uint64_t seen_from(uint64_t word, int first_minus_pas
 
 // Eight i8 values as halves: u = v + 128 in the low bits of 0x6400 is the half
 // 1024 + u, and 1152 off that is v.
-__device__ __forceinline__ uint4 i8_to_halves(uint2 w) {
+__device__ __forceinline__ u32x4 i8_to_halves(u32x2 w) {
   const uint32_t u[2] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u};
   uint32_t o[4];
 #pragma unroll
@@ -101,27 +101,28 @@ __device__ __forceinline__ uint4 i8_to_halves(uint2 w) {
     const half2v x = __builtin_bit_cast(half2v, pair) - half2v{1152.0f16, 1152.0f16};
     o[j] = __builtin_bit_cast(uint32_t, x);
   }
-  return make_uint4(o[0], o[1], o[2], o[3]);
+  return u32x4{o[0], o[1], o[2], o[3]};
 }
 
-// Eight values of a cache row as loaded, and as halves.
+// Eight values of a cache row as loaded, and as halves. Addresses are a
+// wave-uniform base, moved from tile to tile, and a lane's 32-bit offset.
 template <bool Q8>
 struct Piece {
-  uint4 w;
-  __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void load(const void* base, size_t at) {
-    w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
+  u32x4 w;
+  __device__ __forceinline__ void zero() { w = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void load(const unsigned char* base, uint32_t off) {
+    w = *reinterpret_cast<const u32x4*>(base + off);
   }
-  __device__ __forceinline__ uint4 halves() const { return w; }
+  __device__ __forceinline__ u32x4 halves() const { return w; }
 };
 template <>
 struct Piece<true> {
-  uint2 w;
-  __device__ __forceinline__ void zero() { w = make_uint2(0, 0); }
-  __device__ __forceinline__ void load(const void* base, size_t at) {
-    w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(base) + at);
+  u32x2 w;
+  __device__ __forceinline__ void zero() { w = u32x2{0, 0}; }
+  __device__ __forceinline__ void load(const unsigned char* base, uint32_t off) {
+    w = *reinterpret_cast<const u32x2*>(base + off);
   }
-  __device__ __forceinline__ uint4 halves() const { return i8_to_halves(w); }
+  __device__ __forceinline__ u32x4 halves() const { return i8_to_halves(w); }
 };
 
 // A row's q as the score product's operand: PIECES pieces of 8 dims, piece s
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[S::kBytes];
   __shared__ __attribute__((aligned(16))) float s_scale[4][64];  // per wave: K scales of 32 keys, V scales
   __shared__ float s_m[4][16 * RB], s_l[4][16 * RB];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   uint16_t* s_v = reinterpret_cast<uint16_t*>(s_mem) + wave * S::kWaveHalves;
   const uint32_t kvh = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
@@ -204,6 +205,52 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
   const uint32_t split = item - sq.item0, hd = a.hd;
   const uint32_t rows = sq.tokens * a.group, total = sq.past + sq.tokens;
   const uint32_t kbeg = split * a.rows_per_split, kend = min(total, kbeg + a.rows_per_split);
+
+  // Pieces past the head's width repeat its last one: q is 0 there for K, and
+  // V columns there are never stored.
+  constexpr uint32_t kSize = Q8 ? 1 : 2;
+  const size_t ld = static_cast<size_t>(a.n_kv) * hd, head = static_cast<size_t>(kvh) * hd;
+  const unsigned char* kbase = static_cast<const unsigned char*>(sq.k) + head * kSize;
+  const unsigned char* vbase = static_cast<const unsigned char*>(sq.v) + head * kSize;
+  Piece<Q8> kr[2][S::kSteps], vr[S::kPieces];
+  float sc = 0.0f;  // lanes 0-31: K scale of key lane; 32-63: V scale of key lane - 32
+  auto fetch = [&](uint32_t k0) {
+    const unsigned char* kp = kbase + k0 * ld * kSize;
+    const unsigned char* vp = vbase + k0 * ld * kSize;
+    if (k0 + 32 <= kend) {
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int s = 0; s < S::kSteps; s++)
+          kr[b][s].load(kp + b * 16 * ld * kSize,
+                        (n * static_cast<uint32_t>(ld) + min(s * 32u + g * 8, hd - 8)) * kSize);
+#pragma unroll
+      for (int p = 0; p < S::kPieces; p++) {
+        const uint32_t e = p * 64 + lane;
+        vr[p].load(vp, (e / (HDP / 8) * static_cast<uint32_t>(ld) + min(e % (HDP / 8) * 8, hd - 8)) * kSize);
+      }
+    } else {  // keys past the end: K repeats the last (and is masked), V is 0
+      const uint32_t last = kend - 1 - k0;
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int s = 0; s < S::kSteps; s++)
+          kr[b][s].load(kp, (min(b * 16u + n, last) * static_cast<uint32_t>(ld) + min(s * 32u + g * 8, hd - 8)) * kSize);
+#pragma unroll
+      for (int p = 0; p < S::kPieces; p++) {
+        const uint32_t e = p * 64 + lane, r = e / (HDP / 8);
+        vr[p].load(vp, (min(r, last) * static_cast<uint32_t>(ld) + min(e % (HDP / 8) * 8, hd - 8)) * kSize);
+        if (r > last) vr[p].zero();
+      }
+    }
+    if constexpr (Q8) {
+      const uint32_t t = k0 + (lane & 31);
+      sc = 0.0f;
+      if (t < kend) sc = (lane < 32 ? sq.ks : sq.vs)[static_cast<size_t>(t) * a.n_kv + kvh];
+    }
+  };
+  uint32_t k0 = kbeg + wave * 32;
+  if (k0 < kend) fetch(k0);  // (on its way while q is read)
 
   half8 qh[RB][S::kSteps], ql[RB][S::kSteps];
   float c[RB], m[RB], l[RB];
@@ -223,36 +270,6 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
       for (int j = 0; j < 4; j++) o[r][mb][j] = 0.0f;
   }
   ScaleTop top;
-
-  const size_t ld = static_cast<size_t>(a.n_kv) * hd, head = static_cast<size_t>(kvh) * hd;
-  Piece<Q8> kr[2][S::kSteps], vr[S::kPieces];
-  float sc = 0.0f;  // lanes 0-31: K scale of key lane; 32-63: V scale of key lane - 32
-  auto fetch = [&](uint32_t k0) {
-#pragma unroll
-    for (int b = 0; b < 2; b++) {
-      const uint32_t t = min(k0 + b * 16 + n, kend - 1);  // (keys past the end repeat the last and are masked)
-#pragma unroll
-      for (int s = 0; s < S::kSteps; s++) {
-        const uint32_t d = s * 32 + g * 8;
-        kr[b][s].zero();
-        if (d < hd) kr[b][s].load(sq.k, t * ld + head + d);
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < S::kPieces; p++) {
-      const int e = p * 64 + lane;
-      const uint32_t t = k0 + e / (HDP / 8), d = (e % (HDP / 8)) * 8;
-      vr[p].zero();
-      if (t < kend && d < hd) vr[p].load(sq.v, t * ld + head + d);
-    }
-    if constexpr (Q8) {
-      const uint32_t t = k0 + (lane & 31);
-      sc = 0.0f;
-      if (t < kend) sc = (lane < 32 ? sq.ks : sq.vs)[static_cast<size_t>(t) * a.n_kv + kvh];
-    }
-  };
-  uint32_t k0 = kbeg + wave * 32;
-  if (k0 < kend) fetch(k0);
   for (; k0 < kend; k0 += 128) {
     const bool edge = k0 + 32 > min(sq.past, kend);  // not every row sees every key
     bool odd = false;
@@ -260,9 +277,10 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
       // a V value that is not finite must not meet the zero probability of a
       // row that does not see it: it is left out and added below
       if (edge) {
+        uint32_t bits = 0;
 #pragma unroll
-        for (int p = 0; p < S::kPieces; p++) odd = odd || any_not_finite(vr[p].w);
-        odd = __any(odd);
+        for (int p = 0; p < S::kPieces; p++) bits |= odd_halves(vr[p].w);
+        odd = __any((bits & kOddBits) != 0);
         if (odd) {
 #pragma unroll
           for (int p = 0; p < S::kPieces; p++) vr[p].w = only_finite(vr[p].w);
@@ -274,7 +292,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
 #pragma unroll
     for (int p = 0; p < S::kPieces; p++) {
       const int e = p * 64 + lane;
-      *reinterpret_cast<uint4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vr[p].halves();
+      *reinterpret_cast<u32x4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vr[p].halves();
     }
     if constexpr (Q8) {
       s_scale[wave][lane] = sc;
@@ -292,13 +310,13 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 
-    f32x4 s[RB][2];
+    f32x4 s[RB][2], s2[RB][2];  // from both halves of q
 #pragma unroll
     for (int r = 0; r < RB; r++)
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[r][b][j] = 0.0f;
+        for (int j = 0; j < 4; j++) s[r][b][j] = s2[r][b][j] = 0.0f;
 #pragma unroll
     for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -307,9 +325,13 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
 #pragma unroll
         for (int r = 0; r < RB; r++) {
           s[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[r][t], s[r][b], 0, 0, 0);
-          s[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[r][t], s[r][b], 0, 0, 0);
+          s2[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[r][t], s2[r][b], 0, 0, 0);
         }
       }
+#pragma unroll
+    for (int r = 0; r < RB; r++)
+#pragma unroll
+      for (int b = 0; b < 2; b++) s[r][b] += s2[r][b];
     const uint32_t kcur = k0;
     if (k0 + 128 < kend) fetch(k0 + 128);
 
@@ -393,7 +415,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
         for (int mb = 0; mb < S::kDimBlocks; mb++) {
           const uint32_t d = mb * 16 + 4 * g;
           if (d >= hd) continue;
-          const half4 x = *reinterpret_cast<const half4*>(static_cast<const uint16_t*>(sq.v) + t * ld + head + d);
+          const half4 x = *reinterpret_cast<const half4*>(vbase + (t * ld + d) * kSize);
 #pragma unroll
           for (int r = 0; r < RB; r++)
 #pragma unroll
@@ -477,7 +499,7 @@ struct WideShape {
 };
 
 template <int HDP, int BN, bool Q8>
-__global__ __launch_bounds__(kTrNT, HDP <= 96 ? 2 : 1) void tree_wide_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(TreeArgs a) {
   using S = WideShape<HDP, BN>;
   static_assert(BN * S::kChunks % kTrNT == 0, "a tile is a whole number of pieces per lane");
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
@@ -496,6 +518,37 @@ __global__ __launch_bounds__(kTrNT, HDP <= 96 ? 2 : 1) void tree_wide_kernel(Tre
   const size_t qrow = static_cast<size_t>(i) * a.n_heads + kvh * a.group + row % a.group;
   const uint64_t word = mask_word(a, sq, i);
 
+  constexpr uint32_t kSize = Q8 ? 1 : 2;
+  const size_t ld = static_cast<size_t>(a.n_kv) * hd, head = static_cast<size_t>(kvh) * hd;
+  const unsigned char* kbase = static_cast<const unsigned char*>(sq.k) + head * kSize;
+  const unsigned char* vbase = static_cast<const unsigned char*>(sq.v) + head * kSize;
+  Piece<Q8> kr[S::kLoads], vr[S::kLoads];
+  float sc = 0.0f;  // lanes 0..BN-1: K scale of key lane; BN..2BN-1: V scales
+  auto fetch = [&](uint32_t k0) {
+    const unsigned char* kp = kbase + k0 * ld * kSize;
+    const unsigned char* vp = vbase + k0 * ld * kSize;
+    const bool whole = k0 + BN <= kend;
+    const uint32_t last = whole ? BN - 1 : kend - 1 - k0;
+#pragma unroll
+    for (int p = 0; p < S::kLoads; p++) {
+      const uint32_t e = p * kTrNT + tid, r = e / S::kChunks;
+      const uint32_t off = (min(r, last) * static_cast<uint32_t>(ld) + min(e % S::kChunks * 8, hd - 8)) * kSize;
+      kr[p].load(kp, off);
+      vr[p].load(vp, off);
+    }
+    if (!whole) {  // keys past the end: K repeats the last (and is masked), V is 0
+#pragma unroll
+      for (int p = 0; p < S::kLoads; p++)
+        if ((p * kTrNT + tid) / S::kChunks > last) vr[p].zero();
+    }
+    if constexpr (Q8) {
+      const uint32_t t = k0 + tid % BN;
+      sc = 0.0f;
+      if (tid < 2 * BN && t < kend) sc = (tid < BN ? sq.ks : sq.vs)[static_cast<size_t>(t) * a.n_kv + kvh];
+    }
+  };
+  fetch(kbeg);  // (on its way while q is read)
+
   half8 qh[S::kStepsQK], ql[S::kStepsQK];
   const float c = load_q<S::kStepsQK, 16, 2>(a.q + (static_cast<size_t>(sq.tok0) * a.n_heads + qrow) * hd, h * 8, hd,
                                              a.scale, qh, ql);
@@ -507,36 +560,15 @@ __global__ __launch_bounds__(kTrNT, HDP <= 96 ? 2 : 1) void tree_wide_kernel(Tre
   float m = -INFINITY, l = 0.0f;
   ScaleTop top;
 
-  const size_t ld = static_cast<size_t>(a.n_kv) * hd, head = static_cast<size_t>(kvh) * hd;
-  Piece<Q8> kr[S::kLoads], vr[S::kLoads];
-  float sc = 0.0f;  // lanes 0..BN-1: K scale of key lane; BN..2BN-1: V scales
-  auto fetch = [&](uint32_t k0) {
-#pragma unroll
-    for (int p = 0; p < S::kLoads; p++) {
-      const int e = p * kTrNT + tid;
-      const uint32_t t = k0 + e / S::kChunks, d = (e % S::kChunks) * 8;
-      kr[p].zero();
-      vr[p].zero();
-      if (t < kend && d < hd) {
-        kr[p].load(sq.k, t * ld + head + d);
-        vr[p].load(sq.v, t * ld + head + d);
-      }
-    }
-    if constexpr (Q8) {
-      const uint32_t t = k0 + tid % BN;
-      sc = 0.0f;
-      if (tid < 2 * BN && t < kend) sc = (tid < BN ? sq.ks : sq.vs)[static_cast<size_t>(t) * a.n_kv + kvh];
-    }
-  };
-  fetch(kbeg);
   for (uint32_t k0 = kbeg; k0 < kend; k0 += BN) {
     const bool edge = k0 + BN > min(sq.past, kend);
     bool odd = false;
     if (!Q8 && edge) {
       if constexpr (!Q8) {
+        uint32_t bits = 0;
 #pragma unroll
-        for (int p = 0; p < S::kLoads; p++) odd = odd || any_not_finite(vr[p].w);
-        odd = __syncthreads_or(odd);
+        for (int p = 0; p < S::kLoads; p++) bits |= odd_halves(vr[p].w);
+        odd = __syncthreads_or((bits & kOddBits) != 0);
         if (odd) {
 #pragma unroll
           for (int p = 0; p < S::kLoads; p++) vr[p].w = only_finite(vr[p].w);
@@ -549,8 +581,8 @@ __global__ __launch_bounds__(kTrNT, HDP <= 96 ? 2 : 1) void tree_wide_kernel(Tre
     for (int p = 0; p < S::kLoads; p++) {
       const int e = p * kTrNT + tid;
       const int r = e / S::kChunks, d = (e % S::kChunks) * 8;
-      *reinterpret_cast<uint4*>(s_k + r * S::kLdK + d) = kr[p].halves();
-      *reinterpret_cast<uint4*>(s_v + r * S::kLdV + d) = vr[p].halves();
+      *reinterpret_cast<u32x4*>(s_k + r * S::kLdK + d) = kr[p].halves();
+      *reinterpret_cast<u32x4*>(s_v + r * S::kLdV + d) = vr[p].halves();
     }
     if constexpr (Q8) {
       if (tid < 2 * BN) s_scale[tid / BN][tid % BN] = sc;
@@ -664,7 +696,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 96 ? 2 : 1) void tree_wide_kernel(Tre
           for (int g = 0; g < 4; g++) {
             const uint32_t d = mb * 32 + 8 * g + 4 * h;
             if (d >= hd) continue;
-            const half4 x = *reinterpret_cast<const half4*>(static_cast<const uint16_t*>(sq.v) + t * ld + head + d);
+            const half4 x = *reinterpret_cast<const half4*>(vbase + (t * ld + d) * kSize);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               const float v = static_cast<float>(x[j]);
@@ -716,11 +748,15 @@ struct JoinArgs {
   JoinSeq seq[kTrSeqs];
 };
 
-// One wave per row: M = max m_s, out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).
-// Lanes 16 bytes of the row apart; with narrow rows several parts at a time.
+// A row: M = max m_s, out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), by
+// T lanes (a wave, or a workgroup where a row has many parts). A part's row is
+// read by LANES lanes, 16 bytes each, T / LANES parts at a time; kBatch loads
+// of a lane are in flight together, the first ones before M is known.
+template <int T, int LANES>
 __global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
-  const uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (r >= a.n_rows) return;
+  constexpr int kBatch = 8, kPG = T / LANES, kWaves = T / 64;
+  const uint32_t r = blockIdx.x * (256 / T) + threadIdx.x / T, tid = threadIdx.x % T, lane = threadIdx.x & 63;
+  if (r >= a.n_rows) return;  // (whole waves; with T = 256 never)
   int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -732,39 +768,76 @@ __global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
   const JoinSeq& sq = a.seq[lo];
   const uint32_t row = r - sq.row0, ns = sq.splits;
   const size_t p0 = sq.part0 + static_cast<size_t>(row) * ns;
-  const float* ml = a.part + a.part_rows * a.hd + p0 * 2;
+  const float2* ml = reinterpret_cast<const float2*>(a.part + a.part_rows * a.hd) + p0;
+  const uint32_t d = (tid % LANES) * 4, s0 = tid / LANES;
+  const float* src = a.part + p0 * a.hd + min(d, a.hd - 4);
+  float4 x[kBatch];
+  float ms[kBatch];
+  auto load = [&](uint32_t s) {
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) {
+      const uint32_t at = min(s + k * kPG, ns - 1);
+      x[k] = *reinterpret_cast<const float4*>(src + static_cast<size_t>(at) * a.hd);
+      ms[k] = ml[at].x;
+    }
+  };
+  load(s0);
   float M = -INFINITY;
-  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, ml[2 * s]);
+  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, ml[s].x);
   M = wave_max_f32(M);
   float L = 0.0f;
-  for (uint32_t s = lane; s < ns; s += 64)
-    if (ml[2 * s] != -INFINITY) L = fmaf(ml[2 * s + 1], exp2_hw(ml[2 * s] - M), L);
+  for (uint32_t s = lane; s < ns; s += 64) {
+    const float2 v = ml[s];
+    if (v.x != -INFINITY) L = fmaf(v.y, exp2_hw(v.x - M), L);
+  }
   for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
-  const uint32_t lanes = a.hd <= 64 ? 16 : a.hd <= 128 ? 32 : 64;  // lanes of a part
-  const uint32_t d = (lane % lanes) * 4;
   float4 y = make_float4(0, 0, 0, 0);
-  if (d < a.hd)
-    for (uint32_t s = lane / lanes; s < ns; s += 64 / lanes) {
-      const float m = ml[2 * s];
-      if (m == -INFINITY) continue;  // (it saw nothing)
-      const float f = exp2_hw(m - M);
-      const float4 x = *reinterpret_cast<const float4*>(a.part + (p0 + s) * a.hd + d);
-      y.x = fmaf(x.x, f, y.x);
-      y.y = fmaf(x.y, f, y.y);
-      y.z = fmaf(x.z, f, y.z);
-      y.w = fmaf(x.w, f, y.w);
+  for (uint32_t s = s0; s < ns; s += kBatch * kPG) {
+    if (s != s0) load(s);
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) {
+      if (s + k * kPG >= ns || ms[k] == -INFINITY) continue;  // (a part that saw nothing holds zeros)
+      const float f = exp2_hw(ms[k] - M);
+      y.x = fmaf(x[k].x, f, y.x);
+      y.y = fmaf(x[k].y, f, y.y);
+      y.z = fmaf(x[k].z, f, y.z);
+      y.w = fmaf(x[k].w, f, y.w);
     }
-  for (uint32_t o = lanes; o < 64; o <<= 1) {
+  }
+#pragma unroll
+  for (int o = LANES; o < 64; o <<= 1) {
     y.x += __shfl_xor(y.x, o, 64);
     y.y += __shfl_xor(y.y, o, 64);
     y.z += __shfl_xor(y.z, o, 64);
     y.w += __shfl_xor(y.w, o, 64);
   }
-  if (lane < lanes && d < a.hd) {
+  if constexpr (kWaves > 1) {
+    __shared__ __attribute__((aligned(16))) float4 s_y[kWaves][64];
+    s_y[threadIdx.x >> 6][lane] = y;
+    __syncthreads();
+    y = s_y[0][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) {
+      const float4 z = s_y[w][lane];
+      y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+    }
+  }
+  if (tid < LANES && d < a.hd) {
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     *reinterpret_cast<float4*>(a.out + (static_cast<size_t>(sq.out0) + row) * a.hd + d) =
         make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
   }
+}
+
+template <int T>
+void launch_join(const JoinArgs& j, hipStream_t s) {
+  const dim3 grid((j.n_rows + 256 / T - 1) / (256 / T)), nt(256);
+  if (j.hd <= 64)
+    hipLaunchKernelGGL((tree_join_kernel<T, 16>), grid, nt, 0, s, j);
+  else if (j.hd <= 128)
+    hipLaunchKernelGGL((tree_join_kernel<T, 32>), grid, nt, 0, s, j);
+  else
+    hipLaunchKernelGGL((tree_join_kernel<T, 64>), grid, nt, 0, s, j);
 }
 
 // ------------------------------------------------------------ plan
@@ -784,7 +857,7 @@ struct Plan {
 // Cache rows of a part: as many workgroups as keep the card busy (kParts of
 // them), in whole tiles, but no part shorter than kLeast rows.
 Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd) {
-  constexpr size_t kParts = 1024, kLeast = 256;
+  constexpr size_t kParts = 768, kLeast = 128;
   const size_t group = n_heads / n_kv;
   size_t work[kWidths] = {};  // cache rows times row tiles
   for (size_t i = 0; i < n_seq; i++) {
@@ -862,7 +935,7 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
   size_t part0 = 0;
   for (int w = 0; w < kWidths; w++) {
     a.rows_per_split = static_cast<uint32_t>(std::min<size_t>(plan.rows_per_split[w], 0x7fffffff));
-    size_t tok0 = 0, items = 0;
+    size_t tok0 = 0, items = 0, most_splits = 0;
     auto flush = [&]() -> int {
       if (a.n_seq) {
         const uint32_t it = static_cast<uint32_t>(items);
@@ -879,11 +952,14 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
         PRANA_LAUNCH_CHECK();
       }
       if (j.n_seq) {
-        hipLaunchKernelGGL(tree_join_kernel, dim3((j.n_rows + 3) / 4), dim3(256), 0, s, j);
+        if (most_splits > 16)
+          launch_join<256>(j, s);
+        else
+          launch_join<64>(j, s);
         PRANA_LAUNCH_CHECK();
       }
       a.n_seq = j.n_seq = j.n_rows = 0;
-      items = 0;
+      items = most_splits = 0;
       return kOk;
     };
     for (size_t i = 0; i < n_seq; tok0 += n_tree[i], i++) {
@@ -899,6 +975,7 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
                   static_cast<uint32_t>(splits), static_cast<uint32_t>(part0)};
       items += splits * (w == kWide ? (rows + kWideRows - 1) / kWideRows : 1);
       if (splits > 1) {
+        most_splits = std::max(most_splits, splits);
         j.seq[j.n_seq++] = JoinSeq{j.n_rows, static_cast<uint32_t>(tok0 * n_heads), t.splits, t.part0};
         j.n_rows += static_cast<uint32_t>(n_tree[i] * n_heads);
         part0 += n_tree[i] * n_heads * splits;
