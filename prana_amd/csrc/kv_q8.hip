@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "seq_table.h"
 #include "serving.h"
 
 namespace prana {
@@ -22,38 +23,35 @@ namespace prana {
 namespace {
 
 constexpr int kKvNT = 256;
-constexpr int kKvSeqs = 64;  // sequences of one launch: 56 bytes each of kernel arguments
-constexpr int kItems = 4;    // heads of a lane group, loads in flight together
-
-struct KvSeq {
-  void *k, *v;
-  float *ks, *vs;
-  uint32_t src;     // first packed row
-  uint32_t rows;    // rows to move
-  uint32_t first;   // first cache row
-  uint32_t block0;  // first workgroup of the sequence
-};
+constexpr int kItems = 4;  // heads of a lane group, loads in flight together
 
 struct KvArgs {
   const void* k;  // the packed side
   const void* v;
   size_t ld;
   uint32_t n_seq, n_kv, hd;
-  KvSeq seq[kKvSeqs];
+  void* kc[kTableSeqs];
+  void* vc[kTableSeqs];
+  float* ks[kTableSeqs];
+  float* vs[kTableSeqs];
+  uint32_t src[kTableSeqs];     // first packed row
+  uint32_t rows[kTableSeqs];    // rows to move
+  uint32_t first[kTableSeqs];   // first cache row
+  uint32_t block0[kTableSeqs];  // first workgroup
 };
 
-// The sequence that workgroup b belongs to: the last whose first workgroup is
-// not past it.
-__device__ __forceinline__ int find_seq(const KvArgs& a, uint32_t b) {
-  int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.seq[mid].block0 <= b)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
+struct KvSeq {
+  void* cache;
+  float* scales;
+  uint32_t src, rows, first, block0;
+};
+
+// The sequence of this workgroup, its K (blockIdx.y 0) or V cache.
+__device__ __forceinline__ KvSeq this_seq(const KvArgs& a) {
+  const int s = table_find(a.block0, a.n_seq, blockIdx.x);
+  const bool second = blockIdx.y != 0;
+  return KvSeq{table_at(second ? a.vc : a.kc, s), table_at(second ? a.vs : a.ks, s), table_at(a.src, s),
+               table_at(a.rows, s), table_at(a.first, s), table_at(a.block0, s)};
 }
 
 // Largest of v over aligned groups of LPH lanes (a power of two).
@@ -84,12 +82,9 @@ __device__ __forceinline__ int quantize_exact(float x, float amax, float inv, bo
 template <int LPH>
 __global__ __launch_bounds__(kKvNT) void kv_write_kernel(KvArgs a) {
   constexpr int kGroups = kKvNT / LPH;  // heads a workgroup takes at a time
-  const int si = find_seq(a, blockIdx.x);
-  const KvSeq& sq = a.seq[si];
-  const bool second = blockIdx.y != 0;
-  const float* src = static_cast<const float*>(second ? a.v : a.k);
-  int8_t* dst = static_cast<int8_t*>(second ? sq.v : sq.k);
-  float* scales = second ? sq.vs : sq.ks;
+  const KvSeq sq = this_seq(a);
+  const float* src = static_cast<const float*>(blockIdx.y ? a.v : a.k);
+  int8_t* dst = static_cast<int8_t*>(sq.cache);
   const int sub = threadIdx.x % LPH, grp = threadIdx.x / LPH;
   const bool live = sub * 8u < a.hd;
   const uint64_t n_items = static_cast<uint64_t>(sq.rows) * a.n_kv;
@@ -134,19 +129,16 @@ __global__ __launch_bounds__(kKvNT) void kv_write_kernel(KvArgs a) {
     const size_t r = static_cast<size_t>(sq.first) + row;
     if (live)
       *reinterpret_cast<uint2*>(dst + (r * a.n_kv + head) * a.hd + sub * 8) = make_uint2(w[0], w[1]);
-    if (sub == 0) scales[r * a.n_kv + head] = scale;
+    if (sub == 0) sq.scales[r * a.n_kv + head] = scale;
   }
 }
 
 template <int LPH, bool HALF>
 __global__ __launch_bounds__(kKvNT) void kv_read_kernel(KvArgs a) {
   constexpr int kGroups = kKvNT / LPH;
-  const int si = find_seq(a, blockIdx.x);
-  const KvSeq& sq = a.seq[si];
-  const bool second = blockIdx.y != 0;
-  const int8_t* src = static_cast<const int8_t*>(second ? sq.v : sq.k);
-  const float* scales = second ? sq.vs : sq.ks;
-  void* dst = const_cast<void*>(second ? a.v : a.k);
+  const KvSeq sq = this_seq(a);
+  const int8_t* src = static_cast<const int8_t*>(sq.cache);
+  void* dst = const_cast<void*>(blockIdx.y ? a.v : a.k);
   const int sub = threadIdx.x % LPH, grp = threadIdx.x / LPH;
   if (sub * 8u >= a.hd) return;
   const uint64_t n_items = static_cast<uint64_t>(sq.rows) * a.n_kv;
@@ -161,7 +153,7 @@ __global__ __launch_bounds__(kKvNT) void kv_read_kernel(KvArgs a) {
     if (item < n_items) {
       const size_t at = static_cast<size_t>(sq.first) * a.n_kv + item;  // (row, head) of the cache
       w[it] = *reinterpret_cast<const uint2*>(src + at * a.hd + sub * 8);
-      scale[it] = scales[at];
+      scale[it] = sq.scales[at];
     }
   }
 #pragma unroll
@@ -243,17 +235,17 @@ int launch_moves(Move m, const void* k, const void* v, size_t ld, const prana_kv
     const size_t part = std::max<size_t>(1, kPartBlocks * per_block / n_kv);
     for (size_t r = 0; r < n_rows[i]; r += part) {
       const size_t rows = std::min(part, n_rows[i] - r);
-      if (a.n_seq == kKvSeqs || blocks > kPartBlocks)
+      if (a.n_seq == kTableSeqs || blocks > kPartBlocks)
         if (int rc = flush()) return rc;
-      KvSeq& q = a.seq[a.n_seq++];
-      q.k = kv[i].k;
-      q.v = kv[i].v;
-      q.ks = kv[i].k_scales;
-      q.vs = kv[i].v_scales;
-      q.src = static_cast<uint32_t>(src + r);
-      q.rows = static_cast<uint32_t>(rows);
-      q.first = static_cast<uint32_t>(first_rows[i] + r);
-      q.block0 = static_cast<uint32_t>(blocks);
+      const uint32_t e = a.n_seq++;
+      a.kc[e] = kv[i].k;
+      a.vc[e] = kv[i].v;
+      a.ks[e] = kv[i].k_scales;
+      a.vs[e] = kv[i].v_scales;
+      a.src[e] = static_cast<uint32_t>(src + r);
+      a.rows[e] = static_cast<uint32_t>(rows);
+      a.first[e] = static_cast<uint32_t>(first_rows[i] + r);
+      a.block0[e] = static_cast<uint32_t>(blocks);
       blocks += (rows * n_kv + per_block - 1) / per_block;
     }
     src += n_rows[i];

@@ -25,13 +25,13 @@
 
 #include "common.h"
 #include "mfma_tile.h"
+#include "seq_table.h"
 #include "serving.h"
 
 namespace prana {
 
 namespace {
 
-constexpr int kPkSeqs = 128;   // sequences of one launch
 constexpr int kPkNT = 256;     // lanes of a workgroup
 constexpr int kPkRows = 128;   // rows of a workgroup
 constexpr float kLag = 8.0f;   // how far (log2) scores may pass the kept maximum
@@ -45,9 +45,9 @@ struct PackedArgs {
   size_t ld_q, ld_kv, ld_out;
   uint32_t n_seq, n_kv, group, hd;
   float scale;  // log2(e) / sqrt(hd)
-  uint32_t start[kPkSeqs];  // first packed row
-  uint32_t len[kPkSeqs];
-  uint32_t tile0[kPkSeqs];  // first row tile
+  uint32_t start[kTableSeqs];  // first packed row
+  uint32_t len[kTableSeqs];
+  uint32_t tile0[kTableSeqs];  // first row tile
 };
 
 // HDP: head width rounded up; the lanes past the real one hold zeros.
@@ -72,19 +72,12 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
   const uint32_t kvh = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv;
-  int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.tile0[mid] <= tile)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const uint32_t len = a.len[lo], rows = len * a.group;
+  const int sq = table_find(a.tile0, a.n_seq, tile);
+  const uint32_t len = table_at(a.len, sq), rows = len * a.group;
   const uint32_t n_tiles = (rows + kPkRows - 1) / kPkRows;
   // the last tiles see the most keys: they go first
-  const uint32_t row0 = (n_tiles - 1 - (tile - a.tile0[lo])) * kPkRows;
-  const size_t base = a.start[lo];
+  const uint32_t row0 = (n_tiles - 1 - (tile - table_at(a.tile0, sq))) * kPkRows;
+  const size_t base = table_at(a.start, sq);
   const uint32_t row_w = row0 + wave * 32;                       // the wave's first row
   const uint32_t row = min(row_w + n, rows - 1);                 // (rows past the end repeat the last one)
   const uint32_t tok = row / a.group, head = kvh * a.group + row % a.group;
@@ -356,7 +349,7 @@ int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v,
   for (size_t i = 0; i < seqs.size();) {
     size_t tiles = 0;
     a.n_seq = 0;
-    while (i < seqs.size() && a.n_seq < kPkSeqs) {
+    while (i < seqs.size() && a.n_seq < kTableSeqs) {
       const size_t t = (seqs[i].len * a.group + kPkRows - 1) / kPkRows;
       if (a.n_seq && tiles + t > most) break;
       a.start[a.n_seq] = static_cast<uint32_t>(seqs[i].start);

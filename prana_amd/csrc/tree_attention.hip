@@ -30,26 +30,16 @@
 
 #include "common.h"
 #include "mfma_tile.h"
+#include "seq_table.h"
 #include "serving.h"
 
 namespace prana {
 
 namespace {
 
-constexpr int kTrSeqs = 64;  // sequences of one launch
 constexpr int kTrNT = 256;
 constexpr float kLag = 8.0f;
 constexpr float kPShift = 7.0f;  // probabilities are kept times 2^7, at most 2^15
-
-struct TreeSeq {
-  const void *k, *v;
-  const float *ks, *vs;
-  uint32_t past, tokens;
-  uint32_t tok0;    // first drafted token in q, mask and out
-  uint32_t item0;   // first work item of the sequence
-  uint32_t splits;  // parts of the cache rows
-  uint32_t part0;   // first partial state, in rows (a sequence holds tokens * n_heads * splits)
-};
 
 struct TreeArgs {
   const float* q;
@@ -60,19 +50,30 @@ struct TreeArgs {
   uint32_t n_seq, n_heads, n_kv, group, hd;
   uint32_t rows_per_split;
   float scale;  // log2(e) / sqrt(hd)
-  TreeSeq seq[kTrSeqs];
+  const void* k[kTableSeqs];
+  const void* v[kTableSeqs];
+  const float* ks[kTableSeqs];
+  const float* vs[kTableSeqs];
+  uint32_t past[kTableSeqs];
+  uint32_t tokens[kTableSeqs];
+  uint32_t tok0[kTableSeqs];   // first drafted token in q, mask and out
+  uint32_t item0[kTableSeqs];  // first work item
+  uint32_t part0[kTableSeqs];  // first partial state, in rows (a sequence has tokens * n_heads * splits)
 };
 
-__device__ __forceinline__ int find_seq(const TreeArgs& a, uint32_t item) {
-  int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.seq[mid].item0 <= item)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
+struct TreeSeq {
+  const void *k, *v;
+  const float *ks, *vs;
+  uint32_t past, tokens, tok0, item0, part0;
+  uint32_t splits;  // parts of the cache rows
+};
+
+__device__ __forceinline__ TreeSeq this_seq(const TreeArgs& a, uint32_t item) {
+  const int s = table_find(a.item0, a.n_seq, item);
+  TreeSeq q{table_at(a.k, s),      table_at(a.v, s),    table_at(a.ks, s),    table_at(a.vs, s),   table_at(a.past, s),
+            table_at(a.tokens, s), table_at(a.tok0, s), table_at(a.item0, s), table_at(a.part0, s), 0};
+  q.splits = (q.past + q.tokens + a.rows_per_split - 1) / a.rows_per_split;
+  return q;
 }
 
 // The mask word of drafted token i, cut to the sequence's tokens.
@@ -192,7 +193,7 @@ struct NarrowShape {
 };
 
 template <int HDP, int RB, bool Q8>
-__global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB == 1 ? 3 : HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
   using S = NarrowShape<HDP>;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[S::kBytes];
   __shared__ __attribute__((aligned(16))) float s_scale[4][64];  // per wave: K scales of 32 keys, V scales
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
   const int n = lane & 15, g = lane >> 4;
   uint16_t* s_v = reinterpret_cast<uint16_t*>(s_mem) + wave * S::kWaveHalves;
   const uint32_t kvh = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
-  const TreeSeq& sq = a.seq[find_seq(a, item)];
+  const TreeSeq sq = this_seq(a, item);
   const uint32_t split = item - sq.item0, hd = a.hd;
   const uint32_t rows = sq.tokens * a.group, total = sq.past + sq.tokens;
   const uint32_t kbeg = split * a.rows_per_split, kend = min(total, kbeg + a.rows_per_split);
@@ -214,39 +215,48 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_narrow_kernel(
   const unsigned char* vbase = static_cast<const unsigned char*>(sq.v) + head * kSize;
   Piece<Q8> kr[2][S::kSteps], vr[S::kPieces];
   float sc = 0.0f;  // lanes 0-31: K scale of key lane; 32-63: V scale of key lane - 32
+  const float* const scales = Q8 ? (lane < 32 ? sq.ks : sq.vs) + kvh : nullptr;
+  // V first: it is used first. The bases are opaque: added up per lane from
+  // tile to tile they would take two registers a piece.
+  constexpr uint32_t kRowPieces = HDP / 8;
+  constexpr bool kEvenRows = 64 % kRowPieces == 0;  // a wave's pieces are whole rows
+  const uint32_t ld32 = static_cast<uint32_t>(ld);
+  uint32_t voff[kEvenRows ? 1 : S::kPieces], koff[S::kSteps];
+#pragma unroll
+  for (int p = 0; p < (kEvenRows ? 1 : S::kPieces); p++)
+    voff[p] = ((p * 64u + lane) / kRowPieces * ld32 + min((p * 64u + lane) % kRowPieces * 8, hd - 8)) * kSize;
+#pragma unroll
+  for (int s = 0; s < S::kSteps; s++) koff[s] = (n * ld32 + min(s * 32u + g * 8, hd - 8)) * kSize;
   auto fetch = [&](uint32_t k0) {
     const unsigned char* kp = kbase + k0 * ld * kSize;
     const unsigned char* vp = vbase + k0 * ld * kSize;
+    asm("" : "+s"(kp), "+s"(vp));
     if (k0 + 32 <= kend) {
+#pragma unroll
+      for (int p = 0; p < S::kPieces; p++)
+        vr[p].load(kEvenRows ? vp + p * (64 / kRowPieces) * ld * kSize : vp, voff[kEvenRows ? 0 : p]);
+      if constexpr (Q8) sc = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int s = 0; s < S::kSteps; s++)
-          kr[b][s].load(kp + b * 16 * ld * kSize,
-                        (n * static_cast<uint32_t>(ld) + min(s * 32u + g * 8, hd - 8)) * kSize);
-#pragma unroll
-      for (int p = 0; p < S::kPieces; p++) {
-        const uint32_t e = p * 64 + lane;
-        vr[p].load(vp, (e / (HDP / 8) * static_cast<uint32_t>(ld) + min(e % (HDP / 8) * 8, hd - 8)) * kSize);
-      }
+        for (int s = 0; s < S::kSteps; s++) kr[b][s].load(kp + b * 16 * ld * kSize, koff[s]);
     } else {  // keys past the end: K repeats the last (and is masked), V is 0
       const uint32_t last = kend - 1 - k0;
 #pragma unroll
+      for (int p = 0; p < S::kPieces; p++) {
+        const uint32_t e = p * 64u + lane, r = e / kRowPieces;
+        vr[p].zero();
+        if (r <= last) vr[p].load(vp, (r * ld32 + min(e % kRowPieces * 8, hd - 8)) * kSize);
+      }
+      if constexpr (Q8) {
+        sc = 0.0f;
+        if ((lane & 31u) <= last) sc = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
+      }
+#pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
         for (int s = 0; s < S::kSteps; s++)
-          kr[b][s].load(kp, (min(b * 16u + n, last) * static_cast<uint32_t>(ld) + min(s * 32u + g * 8, hd - 8)) * kSize);
-#pragma unroll
-      for (int p = 0; p < S::kPieces; p++) {
-        const uint32_t e = p * 64 + lane, r = e / (HDP / 8);
-        vr[p].load(vp, (min(r, last) * static_cast<uint32_t>(ld) + min(e % (HDP / 8) * 8, hd - 8)) * kSize);
-        if (r > last) vr[p].zero();
-      }
-    }
-    if constexpr (Q8) {
-      const uint32_t t = k0 + (lane & 31);
-      sc = 0.0f;
-      if (t < kend) sc = (lane < 32 ? sq.ks : sq.vs)[static_cast<size_t>(t) * a.n_kv + kvh];
+          kr[b][s].load(kp, (min(b * 16u + n, last) * ld32 + min(s * 32u + g * 8, hd - 8)) * kSize);
     }
   };
   uint32_t k0 = kbeg + wave * 32;
@@ -508,7 +518,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = lane & 31, h = lane >> 5;
   const uint32_t kvh = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
-  const TreeSeq& sq = a.seq[find_seq(a, item)];
+  const TreeSeq sq = this_seq(a, item);
   const uint32_t hd = a.hd, rows = sq.tokens * a.group, total = sq.past + sq.tokens;
   const uint32_t row_tiles = (rows + kWideRows - 1) / kWideRows;
   const uint32_t split = (item - sq.item0) / row_tiles, row0 = (item - sq.item0) % row_tiles * kWideRows;
@@ -523,12 +533,14 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   const unsigned char* kbase = static_cast<const unsigned char*>(sq.k) + head * kSize;
   const unsigned char* vbase = static_cast<const unsigned char*>(sq.v) + head * kSize;
   Piece<Q8> kr[S::kLoads], vr[S::kLoads];
-  float sc = 0.0f;  // lanes 0..BN-1: K scale of key lane; BN..2BN-1: V scales
+  float sc = 0.0f;  // lanes 0..BN-1: K scale of key lane; BN..2BN-1: V scales (the rest repeat them)
+  const float* const scales = Q8 ? (tid / BN % 2 == 0 ? sq.ks : sq.vs) + kvh : nullptr;
   auto fetch = [&](uint32_t k0) {
     const unsigned char* kp = kbase + k0 * ld * kSize;
     const unsigned char* vp = vbase + k0 * ld * kSize;
     const bool whole = k0 + BN <= kend;
-    const uint32_t last = whole ? BN - 1 : kend - 1 - k0;
+    const uint32_t last = whole ? BN - 1 : kend - 1 - k0;  // keys past the end repeat the last
+    if constexpr (Q8) sc = scales[static_cast<size_t>(k0 + min(tid % BN + 0u, last)) * a.n_kv];
 #pragma unroll
     for (int p = 0; p < S::kLoads; p++) {
       const uint32_t e = p * kTrNT + tid, r = e / S::kChunks;
@@ -536,15 +548,12 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
       kr[p].load(kp, off);
       vr[p].load(vp, off);
     }
-    if (!whole) {  // keys past the end: K repeats the last (and is masked), V is 0
+    if (!whole) {  // their V is 0 (K's scores are masked)
 #pragma unroll
       for (int p = 0; p < S::kLoads; p++)
         if ((p * kTrNT + tid) / S::kChunks > last) vr[p].zero();
-    }
-    if constexpr (Q8) {
-      const uint32_t t = k0 + tid % BN;
-      sc = 0.0f;
-      if (tid < 2 * BN && t < kend) sc = (tid < BN ? sq.ks : sq.vs)[static_cast<size_t>(t) * a.n_kv + kvh];
+      if constexpr (Q8)
+        if (tid % BN + 0u > last) sc = 0.0f;
     }
   };
   fetch(kbeg);  // (on its way while q is read)
@@ -735,17 +744,15 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
 }
 
 // ------------------------------------------------------------ joining the parts
-struct JoinSeq {
-  uint32_t row0;    // first (token, head) row of the sequence in this launch
-  uint32_t out0;    // its first row of out
-  uint32_t splits, part0;
-};
 struct JoinArgs {
   const float* part;
   size_t part_rows;
   float* out;
   uint32_t n_seq, n_rows, hd;
-  JoinSeq seq[kTrSeqs];
+  uint32_t row0[kTableSeqs];  // first (token, head) row of the sequence in this launch
+  uint32_t out0[kTableSeqs];  // its first row of out
+  uint32_t splits[kTableSeqs];
+  uint32_t part0[kTableSeqs];
 };
 
 // A row: M = max m_s, out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), by
@@ -755,19 +762,12 @@ struct JoinArgs {
 template <int T, int LANES>
 __global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
   constexpr int kBatch = 8, kPG = T / LANES, kWaves = T / 64;
-  const uint32_t r = blockIdx.x * (256 / T) + threadIdx.x / T, tid = threadIdx.x % T, lane = threadIdx.x & 63;
+  const uint32_t r = blockIdx.x * (256 / T) + __builtin_amdgcn_readfirstlane(threadIdx.x / T), tid = threadIdx.x % T, lane = threadIdx.x & 63;
   if (r >= a.n_rows) return;  // (whole waves; with T = 256 never)
-  int lo = 0, hi = static_cast<int>(a.n_seq) - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.seq[mid].row0 <= r)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const JoinSeq& sq = a.seq[lo];
-  const uint32_t row = r - sq.row0, ns = sq.splits;
-  const size_t p0 = sq.part0 + static_cast<size_t>(row) * ns;
+  const int si = table_find(a.row0, a.n_seq, r);
+  const uint32_t row = r - table_at(a.row0, si), ns = table_at(a.splits, si);
+  const size_t out_row = static_cast<size_t>(table_at(a.out0, si)) + row;
+  const size_t p0 = table_at(a.part0, si) + static_cast<size_t>(row) * ns;
   const float2* ml = reinterpret_cast<const float2*>(a.part + a.part_rows * a.hd) + p0;
   const uint32_t d = (tid % LANES) * 4, s0 = tid / LANES;
   const float* src = a.part + p0 * a.hd + min(d, a.hd - 4);
@@ -824,7 +824,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
   }
   if (tid < LANES && d < a.hd) {
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    *reinterpret_cast<float4*>(a.out + (static_cast<size_t>(sq.out0) + row) * a.hd + d) =
+    *reinterpret_cast<float4*>(a.out + out_row * a.hd + d) =
         make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
   }
 }
@@ -854,23 +854,38 @@ struct Plan {
   size_t floats;
 };
 
-// Cache rows of a part: as many workgroups as keep the card busy (kParts of
-// them), in whole tiles, but no part shorter than kLeast rows.
+// Workgroups that run at once: 256 compute units times those whose registers
+// fit one (the kernels' launch bounds).
+size_t resident(Width w, size_t hd) {
+  const size_t per_cu = w == kNarrow16 ? (hd <= 64 ? 4 : hd <= 128 ? 3 : 1) : hd <= 128 ? 2 : 1;
+  return 256 * per_cu;
+}
+
+// Cache rows of a part, per kernel: the fewest, in whole tiles, that leave no
+// more workgroups than run at once (a few left over for a second round would
+// take as long as all of the first), but no fewer than kLeast.
 Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd) {
-  constexpr size_t kParts = 768, kLeast = 128;
+  constexpr size_t kLeast = 128;
   const size_t group = n_heads / n_kv;
-  size_t work[kWidths] = {};  // cache rows times row tiles
-  for (size_t i = 0; i < n_seq; i++) {
-    if (!n_tree[i]) continue;
+  auto tiles = [&](size_t i) {
     const size_t rows = n_tree[i] * group;
-    const Width w = width_of(rows, hd);
-    work[w] += (past[i] + n_tree[i]) * (w == kWide ? (rows + kWideRows - 1) / kWideRows : 1);
-  }
+    return width_of(rows, hd) == kWide ? (rows + kWideRows - 1) / kWideRows : 1;
+  };
+  size_t work[kWidths] = {};  // cache rows times row tiles
+  for (size_t i = 0; i < n_seq; i++)
+    if (n_tree[i]) work[width_of(n_tree[i] * group, hd)] += (past[i] + n_tree[i]) * tiles(i);
   Plan p{};
   for (int w = 0; w < kWidths; w++) {
-    const size_t unit = w == kWide ? 64 : 128;
-    const size_t r = std::max(kLeast, work[w] * n_kv / kParts);
-    p.rows_per_split[w] = (r + unit - 1) / unit * unit;
+    const size_t unit = w == kWide ? 64 : 128, most = resident(static_cast<Width>(w), hd);
+    size_t r = std::max(kLeast, (work[w] * n_kv / most + unit - 1) / unit * unit);
+    for (int tries = 0; tries < 16; tries++) {
+      size_t n = 0;
+      for (size_t i = 0; i < n_seq; i++)
+        if (n_tree[i] && width_of(n_tree[i] * group, hd) == w) n += (past[i] + n_tree[i] + r - 1) / r * tiles(i);
+      if (n * n_kv <= most) break;
+      r += std::max(unit, r / 16 / unit * unit);
+    }
+    p.rows_per_split[w] = r;
   }
   for (size_t i = 0; i < n_seq; i++) {
     if (!n_tree[i]) continue;
@@ -967,16 +982,26 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
       const size_t rows = n_tree[i] * a.group;
       if (width_of(rows, head_dim) != w) continue;
       const size_t splits = (past[i] + n_tree[i] + plan.rows_per_split[w] - 1) / plan.rows_per_split[w];
-      if (a.n_seq == kTrSeqs)
+      if (a.n_seq == kTableSeqs)
         if (int rc = flush()) return rc;
-      TreeSeq& t = a.seq[a.n_seq++];
-      t = TreeSeq{kv[i].k, kv[i].v, kv[i].k_scales, kv[i].v_scales, static_cast<uint32_t>(past[i]),
-                  static_cast<uint32_t>(n_tree[i]), static_cast<uint32_t>(tok0), static_cast<uint32_t>(items),
-                  static_cast<uint32_t>(splits), static_cast<uint32_t>(part0)};
+      const uint32_t e = a.n_seq++;
+      a.k[e] = kv[i].k;
+      a.v[e] = kv[i].v;
+      a.ks[e] = kv[i].k_scales;
+      a.vs[e] = kv[i].v_scales;
+      a.past[e] = static_cast<uint32_t>(past[i]);
+      a.tokens[e] = static_cast<uint32_t>(n_tree[i]);
+      a.tok0[e] = static_cast<uint32_t>(tok0);
+      a.item0[e] = static_cast<uint32_t>(items);
+      a.part0[e] = static_cast<uint32_t>(part0);
       items += splits * (w == kWide ? (rows + kWideRows - 1) / kWideRows : 1);
       if (splits > 1) {
         most_splits = std::max(most_splits, splits);
-        j.seq[j.n_seq++] = JoinSeq{j.n_rows, static_cast<uint32_t>(tok0 * n_heads), t.splits, t.part0};
+        const uint32_t f = j.n_seq++;
+        j.row0[f] = j.n_rows;
+        j.out0[f] = static_cast<uint32_t>(tok0 * n_heads);
+        j.splits[f] = static_cast<uint32_t>(splits);
+        j.part0[f] = static_cast<uint32_t>(part0);
         j.n_rows += static_cast<uint32_t>(n_tree[i] * n_heads);
         part0 += n_tree[i] * n_heads * splits;
       }
