@@ -189,15 +189,17 @@ struct NarrowShape {
   static constexpr int kLdV = HDP + 16;
   static constexpr int kWaveHalves = 32 * kLdV;
   static constexpr int kLdO = HDP + 4;  // joining the waves: floats per row
+  static constexpr int kLdQ = HDP + 8;  // q: 16 rows' reads of 16 bytes on different banks
   static constexpr int kBytes = std::max(4 * kWaveHalves * 2, 4 * 16 * kLdO * 4);
 };
 
 template <int HDP, int RB, bool Q8>
-__global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB == 1 ? 3 : HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
   using S = NarrowShape<HDP>;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[S::kBytes];
+  __shared__ __attribute__((aligned(16))) uint16_t s_q[2][16 * RB * S::kLdQ];  // the halves of q
   __shared__ __attribute__((aligned(16))) float s_scale[4][64];  // per wave: K scales of 32 keys, V scales
-  __shared__ float s_m[4][16 * RB], s_l[4][16 * RB];
+  __shared__ float s_c[16 * RB], s_m[4][16 * RB], s_l[4][16 * RB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   uint16_t* s_v = reinterpret_cast<uint16_t*>(s_mem) + wave * S::kWaveHalves;
@@ -213,8 +215,8 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
   const size_t ld = static_cast<size_t>(a.n_kv) * hd, head = static_cast<size_t>(kvh) * hd;
   const unsigned char* kbase = static_cast<const unsigned char*>(sq.k) + head * kSize;
   const unsigned char* vbase = static_cast<const unsigned char*>(sq.v) + head * kSize;
-  Piece<Q8> kr[2][S::kSteps], vr[S::kPieces];
-  float sc = 0.0f;  // lanes 0-31: K scale of key lane; 32-63: V scale of key lane - 32
+  Piece<Q8> kr[2][S::kSteps], vr[S::kPieces];  // the next keys, on their way
+  float sr = 0.0f;  // lanes 0-31: K scale of key lane; 32-63: V scale of key lane - 32
   const float* const scales = Q8 ? (lane < 32 ? sq.ks : sq.vs) + kvh : nullptr;
   // V first: it is used first. The bases are opaque: added up per lane from
   // tile to tile they would take two registers a piece.
@@ -235,7 +237,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
 #pragma unroll
       for (int p = 0; p < S::kPieces; p++)
         vr[p].load(kEvenRows ? vp + p * (64 / kRowPieces) * ld * kSize : vp, voff[kEvenRows ? 0 : p]);
-      if constexpr (Q8) sc = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
+      if constexpr (Q8) sr = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -249,8 +251,8 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
         if (r <= last) vr[p].load(vp, (r * ld32 + min(e % kRowPieces * 8, hd - 8)) * kSize);
       }
       if constexpr (Q8) {
-        sc = 0.0f;
-        if ((lane & 31u) <= last) sc = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
+        sr = 0.0f;
+        if ((lane & 31u) <= last) sr = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
       }
 #pragma unroll
       for (int b = 0; b < 2; b++)
@@ -262,15 +264,23 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
   uint32_t k0 = kbeg + wave * 32;
   if (k0 < kend) fetch(k0);  // (on its way while q is read)
 
-  half8 qh[RB][S::kSteps], ql[RB][S::kSteps];
   float c[RB], m[RB], l[RB];
   uint64_t word[RB];
   f32x4 o[RB][S::kDimBlocks];
 #pragma unroll
   for (int r = 0; r < RB; r++) {
     const uint32_t row = min(r * 16u + n, rows - 1), i = row / a.group;
-    const size_t at = (static_cast<size_t>(sq.tok0) + i) * a.n_heads + kvh * a.group + row % a.group;
-    c[r] = load_q<S::kSteps, 32, 4>(a.q + at * hd, g * 8, hd, a.scale, qh[r], ql[r]);
+    if (wave == r) {
+      const size_t at = (static_cast<size_t>(sq.tok0) + i) * a.n_heads + kvh * a.group + row % a.group;
+      half8 qh[S::kSteps], ql[S::kSteps];
+      const float f = load_q<S::kSteps, 32, 4>(a.q + at * hd, g * 8, hd, a.scale, qh, ql);
+      if (g == 0) s_c[r * 16 + n] = f;
+#pragma unroll
+      for (int s = 0; s < S::kSteps; s++) {
+        *reinterpret_cast<half8*>(s_q[0] + (r * 16 + n) * S::kLdQ + s * 32 + g * 8) = qh[s];
+        *reinterpret_cast<half8*>(s_q[1] + (r * 16 + n) * S::kLdQ + s * 32 + g * 8) = ql[s];
+      }
+    }
     word[r] = mask_word(a, sq, i);
     m[r] = -INFINITY;
     l[r] = 0.0f;
@@ -279,8 +289,21 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
 #pragma unroll
       for (int j = 0; j < 4; j++) o[r][mb][j] = 0.0f;
   }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < RB; r++) c[r] = s_c[r * 16 + n];
   ScaleTop top;
   for (; k0 < kend; k0 += 128) {
+    // the next keys are under way while these are computed
+    Piece<Q8> kc[2][S::kSteps], vc[S::kPieces];
+#pragma unroll
+    for (int p = 0; p < S::kPieces; p++) vc[p] = vr[p];
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int s = 0; s < S::kSteps; s++) kc[b][s] = kr[b][s];
+    const float sc = sr;
+    if (k0 + 128 < kend) fetch(k0 + 128);
     const bool edge = k0 + 32 > min(sq.past, kend);  // not every row sees every key
     bool odd = false;
     if constexpr (!Q8) {
@@ -289,11 +312,11 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
       if (edge) {
         uint32_t bits = 0;
 #pragma unroll
-        for (int p = 0; p < S::kPieces; p++) bits |= odd_halves(vr[p].w);
+        for (int p = 0; p < S::kPieces; p++) bits |= odd_halves(vc[p].w);
         odd = __any((bits & kOddBits) != 0);
         if (odd) {
 #pragma unroll
-          for (int p = 0; p < S::kPieces; p++) vr[p].w = only_finite(vr[p].w);
+          for (int p = 0; p < S::kPieces; p++) vc[p].w = only_finite(vc[p].w);
         }
       }
     }
@@ -302,7 +325,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
 #pragma unroll
     for (int p = 0; p < S::kPieces; p++) {
       const int e = p * 64 + lane;
-      *reinterpret_cast<u32x4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vr[p].halves();
+      *reinterpret_cast<u32x4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vc[p].halves();
     }
     if constexpr (Q8) {
       s_scale[wave][lane] = sc;
@@ -331,19 +354,20 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
     for (int b = 0; b < 2; b++)
 #pragma unroll
       for (int t = 0; t < S::kSteps; t++) {
-        const half8 kf = __builtin_bit_cast(half8, kr[b][t].halves());
+        const half8 kf = __builtin_bit_cast(half8, kc[b][t].halves());
 #pragma unroll
         for (int r = 0; r < RB; r++) {
-          s[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[r][t], s[r][b], 0, 0, 0);
-          s2[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[r][t], s2[r][b], 0, 0, 0);
+          const uint16_t* qp = s_q[0] + (r * 16 + n) * S::kLdQ + t * 32 + g * 8;
+          const half8 qh = *reinterpret_cast<const half8*>(qp);
+          const half8 ql = *reinterpret_cast<const half8*>(qp + 16 * RB * S::kLdQ);
+          s[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh, s[r][b], 0, 0, 0);
+          s2[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql, s2[r][b], 0, 0, 0);
         }
       }
 #pragma unroll
     for (int r = 0; r < RB; r++)
 #pragma unroll
       for (int b = 0; b < 2; b++) s[r][b] += s2[r][b];
-    const uint32_t kcur = k0;
-    if (k0 + 128 < kend) fetch(k0 + 128);
 
     float ks[2][4], vs[2][4];
     if constexpr (Q8) {
@@ -368,7 +392,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
       }
       uint32_t seen = ~0u;  // bit 16 b + j: this row sees key b * 16 + 4g + j
       if (edge) {
-        const int first = static_cast<int>(kcur + 4 * g);
+        const int first = static_cast<int>(k0 + 4 * g);
         seen = static_cast<uint32_t>(seen_from(word[r], first - static_cast<int>(sq.past)));
         const int left = static_cast<int>(kend) - first;  // keys before the end of this part
         seen &= left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
@@ -420,7 +444,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 4 : HDP <= 128 && RB 
       }
     }
     if (odd) {  // rare
-      for (uint32_t t = kcur; t < min(kcur + 32, kend); t++)
+      for (uint32_t t = k0; t < min(k0 + 32, kend); t++)
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++) {
           const uint32_t d = mb * 16 + 4 * g;
@@ -857,7 +881,7 @@ struct Plan {
 // Workgroups that run at once: 256 compute units times those whose registers
 // fit one (the kernels' launch bounds).
 size_t resident(Width w, size_t hd) {
-  const size_t per_cu = w == kNarrow16 ? (hd <= 64 ? 4 : hd <= 128 ? 3 : 1) : hd <= 128 ? 2 : 1;
+  const size_t per_cu = w == kNarrow16 ? (hd <= 64 ? 3 : hd <= 128 ? 2 : 1) : hd <= 128 ? 2 : 1;
   return 256 * per_cu;
 }
 
