@@ -63,8 +63,135 @@ struct PkShape {
   static constexpr int kLoads = BN * kChunks / kPkNT;  // 16-byte pieces a lane stages of K (and of V)
 };
 
+// A row's q as the score product's operand, PIECES pieces of 8 dims, piece s at
+// dim s * STEP + d0: loaded raw first (so that the first tile's loads can
+// follow at once; loads return in order), then as halves, the f32 form as two
+// each, normalised. LANES: lanes (a power of two apart) that hold one row.
+template <int PIECES, int STEP, int LANES, bool HALF>
+struct QRow {
+  static constexpr int kWords = HALF ? 4 : 8;  // registers of 8 values
+  uint32_t raw[PIECES][kWords];
+  __device__ __forceinline__ void load(const void* q, size_t at, uint32_t d0, uint32_t hd) {
+#pragma unroll
+    for (int s = 0; s < PIECES; s++) {
+      const unsigned char* p =
+          static_cast<const unsigned char*>(q) + (at + min(s * STEP + d0, hd - 8)) * (HALF ? 2 : 4);
+#pragma unroll
+      for (int j = 0; j < kWords; j += 4) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(p + j * 4);
+        raw[s][j] = w.x;
+        raw[s][j + 1] = w.y;
+        raw[s][j + 2] = w.z;
+        raw[s][j + 3] = w.w;
+      }
+    }
+  }
+  // Returns what a score is multiplied with to be in log2 units.
+  __device__ __forceinline__ float halves(float scale, uint32_t d0, uint32_t hd, half8* qh, half8* ql) {
+#pragma unroll
+    for (int s = 0; s < PIECES; s++)
+      if (s * STEP + d0 >= hd)
+#pragma unroll
+        for (int j = 0; j < kWords; j++) raw[s][j] = 0;  // past the head's width
+    if constexpr (HALF) {
+#pragma unroll
+      for (int s = 0; s < PIECES; s++)
+        qh[s] = __builtin_bit_cast(half8, u32x4{raw[s][0], raw[s][1], raw[s][2], raw[s][3]});
+      return scale;
+    } else {
+      float amax = 0.0f;
+#pragma unroll
+      for (int s = 0; s < PIECES; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(__uint_as_float(raw[s][j])));
+#pragma unroll
+      for (int o = 64 / LANES; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+      const float f = row_factor(amax);
+#pragma unroll
+      for (int s = 0; s < PIECES; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          _Float16 xh, xl;
+          split_half(__uint_as_float(raw[s][j]) * f * scale, xh, xl);
+          qh[s][j] = xh;
+          ql[s][j] = xl;
+        }
+      return 1.0f / f;  // a power of two: exact
+    }
+  }
+};
+
+// The pieces of K and V rows k0 .. k0+BN-1 (of len) that a lane stages.
+// Addresses: a uniform base per tile and a lane's offset. Pieces past the
+// head's width repeat its last one (q is 0 there for K, and V columns there
+// are never stored).
+template <int BN, int CHUNKS>
+__device__ __forceinline__ void fetch_tile(const uint16_t* kb, const uint16_t* vb, size_t ld, uint32_t len, uint32_t k0,
+                                           uint32_t hd, u32x4* kr, u32x4* vr) {
+  constexpr int kLoads = BN * CHUNKS / kPkNT;
+  const unsigned char* kp = reinterpret_cast<const unsigned char*>(kb + k0 * ld);
+  const unsigned char* vp = reinterpret_cast<const unsigned char*>(vb + k0 * ld);
+  const bool whole = k0 + BN <= len;
+  const uint32_t last = whole ? BN - 1 : len - 1 - k0;
+#pragma unroll
+  for (int i = 0; i < kLoads; i++) {
+    const uint32_t e = i * kPkNT + threadIdx.x;
+    const uint64_t off = (static_cast<uint64_t>(min(e / CHUNKS, last)) * ld + min(e % CHUNKS * 8, hd - 8)) * 2;
+    kr[i] = *reinterpret_cast<const u32x4*>(kp + off);
+    vr[i] = *reinterpret_cast<const u32x4*>(vp + off);
+  }
+  if (!whole) {  // keys past the end: K repeats the last (and is masked), V is 0
+#pragma unroll
+    for (int i = 0; i < kLoads; i++)
+      if ((i * kPkNT + threadIdx.x) / CHUNKS > last) vr[i] = u32x4{0, 0, 0, 0};
+  }
+}
+
+// Puts a tile from registers into LDS, when every wave is done with the one
+// before. Where the tile reaches past some row's token (`edge`), a V value
+// that is not finite must not meet that row's zero probability: such values
+// stay out of the tile, and true is returned, for them to be added to the rows
+// that see them.
+template <int BN, int CHUNKS, int LD_K, int LD_V>
+__device__ __forceinline__ bool stage_tile(uint16_t* s_k, uint16_t* s_v, u32x4* kr, u32x4* vr, bool edge) {
+  constexpr int kLoads = BN * CHUNKS / kPkNT;
+  bool odd = false;
+  if (edge) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) bits |= odd_halves(vr[i]);
+    odd = __syncthreads_or((bits & kOddBits) != 0);
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) vr[i] = only_finite(vr[i]);
+    }
+  } else {
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; i++) {
+    const int e = i * kPkNT + threadIdx.x;
+    const int r = e / CHUNKS, d = (e % CHUNKS) * 8;
+    *reinterpret_cast<u32x4*>(s_k + r * LD_K + d) = kr[i];
+    *reinterpret_cast<u32x4*>(s_v + r * LD_V + d) = vr[i];
+  }
+  __syncthreads();
+  return odd;
+}
+
+template <bool HALF>
+__device__ __forceinline__ void store4(void* out, size_t at, float a, float b, float c, float d) {
+  if constexpr (HALF) {
+    const half4 y = {static_cast<_Float16>(a), static_cast<_Float16>(b), static_cast<_Float16>(c),
+                     static_cast<_Float16>(d)};
+    *reinterpret_cast<half4*>(static_cast<uint16_t*>(out) + at) = y;
+  } else {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(a, b, c, d);
+  }
+}
+
 template <int HDP, int BN, bool HALF>
-__global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(PackedArgs a) {
+__global__ __launch_bounds__(kPkNT, 2) void packed_kernel(PackedArgs a) {
   using S = PkShape<HDP, BN>;
   static_assert(BN * S::kChunks % kPkNT == 0, "a tile is a whole number of pieces per lane");
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
@@ -87,78 +214,14 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
   const uint32_t tok_last = min(row_w + 31, rows - 1) / a.group;
   const uint32_t hd = a.hd;
 
-  // Addresses: a uniform base per tile and a lane's 32-bit offset. Pieces past
-  // the head's width repeat its last one (q is 0 there for K, and V columns
-  // there are never stored).
+  QRow<S::kStepsQK, 16, 2, HALF> q;
+  q.load(a.q, (base + tok) * a.ld_q + static_cast<size_t>(head) * hd, h * 8, hd);
   const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   u32x4 kr[S::kLoads], vr[S::kLoads];
-  auto fetch = [&](uint32_t k0) {
-    const unsigned char* kp = reinterpret_cast<const unsigned char*>(kb + k0 * a.ld_kv);
-    const unsigned char* vp = reinterpret_cast<const unsigned char*>(vb + k0 * a.ld_kv);
-    const bool whole = k0 + BN <= len;
-    const uint32_t last = whole ? BN - 1 : len - 1 - k0;
-#pragma unroll
-    for (int i = 0; i < S::kLoads; i++) {
-      const uint32_t e = i * kPkNT + tid;
-      const uint64_t off = (static_cast<uint64_t>(min(e / S::kChunks, last)) * a.ld_kv +
-                            min(e % S::kChunks * 8, hd - 8)) * 2;
-      kr[i] = *reinterpret_cast<const u32x4*>(kp + off);
-      vr[i] = *reinterpret_cast<const u32x4*>(vp + off);
-    }
-    if (!whole) {  // keys past the end: K repeats the last (and is masked), V is 0
-#pragma unroll
-      for (int i = 0; i < S::kLoads; i++)
-        if ((i * kPkNT + tid) / S::kChunks > last) vr[i] = u32x4{0, 0, 0, 0};
-    }
-  };
-  fetch(0);  // (on its way while q is read)
-
-  // this row's q: operand B of the score product
+  fetch_tile<BN, S::kChunks>(kb, vb, a.ld_kv, len, 0, hd, kr, vr);
   half8 qh[S::kStepsQK], ql[HALF ? 1 : S::kStepsQK];
-  float c = a.scale;  // scores times c are in log2 units
-  if constexpr (HALF) {
-    const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (base + tok) * a.ld_q + static_cast<size_t>(head) * hd;
-#pragma unroll
-    for (int s = 0; s < S::kStepsQK; s++) {
-      const uint32_t d = s * 16 + h * 8;
-      u32x4 w = {0, 0, 0, 0};
-      if (d < hd) w = *reinterpret_cast<const u32x4*>(qp + d);
-      qh[s] = __builtin_bit_cast(half8, w);
-    }
-  } else {
-    const float* qp = static_cast<const float*>(a.q) + (base + tok) * a.ld_q + static_cast<size_t>(head) * hd;
-    float amax = 0.0f;
-#pragma unroll
-    for (int s = 0; s < S::kStepsQK; s++) {
-      const uint32_t d = s * 16 + h * 8;
-      if (d < hd) {
-        const float4 x = *reinterpret_cast<const float4*>(qp + d), y = *reinterpret_cast<const float4*>(qp + d + 4);
-        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-      }
-    }
-    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-    const float f = row_factor(amax);
-#pragma unroll
-    for (int s = 0; s < S::kStepsQK; s++) {
-      const uint32_t d = s * 16 + h * 8;
-      float x[8] = {};
-      if (d < hd) {
-        const float4 u = *reinterpret_cast<const float4*>(qp + d), w = *reinterpret_cast<const float4*>(qp + d + 4);
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        _Float16 xh, xl;
-        split_half(x[j] * f * a.scale, xh, xl);
-        qh[s][j] = xh;
-        ql[s][j] = xl;
-      }
-    }
-    c = 1.0f / f;  // a power of two: exact
-  }
+  const float c = q.halves(a.scale, h * 8, hd, qh, ql);
 
   f32x16 o[S::kDimBlocks];
 #pragma unroll
@@ -168,35 +231,10 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
   float m = -INFINITY, l = 0.0f;  // kept maximum (log2 units) and this lane's share of the sum
 
   for (uint32_t k0 = 0; k0 <= tok_last_wg; k0 += BN) {
-    // Where the tile reaches past some row's token, a V value that is not
-    // finite must not meet that row's zero probability: such values stay out
-    // of the tile and are added below to the rows that see them.
-    const bool diagonal = k0 + BN - 1 > tok_first_wg;
-    bool odd = false;
-    if (diagonal) {
-      uint32_t bits = 0;
-#pragma unroll
-      for (int i = 0; i < S::kLoads; i++) bits |= odd_halves(vr[i]);
-      odd = __syncthreads_or((bits & kOddBits) != 0);  // (also: every wave is done with the tile before)
-      if (odd) {
-#pragma unroll
-        for (int i = 0; i < S::kLoads; i++) vr[i] = only_finite(vr[i]);
-      }
-    } else {
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < S::kLoads; i++) {
-      const int e = i * kPkNT + tid;
-      const int r = e / S::kChunks, d = (e % S::kChunks) * 8;
-      *reinterpret_cast<u32x4*>(s_k + r * S::kLdK + d) = kr[i];
-      *reinterpret_cast<u32x4*>(s_v + r * S::kLdV + d) = vr[i];
-    }
-    __syncthreads();
-    if (k0 + BN <= tok_last_wg) fetch(k0 + BN);
+    const bool odd =
+        stage_tile<BN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, k0 + BN - 1 > tok_first_wg);
+    if (k0 + BN <= tok_last_wg) fetch_tile<BN, S::kChunks>(kb, vb, a.ld_kv, len, k0 + BN, hd, kr, vr);
     if (k0 > tok_last) continue;  // (the wave's rows see nothing of this tile)
-
-    // scores
     f32x16 s[S::kKeyBlocks];
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
@@ -237,23 +275,17 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        s[b][i] = exp2_hw(fmaf(s[b][i], c, -ms));
-        l += s[b][i];
-      }
-    // values
-#pragma unroll
-    for (int b = 0; b < S::kKeyBlocks; b++)
-#pragma unroll
       for (int t = 0; t < 2; t++) {
         half8 ph, pl;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
+          const float p = exp2_hw(fmaf(s[b][t * 8 + j], c, -ms));
+          l += p;
           if constexpr (HALF) {
-            ph[j] = static_cast<_Float16>(s[b][t * 8 + j]);
+            ph[j] = static_cast<_Float16>(p);
           } else {
             _Float16 xh, xl;
-            split_half(s[b][t * 8 + j], xh, xl);
+            split_half(p, xh, xl);
             ph[j] = xh;
             pl[j] = xl;
           }
@@ -295,26 +327,181 @@ __global__ __launch_bounds__(kPkNT, HDP <= 128 ? 2 : 1) void packed_kernel(Packe
     for (int g = 0; g < 4; g++) {
       const uint32_t d = mb * 32 + 8 * g + 4 * h;
       if (d >= hd) continue;
-      const size_t at = (base + tok) * a.ld_out + static_cast<size_t>(head) * hd + d;
-      if constexpr (HALF) {
-        half4 y;
-#pragma unroll
-        for (int j = 0; j < 4; j++) y[j] = static_cast<_Float16>(o[mb][4 * g + j] * inv);
-        *reinterpret_cast<half4*>(static_cast<uint16_t*>(a.out) + at) = y;
-      } else {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
-            make_float4(o[mb][4 * g] * inv, o[mb][4 * g + 1] * inv, o[mb][4 * g + 2] * inv, o[mb][4 * g + 3] * inv);
-      }
+      store4<HALF>(a.out, (base + tok) * a.ld_out + static_cast<size_t>(head) * hd + d, o[mb][4 * g] * inv,
+                   o[mb][4 * g + 1] * inv, o[mb][4 * g + 2] * inv, o[mb][4 * g + 3] * inv);
     }
 }
 
-template <int HDP, int BN>
+// ------------------------------------------------------------ heads wider than 128
+// 32 rows of such heads would fill the registers of a wave that runs alone on
+// its unit, with nothing to hide its waits behind. So a wave takes 16 rows
+// (16x16x32 products, twice the LDS reads per product) and a workgroup 64,
+// three of which run side by side; tiles of 32 keys.
+constexpr int kWideRows = 64, kWideBN = 32;
+
+template <int HDP>
+struct PkWideShape {
+  static constexpr int kSteps = HDP / 32, kDimBlocks = HDP / 16, kChunks = HDP / 8;
+  static constexpr int kLdK = HDP + 8;
+  static constexpr int kLdV = HDP + 16;  // 32-byte pieces of 8 rows on different banks
+  static constexpr int kLoads = kWideBN * kChunks / kPkNT;
+};
+
+template <int HDP, bool HALF>
+__global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
+  using S = PkWideShape<HDP>;
+  static_assert(kWideBN * S::kChunks % kPkNT == 0, "a tile is a whole number of pieces per lane");
+  __shared__ __attribute__((aligned(16))) uint16_t s_k[kWideBN * S::kLdK];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[kWideBN * S::kLdV];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const uint32_t kvh = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv;
+  const int sq = table_find(a.tile0, a.n_seq, tile);
+  const uint32_t len = table_at(a.len, sq), rows = len * a.group;
+  const uint32_t n_tiles = (rows + kWideRows - 1) / kWideRows;
+  const uint32_t row0 = (n_tiles - 1 - (tile - table_at(a.tile0, sq))) * kWideRows;
+  const size_t base = table_at(a.start, sq);
+  const uint32_t row_w = row0 + wave * 16;
+  const uint32_t row = min(row_w + n, rows - 1);
+  const uint32_t tok = row / a.group, head = kvh * a.group + row % a.group;
+  const uint32_t tok_first_wg = row0 / a.group;
+  const uint32_t tok_last_wg = (min(row0 + kWideRows, rows) - 1) / a.group;
+  const uint32_t tok_first = min(row_w, rows - 1) / a.group;
+  const uint32_t tok_last = min(row_w + 15, rows - 1) / a.group;
+  const uint32_t hd = a.hd;
+
+  QRow<S::kSteps, 32, 4, HALF> q;
+  q.load(a.q, (base + tok) * a.ld_q + static_cast<size_t>(head) * hd, g * 8, hd);
+  const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
+  const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
+  u32x4 kr[S::kLoads], vr[S::kLoads];
+  fetch_tile<kWideBN, S::kChunks>(kb, vb, a.ld_kv, len, 0, hd, kr, vr);
+  half8 qh[S::kSteps], ql[HALF ? 1 : S::kSteps];
+  const float c = q.halves(a.scale, g * 8, hd, qh, ql);
+
+  f32x4 o[S::kDimBlocks];
+#pragma unroll
+  for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[mb][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+
+  for (uint32_t k0 = 0; k0 <= tok_last_wg; k0 += kWideBN) {
+    const bool odd = stage_tile<kWideBN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr,
+                                                                       k0 + kWideBN - 1 > tok_first_wg);
+    if (k0 + kWideBN <= tok_last_wg)
+      fetch_tile<kWideBN, S::kChunks>(kb, vb, a.ld_kv, len, k0 + kWideBN, hd, kr, vr);
+    if (k0 > tok_last) continue;  // (the wave's rows see nothing of this tile)
+
+    f32x4 s[2], s2[2];  // (two chains of products each)
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[b][i] = s2[b][i] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < S::kSteps; t++)
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const half8 kf = *reinterpret_cast<const half8*>(s_k + (b * 16 + n) * S::kLdK + t * 32 + g * 8);
+        if constexpr (HALF) {
+          f32x4& x = t % 2 ? s2[b] : s[b];
+          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t], x, 0, 0, 0);
+        } else {
+          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t], s[b], 0, 0, 0);
+          s2[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t], s2[b], 0, 0, 0);
+        }
+      }
+#pragma unroll
+    for (int b = 0; b < 2; b++) s[b] += s2[b];
+    if (k0 + kWideBN - 1 > tok_first) {
+      const int lim = static_cast<int>(tok - k0) - 4 * g;
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (b * 16 + i > lim) s[b][i] = -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+    if (__any(mx > m + kLag)) {
+      const float mn = fmaxf(m, mx), al = exp2_hw(m - mn);
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[mb][i] *= al;
+    }
+    const float ms = HALF ? m : m - kPShift;
+    half8 ph, pl;
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float p = exp2_hw(fmaf(s[b][i], c, -ms));
+        l += p;
+        if constexpr (HALF) {
+          ph[b * 4 + i] = static_cast<_Float16>(p);
+        } else {
+          _Float16 xh, xl;
+          split_half(p, xh, xl);
+          ph[b * 4 + i] = xh;
+          pl[b * 4 + i] = xl;
+        }
+      }
+    const uint16_t* vp = s_v + (4 * g + (n >> 2)) * S::kLdV + (n & 3) * 4;
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++) {
+      const half8 vf = join(lds_read_tr(vp + mb * 16), lds_read_tr(vp + 16 * S::kLdV + mb * 16));
+      o[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[mb], 0, 0, 0);
+      if constexpr (!HALF) o[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[mb], 0, 0, 0);
+    }
+    if (odd) {  // rare: the values left out, for the rows that see them
+      for (uint32_t r = k0; r < min(k0 + kWideBN, len); r++) {
+        if (r > tok) break;
+#pragma unroll
+        for (int mb = 0; mb < S::kDimBlocks; mb++) {
+          const uint32_t d = mb * 16 + 4 * g;
+          const half4 x = *reinterpret_cast<const half4*>(vb + r * a.ld_kv + min(d, hd - 4));
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float v = static_cast<float>(x[j]);
+            o[mb][j] += fabsf(v) < INFINITY ? 0.0f : v;
+          }
+        }
+      }
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (row_w + n >= rows) return;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int mb = 0; mb < S::kDimBlocks; mb++) {
+    const uint32_t d = mb * 16 + 4 * g;
+    if (d < hd) {
+      const size_t at = (base + tok) * a.ld_out + static_cast<size_t>(head) * hd + d;
+      store4<HALF>(a.out, at, o[mb][0] * inv, o[mb][1] * inv, o[mb][2] * inv, o[mb][3] * inv);
+    }
+  }
+}
+
+template <int HDP>
 void launch_shape(const PackedArgs& a, bool half, uint32_t tiles, hipStream_t s) {
-  const dim3 grid(tiles * a.n_kv);
-  if (half)
-    hipLaunchKernelGGL((packed_kernel<HDP, BN, true>), grid, dim3(kPkNT), 0, s, a);
-  else
-    hipLaunchKernelGGL((packed_kernel<HDP, BN, false>), grid, dim3(kPkNT), 0, s, a);
+  const dim3 grid(tiles * a.n_kv), nt(kPkNT);
+  if constexpr (HDP <= 128) {
+    if (half)
+      hipLaunchKernelGGL((packed_kernel<HDP, 64, true>), grid, nt, 0, s, a);
+    else
+      hipLaunchKernelGGL((packed_kernel<HDP, 64, false>), grid, nt, 0, s, a);
+  } else {
+    if (half)
+      hipLaunchKernelGGL((packed_wide_kernel<HDP, true>), grid, nt, 0, s, a);
+    else
+      hipLaunchKernelGGL((packed_wide_kernel<HDP, false>), grid, nt, 0, s, a);
+  }
 }
 
 }  // namespace
@@ -345,12 +532,13 @@ int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v,
   }
   // the longest first: a workgroup's work grows with its place in its sequence
   std::stable_sort(seqs.begin(), seqs.end(), [](const Seq& x, const Seq& y) { return x.len > y.len; });
+  const size_t tile_rows = head_dim <= 128 ? kPkRows : kWideRows;
   const size_t most = 0x7fffffffu / n_kv_heads;  // tiles of one grid
   for (size_t i = 0; i < seqs.size();) {
     size_t tiles = 0;
     a.n_seq = 0;
     while (i < seqs.size() && a.n_seq < kTableSeqs) {
-      const size_t t = (seqs[i].len * a.group + kPkRows - 1) / kPkRows;
+      const size_t t = (seqs[i].len * a.group + tile_rows - 1) / tile_rows;
       if (a.n_seq && tiles + t > most) break;
       a.start[a.n_seq] = static_cast<uint32_t>(seqs[i].start);
       a.len[a.n_seq] = static_cast<uint32_t>(seqs[i].len);
@@ -360,15 +548,15 @@ int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v,
     }
     const uint32_t t = static_cast<uint32_t>(tiles);
     if (head_dim <= 64)
-      launch_shape<64, 64>(a, half, t, s);
+      launch_shape<64>(a, half, t, s);
     else if (head_dim <= 96)
-      launch_shape<96, 64>(a, half, t, s);
+      launch_shape<96>(a, half, t, s);
     else if (head_dim <= 128)
-      launch_shape<128, 64>(a, half, t, s);
+      launch_shape<128>(a, half, t, s);
     else if (head_dim <= 192)
-      launch_shape<192, 64>(a, half, t, s);
+      launch_shape<192>(a, half, t, s);
     else
-      launch_shape<256, 32>(a, half, t, s);
+      launch_shape<256>(a, half, t, s);
     PRANA_LAUNCH_CHECK();
   }
   return kOk;

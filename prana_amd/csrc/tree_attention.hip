@@ -594,6 +594,8 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   ScaleTop top;
 
   for (uint32_t k0 = kbeg; k0 < kend; k0 += BN) {
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++) keep_accumulator<(HDP > 128)>(o[mb]);
     const bool edge = k0 + BN > min(sq.past, kend);
     bool odd = false;
     if (!Q8 && edge) {
@@ -685,6 +687,8 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
 #pragma unroll
         for (int j = 0; j < 16; j++) o[mb][j] *= al;
     }
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++) keep_accumulator<(HDP > 128)>(o[mb]);
     const float ms = m == -INFINITY ? 0.0f : m - kPShift;
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
