@@ -64,19 +64,19 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 
 // round(|x| * 127 / amax) with ties up, exactly. In f32 the quotient is within
 // 127 * 3 * 2^-24 < 2.4e-5 of the real one, so a fraction further than 1e-4
-// from a half decides; otherwise (2 values in 10^4) it is taken in f64: |x| and
-// amax have 24 bits, so a quotient up to 127 that is not a tie is at least
-// 2^-33 from one, while the f64 evaluation is off by 2^-43 and the 2^-44 that
-// is added in relative terms (2^-37 at most) lifts exact ties over the half.
-__device__ __forceinline__ int quantize_exact(float x, float amax, float inv, bool fast) {
-  const float t = fabsf(x) * inv;
-  const float f = t - floorf(t);
-  float r = floorf(t + 0.5f);
-  if (!fast || fabsf(f - 0.5f) < 1e-4f) {
-    const double d = static_cast<double>(fabsf(x)) * 127.0 / static_cast<double>(amax);
-    r = static_cast<float>(floor(__fma_rn(d, 0x1p-44, d) + 0.5));
-  }
+// from a half decides (quantize_fast, whose second result is true otherwise);
+// the others (2 values in 10^4) are taken in f64: |x| and amax have 24 bits, so
+// a quotient up to 127 that is not a tie is at least 2^-33 from one, while the
+// f64 evaluation is off by 2^-43 and the 2^-44 that is added in relative terms
+// (2^-37 at most) lifts exact ties over the half.
+__device__ __forceinline__ int quantize_fast(float x, float inv, bool& close) {
+  const float t = fabsf(x) * inv, u = t + 0.5f, r = floorf(u);
+  close = close || fabsf(u - r - 0.5f) > 0.4999f;  // (u is within 1e-4 of a whole number)
   return static_cast<int>(copysignf(r, x));
+}
+__device__ __forceinline__ int quantize_exact(float x, float amax) {
+  const double d = static_cast<double>(fabsf(x)) * 127.0 / static_cast<double>(amax);
+  return static_cast<int>(copysignf(static_cast<float>(floor(__fma_rn(d, 0x1p-44, d) + 0.5)), x));
 }
 
 template <int LPH>
@@ -121,9 +121,26 @@ __global__ __launch_bounds__(kKvNT) void kv_write_kernel(KvArgs a) {
     if (item >= n_items) continue;
     uint32_t w[2] = {0, 0};
     if (finite && top) {
+      bool close = !fast;
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        w[j / 4] |= static_cast<uint32_t>(quantize_exact(x[it][j], amax, inv, fast) & 0xff) << (8 * (j % 4));
+        w[j / 4] |= static_cast<uint32_t>(quantize_fast(x[it][j], inv, close) & 0xff) << (8 * (j % 4));
+      if (close) {
+        // (one value after another: unrolled, this branch would be most of the kernel's code)
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = x[it][j];
+        w[0] = w[1] = 0;
+#pragma unroll 1
+        for (int j = 0; j < 8; j++) {
+          const uint64_t b = static_cast<uint64_t>(quantize_exact(y[0], amax) & 0xff) << 56;
+          const uint64_t v = (static_cast<uint64_t>(w[1]) << 32 | w[0]) >> 8 | b;
+          w[0] = static_cast<uint32_t>(v);
+          w[1] = static_cast<uint32_t>(v >> 32);
+#pragma unroll
+          for (int i = 0; i < 7; i++) y[i] = y[i + 1];
+        }
+      }
     }
     if (!finite) scale = __uint_as_float(0x7fc00000u);  // reads back as NaN
     const size_t r = static_cast<size_t>(sq.first) + row;

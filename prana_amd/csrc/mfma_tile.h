@@ -80,4 +80,62 @@ __device__ __forceinline__ float row_factor(float amax) {
   return __builtin_ldexpf(1.0f, k < -126 ? -126 : k > 126 ? 126 : k);
 }
 
+// A row's q as the score product's operand, PIECES pieces of 8 dims, piece s at
+// dim s * STEP + d0: loaded raw first (so that the first tile's loads can
+// follow at once; loads return in order), then as halves, the f32 form as two
+// each, normalised. LANES: lanes (a power of two apart) that hold one row.
+template <int PIECES, int STEP, int LANES, bool HALF>
+struct QRow {
+  static constexpr int kWords = HALF ? 4 : 8;  // registers of 8 values
+  uint32_t raw[PIECES][kWords];
+  __device__ __forceinline__ void load(const void* q, size_t at, uint32_t d0, uint32_t hd) {
+#pragma unroll
+    for (int s = 0; s < PIECES; s++) {
+      const unsigned char* p =
+          static_cast<const unsigned char*>(q) + (at + min(s * STEP + d0, hd - 8)) * (HALF ? 2 : 4);
+#pragma unroll
+      for (int j = 0; j < kWords; j += 4) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(p + j * 4);
+        raw[s][j] = w.x;
+        raw[s][j + 1] = w.y;
+        raw[s][j + 2] = w.z;
+        raw[s][j + 3] = w.w;
+      }
+    }
+  }
+  // Returns what a score is multiplied with to be in log2 units.
+  __device__ __forceinline__ float halves(float scale, uint32_t d0, uint32_t hd, half8* qh, half8* ql) {
+#pragma unroll
+    for (int s = 0; s < PIECES; s++)
+      if (s * STEP + d0 >= hd)
+#pragma unroll
+        for (int j = 0; j < kWords; j++) raw[s][j] = 0;  // past the head's width
+    if constexpr (HALF) {
+#pragma unroll
+      for (int s = 0; s < PIECES; s++)
+        qh[s] = __builtin_bit_cast(half8, u32x4{raw[s][0], raw[s][1], raw[s][2], raw[s][3]});
+      return scale;
+    } else {
+      float amax = 0.0f;
+#pragma unroll
+      for (int s = 0; s < PIECES; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(__uint_as_float(raw[s][j])));
+#pragma unroll
+      for (int o = 64 / LANES; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+      const float f = row_factor(amax);
+#pragma unroll
+      for (int s = 0; s < PIECES; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          _Float16 xh, xl;
+          split_half(__uint_as_float(raw[s][j]) * f * scale, xh, xl);
+          qh[s][j] = xh;
+          ql[s][j] = xl;
+        }
+      return 1.0f / f;  // a power of two: exact
+    }
+  }
+};
+
 }  // namespace prana

@@ -63,89 +63,52 @@ struct PkShape {
   static constexpr int kLoads = BN * kChunks / kPkNT;  // 16-byte pieces a lane stages of K (and of V)
 };
 
-// A row's q as the score product's operand, PIECES pieces of 8 dims, piece s at
-// dim s * STEP + d0: loaded raw first (so that the first tile's loads can
-// follow at once; loads return in order), then as halves, the f32 form as two
-// each, normalised. LANES: lanes (a power of two apart) that hold one row.
-template <int PIECES, int STEP, int LANES, bool HALF>
-struct QRow {
-  static constexpr int kWords = HALF ? 4 : 8;  // registers of 8 values
-  uint32_t raw[PIECES][kWords];
-  __device__ __forceinline__ void load(const void* q, size_t at, uint32_t d0, uint32_t hd) {
-#pragma unroll
-    for (int s = 0; s < PIECES; s++) {
-      const unsigned char* p =
-          static_cast<const unsigned char*>(q) + (at + min(s * STEP + d0, hd - 8)) * (HALF ? 2 : 4);
-#pragma unroll
-      for (int j = 0; j < kWords; j += 4) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(p + j * 4);
-        raw[s][j] = w.x;
-        raw[s][j + 1] = w.y;
-        raw[s][j + 2] = w.z;
-        raw[s][j + 3] = w.w;
-      }
-    }
-  }
-  // Returns what a score is multiplied with to be in log2 units.
-  __device__ __forceinline__ float halves(float scale, uint32_t d0, uint32_t hd, half8* qh, half8* ql) {
-#pragma unroll
-    for (int s = 0; s < PIECES; s++)
-      if (s * STEP + d0 >= hd)
-#pragma unroll
-        for (int j = 0; j < kWords; j++) raw[s][j] = 0;  // past the head's width
-    if constexpr (HALF) {
-#pragma unroll
-      for (int s = 0; s < PIECES; s++)
-        qh[s] = __builtin_bit_cast(half8, u32x4{raw[s][0], raw[s][1], raw[s][2], raw[s][3]});
-      return scale;
-    } else {
-      float amax = 0.0f;
-#pragma unroll
-      for (int s = 0; s < PIECES; s++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(__uint_as_float(raw[s][j])));
-#pragma unroll
-      for (int o = 64 / LANES; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-      const float f = row_factor(amax);
-#pragma unroll
-      for (int s = 0; s < PIECES; s++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          _Float16 xh, xl;
-          split_half(__uint_as_float(raw[s][j]) * f * scale, xh, xl);
-          qh[s][j] = xh;
-          ql[s][j] = xl;
-        }
-      return 1.0f / f;  // a power of two: exact
-    }
-  }
-};
-
 // The pieces of K and V rows k0 .. k0+BN-1 (of len) that a lane stages.
-// Addresses: a uniform base per tile and a lane's offset. Pieces past the
+// Addresses: a uniform base per tile and piece, and a lane's 32-bit offset that
+// stays (the base is opaque: added up per lane from tile to tile the addresses
+// would take two registers a piece and as many additions). Pieces past the
 // head's width repeat its last one (q is 0 there for K, and V columns there
 // are never stored).
 template <int BN, int CHUNKS>
-__device__ __forceinline__ void fetch_tile(const uint16_t* kb, const uint16_t* vb, size_t ld, uint32_t len, uint32_t k0,
-                                           uint32_t hd, u32x4* kr, u32x4* vr) {
-  constexpr int kLoads = BN * CHUNKS / kPkNT;
-  const unsigned char* kp = reinterpret_cast<const unsigned char*>(kb + k0 * ld);
-  const unsigned char* vp = reinterpret_cast<const unsigned char*>(vb + k0 * ld);
-  const bool whole = k0 + BN <= len;
-  const uint32_t last = whole ? BN - 1 : len - 1 - k0;
-#pragma unroll
-  for (int i = 0; i < kLoads; i++) {
-    const uint32_t e = i * kPkNT + threadIdx.x;
-    const uint64_t off = (static_cast<uint64_t>(min(e / CHUNKS, last)) * ld + min(e % CHUNKS * 8, hd - 8)) * 2;
-    kr[i] = *reinterpret_cast<const u32x4*>(kp + off);
-    vr[i] = *reinterpret_cast<const u32x4*>(vp + off);
+struct TileFetch {
+  static constexpr int kLoads = BN * CHUNKS / kPkNT;
+  static constexpr bool kEven = kPkNT % CHUNKS == 0;  // a workgroup's pieces are whole rows
+  const unsigned char *kb, *vb;
+  size_t ld;  // bytes
+  uint32_t len, hd;
+  uint32_t off[kEven ? 1 : kLoads];
+  __device__ __forceinline__ uint32_t offset(uint32_t e, uint32_t last) const {
+    return min(e / CHUNKS, last) * static_cast<uint32_t>(ld) + min(e % CHUNKS * 8, hd - 8) * 2;
   }
-  if (!whole) {  // keys past the end: K repeats the last (and is masked), V is 0
+  __device__ __forceinline__ TileFetch(const uint16_t* k, const uint16_t* v, size_t ld_, uint32_t len_, uint32_t hd_)
+      : kb(reinterpret_cast<const unsigned char*>(k)), vb(reinterpret_cast<const unsigned char*>(v)), ld(ld_ * 2),
+        len(len_), hd(hd_) {
 #pragma unroll
-    for (int i = 0; i < kLoads; i++)
-      if ((i * kPkNT + threadIdx.x) / CHUNKS > last) vr[i] = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < (kEven ? 1 : kLoads); i++) off[i] = offset(i * kPkNT + threadIdx.x, BN);
   }
-}
+  __device__ __forceinline__ void operator()(uint32_t k0, u32x4* kr, u32x4* vr) const {
+    const unsigned char* kp = kb + k0 * ld;
+    const unsigned char* vp = vb + k0 * ld;
+    asm("" : "+s"(kp), "+s"(vp));
+    if (k0 + BN <= len) {
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const size_t up = kEven ? i * (kPkNT / CHUNKS) * ld : 0;
+        kr[i] = *reinterpret_cast<const u32x4*>(kp + up + off[kEven ? 0 : i]);
+        vr[i] = *reinterpret_cast<const u32x4*>(vp + up + off[kEven ? 0 : i]);
+      }
+    } else {  // keys past the end: K repeats the last (and is masked), V is 0
+      const uint32_t last = len - 1 - k0;
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const uint32_t e = i * kPkNT + threadIdx.x, at = offset(e, last);
+        kr[i] = *reinterpret_cast<const u32x4*>(kp + at);
+        vr[i] = u32x4{0, 0, 0, 0};
+        if (e / CHUNKS <= last) vr[i] = *reinterpret_cast<const u32x4*>(vp + at);
+      }
+    }
+  }
+};
 
 // Puts a tile from registers into LDS, when every wave is done with the one
 // before. Where the tile reaches past some row's token (`edge`), a V value
@@ -191,7 +154,7 @@ __device__ __forceinline__ void store4(void* out, size_t at, float a, float b, f
 }
 
 template <int HDP, int BN, bool HALF>
-__global__ __launch_bounds__(kPkNT, 2) void packed_kernel(PackedArgs a) {
+__global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(PackedArgs a) {
   using S = PkShape<HDP, BN>;
   static_assert(BN * S::kChunks % kPkNT == 0, "a tile is a whole number of pieces per lane");
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
@@ -219,7 +182,8 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_kernel(PackedArgs a) {
   const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   u32x4 kr[S::kLoads], vr[S::kLoads];
-  fetch_tile<BN, S::kChunks>(kb, vb, a.ld_kv, len, 0, hd, kr, vr);
+  const TileFetch<BN, S::kChunks> fetch(kb, vb, a.ld_kv, len, hd);
+  fetch(0, kr, vr);
   half8 qh[S::kStepsQK], ql[HALF ? 1 : S::kStepsQK];
   const float c = q.halves(a.scale, h * 8, hd, qh, ql);
 
@@ -233,7 +197,7 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_kernel(PackedArgs a) {
   for (uint32_t k0 = 0; k0 <= tok_last_wg; k0 += BN) {
     const bool odd =
         stage_tile<BN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, k0 + BN - 1 > tok_first_wg);
-    if (k0 + BN <= tok_last_wg) fetch_tile<BN, S::kChunks>(kb, vb, a.ld_kv, len, k0 + BN, hd, kr, vr);
+    if (k0 + BN <= tok_last_wg) fetch(k0 + BN, kr, vr);
     if (k0 > tok_last) continue;  // (the wave's rows see nothing of this tile)
     f32x16 s[S::kKeyBlocks];
 #pragma unroll
@@ -375,7 +339,8 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
   const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   u32x4 kr[S::kLoads], vr[S::kLoads];
-  fetch_tile<kWideBN, S::kChunks>(kb, vb, a.ld_kv, len, 0, hd, kr, vr);
+  const TileFetch<kWideBN, S::kChunks> fetch(kb, vb, a.ld_kv, len, hd);
+  fetch(0, kr, vr);
   half8 qh[S::kSteps], ql[HALF ? 1 : S::kSteps];
   const float c = q.halves(a.scale, g * 8, hd, qh, ql);
 
@@ -389,8 +354,7 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
   for (uint32_t k0 = 0; k0 <= tok_last_wg; k0 += kWideBN) {
     const bool odd = stage_tile<kWideBN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr,
                                                                        k0 + kWideBN - 1 > tok_first_wg);
-    if (k0 + kWideBN <= tok_last_wg)
-      fetch_tile<kWideBN, S::kChunks>(kb, vb, a.ld_kv, len, k0 + kWideBN, hd, kr, vr);
+    if (k0 + kWideBN <= tok_last_wg) fetch(k0 + kWideBN, kr, vr);
     if (k0 > tok_last) continue;  // (the wave's rows see nothing of this tile)
 
     f32x4 s[2], s2[2];  // (two chains of products each)

@@ -12,6 +12,8 @@ namespace {
 
 constexpr size_t kMaxRows = size_t{1} << 30;  // rows of one sequence: row and key indices fit 32 bits
 
+constexpr size_t kMaxStride = size_t{1} << 24;  // row strides: 63 rows' bytes fit 32 bits
+
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int refuse(const char* what, const std::string& why) { return fail(kErrInvalid, std::string(what) + ": " + why); }
@@ -49,7 +51,7 @@ int check_attention_packed(const void* q, const uint16_t* k, const uint16_t* v, 
   if (ld_q % per16 || ld_out % per16 || ld_kv % 8) return refuse(what, "row strides must be multiples of 16 bytes");
   if (ld_q < n_heads * head_dim || ld_out < n_heads * head_dim || ld_kv < n_kv_heads * head_dim)
     return refuse(what, "a row stride is shorter than its row");
-  if (ld_q > kMaxRows || ld_out > kMaxRows || ld_kv > kMaxRows) return refuse(what, "a row stride is too long");
+  if (ld_q > kMaxStride || ld_out > kMaxStride || ld_kv > kMaxStride) return refuse(what, "a row stride is too long");
   return kOk;
 }
 
@@ -74,7 +76,7 @@ int check_kv_q8(const char* what, const prana_kv* kv, const size_t* first_rows, 
   if (total == 0) return kOk;
   if (!k || !v) return refuse(what, "null buffer");
   if (!aligned(k, 16) || !aligned(v, 16)) return refuse(what, "buffers must be 16-byte aligned");
-  if (ld > kMaxRows) return refuse(what, "row stride too long");
+  if (ld > kMaxStride) return refuse(what, "row stride too long");
   if (ld * size % 16) return refuse(what, "row stride must be a multiple of 16 bytes");
   if (ld < n_kv_heads * head_dim) return refuse(what, "row stride shorter than a row");
   return kOk;

@@ -14,7 +14,7 @@
 // multiplies its scores, its V scale its probabilities.
 //
 // Two kernels, by the rows of a sequence and KV head:
-//   narrow (up to 32 rows): bound by reading the cache. The four waves of a
+//   narrow (up to 32 rows): bound by reading the cache. The eight waves of a
 //     workgroup share the rows and take different keys, 32 at a time: K goes
 //     from memory straight into the operand's registers, V through a corner of
 //     LDS that only its wave uses, so no wave waits for another until the end.
@@ -126,42 +126,6 @@ struct Piece<true> {
   __device__ __forceinline__ u32x4 halves() const { return i8_to_halves(w); }
 };
 
-// A row's q as the score product's operand: PIECES pieces of 8 dims, piece s
-// at dim s * STEP + d0, as two halves, normalised. Returns the factor that
-// brings the scores back (a power of two). LANES: lanes (a power of two apart)
-// that hold one row.
-template <int PIECES, int STEP, int LANES>
-__device__ __forceinline__ float load_q(const float* qp, uint32_t d0, uint32_t hd, float scale, half8* qh, half8* ql) {
-  float amax = 0.0f;
-  float x[PIECES][8];
-#pragma unroll
-  for (int s = 0; s < PIECES; s++) {
-    const uint32_t d = s * STEP + d0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[s][j] = 0.0f;
-    if (d < hd) {
-      const float4 u = *reinterpret_cast<const float4*>(qp + d), w = *reinterpret_cast<const float4*>(qp + d + 4);
-      x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
-      x[s][4] = w.x; x[s][5] = w.y; x[s][6] = w.z; x[s][7] = w.w;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[s][j]));
-  }
-#pragma unroll
-  for (int o = 64 / LANES; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-  const float f = row_factor(amax);
-#pragma unroll
-  for (int s = 0; s < PIECES; s++)
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      _Float16 xh, xl;
-      split_half(x[s][j] * f * scale, xh, xl);
-      qh[s][j] = xh;
-      ql[s][j] = xl;
-    }
-  return 1.0f / f;
-}
-
 // V scales of 8-bit caches are taken relative to a power of two no smaller
 // than any scale met so far, so that a probability times its scale stays below
 // 2^15 as the probability does.
@@ -181,8 +145,14 @@ struct ScaleTop {
 };
 
 // ------------------------------------------------------------ narrow: up to 16 RB rows
+// Waves of a workgroup: eight, or four of heads that take more than half of a
+// unit's registers.
+constexpr int narrow_waves(int hdp) { return hdp <= 128 ? 8 : 4; }
+
 template <int HDP>
 struct NarrowShape {
+  static constexpr int kWaves = narrow_waves(HDP), kNT = 64 * kWaves;
+  static constexpr int kRound = 32 * kWaves;  // keys of a workgroup at a time
   static constexpr int kSteps = HDP / 32, kDimBlocks = HDP / 16, kPieces = HDP / 16;
   // V rows an odd multiple of 32 bytes apart: the 32-byte pieces of 8 rows
   // that a transposing read takes at a time fall on different banks
@@ -190,16 +160,24 @@ struct NarrowShape {
   static constexpr int kWaveHalves = 32 * kLdV;
   static constexpr int kLdO = HDP + 4;  // joining the waves: floats per row
   static constexpr int kLdQ = HDP + 8;  // q: 16 rows' reads of 16 bytes on different banks
-  static constexpr int kBytes = std::max(4 * kWaveHalves * 2, 4 * 16 * kLdO * 4);
+  static constexpr int kBytes = kWaves * std::max(kWaveHalves * 2, 16 * kLdO * 4);
 };
 
+template <bool FIRST, class T>
+__device__ __forceinline__ T& pick_pieces(T& a, T& b) {
+  if constexpr (FIRST)
+    return a;
+  else
+    return b;
+}
+
 template <int HDP, int RB, bool Q8>
-__global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
   using S = NarrowShape<HDP>;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[S::kBytes];
   __shared__ __attribute__((aligned(16))) uint16_t s_q[2][16 * RB * S::kLdQ];  // the halves of q
-  __shared__ __attribute__((aligned(16))) float s_scale[4][64];  // per wave: K scales of 32 keys, V scales
-  __shared__ float s_c[16 * RB], s_m[4][16 * RB], s_l[4][16 * RB];
+  __shared__ __attribute__((aligned(16))) float s_scale[S::kWaves][64];  // per wave: K scales of 32 keys, V scales
+  __shared__ float s_c[16 * RB], s_m[S::kWaves][16 * RB], s_l[S::kWaves][16 * RB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   uint16_t* s_v = reinterpret_cast<uint16_t*>(s_mem) + wave * S::kWaveHalves;
@@ -229,20 +207,15 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
     voff[p] = ((p * 64u + lane) / kRowPieces * ld32 + min((p * 64u + lane) % kRowPieces * 8, hd - 8)) * kSize;
 #pragma unroll
   for (int s = 0; s < S::kSteps; s++) koff[s] = (n * ld32 + min(s * 32u + g * 8, hd - 8)) * kSize;
-  auto fetch = [&](uint32_t k0) {
-    const unsigned char* kp = kbase + k0 * ld * kSize;
+  auto fetch_v = [&](uint32_t k0) {
     const unsigned char* vp = vbase + k0 * ld * kSize;
-    asm("" : "+s"(kp), "+s"(vp));
+    asm("" : "+s"(vp));
     if (k0 + 32 <= kend) {
 #pragma unroll
       for (int p = 0; p < S::kPieces; p++)
         vr[p].load(kEvenRows ? vp + p * (64 / kRowPieces) * ld * kSize : vp, voff[kEvenRows ? 0 : p]);
       if constexpr (Q8) sr = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
-#pragma unroll
-      for (int b = 0; b < 2; b++)
-#pragma unroll
-        for (int s = 0; s < S::kSteps; s++) kr[b][s].load(kp + b * 16 * ld * kSize, koff[s]);
-    } else {  // keys past the end: K repeats the last (and is masked), V is 0
+    } else {  // keys past the end: V is 0
       const uint32_t last = kend - 1 - k0;
 #pragma unroll
       for (int p = 0; p < S::kPieces; p++) {
@@ -254,6 +227,18 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
         sr = 0.0f;
         if ((lane & 31u) <= last) sr = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
       }
+    }
+  };
+  auto fetch_k = [&](uint32_t k0) {
+    const unsigned char* kp = kbase + k0 * ld * kSize;
+    asm("" : "+s"(kp));
+    if (k0 + 32 <= kend) {
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int s = 0; s < S::kSteps; s++) kr[b][s].load(kp + b * 16 * ld * kSize, koff[s]);
+    } else {  // keys past the end repeat the last (and are masked)
+      const uint32_t last = kend - 1 - k0;
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -261,26 +246,35 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
           kr[b][s].load(kp, (min(b * 16u + n, last) * ld32 + min(s * 32u + g * 8, hd - 8)) * kSize);
     }
   };
+  // wave r reads the rows of block r, before the first keys: loads return in order
+  QRow<S::kSteps, 32, 4, false> q;
+  if (wave < RB) {
+    const uint32_t row = min(wave * 16u + n, rows - 1);
+    q.load(a.q, ((static_cast<size_t>(sq.tok0) + row / a.group) * a.n_heads + kvh * a.group + row % a.group) * hd,
+           g * 8, hd);
+  }
   uint32_t k0 = kbeg + wave * 32;
-  if (k0 < kend) fetch(k0);  // (on its way while q is read)
+  if (k0 < kend) {
+    fetch_v(k0);
+    fetch_k(k0);
+  }
+  if (wave < RB) {
+    half8 qh[S::kSteps], ql[S::kSteps];
+    const float f = q.halves(a.scale, g * 8, hd, qh, ql);
+    if (g == 0) s_c[wave * 16 + n] = f;
+#pragma unroll
+    for (int s = 0; s < S::kSteps; s++) {
+      *reinterpret_cast<half8*>(s_q[0] + (wave * 16 + n) * S::kLdQ + s * 32 + g * 8) = qh[s];
+      *reinterpret_cast<half8*>(s_q[1] + (wave * 16 + n) * S::kLdQ + s * 32 + g * 8) = ql[s];
+    }
+  }
 
   float c[RB], m[RB], l[RB];
   uint64_t word[RB];
   f32x4 o[RB][S::kDimBlocks];
 #pragma unroll
   for (int r = 0; r < RB; r++) {
-    const uint32_t row = min(r * 16u + n, rows - 1), i = row / a.group;
-    if (wave == r) {
-      const size_t at = (static_cast<size_t>(sq.tok0) + i) * a.n_heads + kvh * a.group + row % a.group;
-      half8 qh[S::kSteps], ql[S::kSteps];
-      const float f = load_q<S::kSteps, 32, 4>(a.q + at * hd, g * 8, hd, a.scale, qh, ql);
-      if (g == 0) s_c[r * 16 + n] = f;
-#pragma unroll
-      for (int s = 0; s < S::kSteps; s++) {
-        *reinterpret_cast<half8*>(s_q[0] + (r * 16 + n) * S::kLdQ + s * 32 + g * 8) = qh[s];
-        *reinterpret_cast<half8*>(s_q[1] + (r * 16 + n) * S::kLdQ + s * 32 + g * 8) = ql[s];
-      }
-    }
+    const uint32_t i = min(r * 16u + n, rows - 1) / a.group;
     word[r] = mask_word(a, sq, i);
     m[r] = -INFINITY;
     l[r] = 0.0f;
@@ -293,17 +287,26 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
 #pragma unroll
   for (int r = 0; r < RB; r++) c[r] = s_c[r * 16 + n];
   ScaleTop top;
-  for (; k0 < kend; k0 += 128) {
-    // the next keys are under way while these are computed
+  for (; k0 < kend; k0 += S::kRound) {
+    // One block of rows: the next keys are under way while these are computed.
+    // Two leave no registers for that: the next ones follow as these are used.
+    const bool more = k0 + S::kRound < kend;
     Piece<Q8> kc[2][S::kSteps], vc[S::kPieces];
+    float sc = sr;
+    if constexpr (RB == 1) {
 #pragma unroll
-    for (int p = 0; p < S::kPieces; p++) vc[p] = vr[p];
+      for (int p = 0; p < S::kPieces; p++) vc[p] = vr[p];
 #pragma unroll
-    for (int b = 0; b < 2; b++)
+      for (int b = 0; b < 2; b++)
 #pragma unroll
-      for (int s = 0; s < S::kSteps; s++) kc[b][s] = kr[b][s];
-    const float sc = sr;
-    if (k0 + 128 < kend) fetch(k0 + 128);
+        for (int s = 0; s < S::kSteps; s++) kc[b][s] = kr[b][s];
+      if (more) {
+        fetch_v(k0 + S::kRound);
+        fetch_k(k0 + S::kRound);
+      }
+    }
+    Piece<Q8>* const vu = RB == 1 ? vc : vr;
+    auto& ku = pick_pieces<RB == 1>(kc, kr);
     const bool edge = k0 + 32 > min(sq.past, kend);  // not every row sees every key
     bool odd = false;
     if constexpr (!Q8) {
@@ -312,11 +315,11 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
       if (edge) {
         uint32_t bits = 0;
 #pragma unroll
-        for (int p = 0; p < S::kPieces; p++) bits |= odd_halves(vc[p].w);
+        for (int p = 0; p < S::kPieces; p++) bits |= odd_halves(vu[p].w);
         odd = __any((bits & kOddBits) != 0);
         if (odd) {
 #pragma unroll
-          for (int p = 0; p < S::kPieces; p++) vc[p].w = only_finite(vc[p].w);
+          for (int p = 0; p < S::kPieces; p++) vu[p].w = only_finite(vu[p].w);
         }
       }
     }
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
 #pragma unroll
     for (int p = 0; p < S::kPieces; p++) {
       const int e = p * 64 + lane;
-      *reinterpret_cast<u32x4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vc[p].halves();
+      *reinterpret_cast<u32x4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vu[p].halves();
     }
     if constexpr (Q8) {
       s_scale[wave][lane] = sc;
@@ -343,6 +346,8 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 
+    if constexpr (RB > 1)
+      if (more) fetch_v(k0 + S::kRound);
     f32x4 s[RB][2], s2[RB][2];  // from both halves of q
 #pragma unroll
     for (int r = 0; r < RB; r++)
@@ -354,7 +359,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
     for (int b = 0; b < 2; b++)
 #pragma unroll
       for (int t = 0; t < S::kSteps; t++) {
-        const half8 kf = __builtin_bit_cast(half8, kc[b][t].halves());
+        const half8 kf = __builtin_bit_cast(half8, ku[b][t].halves());
 #pragma unroll
         for (int r = 0; r < RB; r++) {
           const uint16_t* qp = s_q[0] + (r * 16 + n) * S::kLdQ + t * 32 + g * 8;
@@ -364,6 +369,8 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
           s2[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql, s2[r][b], 0, 0, 0);
         }
       }
+    if constexpr (RB > 1)
+      if (more) fetch_k(k0 + S::kRound);
 #pragma unroll
     for (int r = 0; r < RB; r++)
 #pragma unroll
@@ -478,7 +485,9 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
   for (int r = 0; r < RB; r++) {
     if (r) __syncthreads();
     const int i = r * 16 + n;
-    const float M = fmaxf(fmaxf(s_m[0][i], s_m[1][i]), fmaxf(s_m[2][i], s_m[3][i]));
+    float M = s_m[0][i];
+#pragma unroll
+    for (int w = 1; w < S::kWaves; w++) M = fmaxf(M, s_m[w][i]);
     float f = m[r] == -INFINITY ? 0.0f : exp2_hw(m[r] - M);
     if constexpr (Q8) f *= top.top;
 #pragma unroll
@@ -488,16 +497,18 @@ __global__ __launch_bounds__(kTrNT, HDP <= 64 && RB == 1 ? 3 : HDP <= 128 ? 2 : 
           make_float4(o[r][mb][0] * f, o[r][mb][1] * f, o[r][mb][2] * f, o[r][mb][3] * f);
     }
     __syncthreads();
-    for (int e = tid; e < 16 * (HDP / 4); e += kTrNT) {
+    for (int e = tid; e < 16 * (HDP / 4); e += S::kNT) {
       const int rr = e / (HDP / 4);
       const uint32_t d = (e % (HDP / 4)) * 4, row = r * 16 + rr;
       if (row >= rows || d >= hd) continue;
       float4 y = make_float4(0, 0, 0, 0);
       const int ri = r * 16 + rr;
-      const float top_m = fmaxf(fmaxf(s_m[0][ri], s_m[1][ri]), fmaxf(s_m[2][ri], s_m[3][ri]));
+      float top_m = s_m[0][ri];
+#pragma unroll
+      for (int w = 1; w < S::kWaves; w++) top_m = fmaxf(top_m, s_m[w][ri]);
       float L = 0.0f;
 #pragma unroll
-      for (int w = 0; w < 4; w++) {
+      for (int w = 0; w < S::kWaves; w++) {
         const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 16 + rr) * S::kLdO + d);
         y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
         if (s_m[w][ri] != -INFINITY) L = fmaf(s_l[w][ri], exp2_hw(s_m[w][ri] - top_m), L);
@@ -580,11 +591,11 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
         if (tid % BN + 0u > last) sc = 0.0f;
     }
   };
-  fetch(kbeg);  // (on its way while q is read)
-
+  QRow<S::kStepsQK, 16, 2, false> q;  // before the first keys: loads return in order
+  q.load(a.q, (static_cast<size_t>(sq.tok0) * a.n_heads + qrow) * hd, h * 8, hd);
+  fetch(kbeg);
   half8 qh[S::kStepsQK], ql[S::kStepsQK];
-  const float c = load_q<S::kStepsQK, 16, 2>(a.q + (static_cast<size_t>(sq.tok0) * a.n_heads + qrow) * hd, h * 8, hd,
-                                             a.scale, qh, ql);
+  const float c = q.halves(a.scale, h * 8, hd, qh, ql);
   f32x16 o[S::kDimBlocks];
 #pragma unroll
   for (int mb = 0; mb < S::kDimBlocks; mb++)
@@ -885,15 +896,16 @@ struct Plan {
 // Workgroups that run at once: 256 compute units times those whose registers
 // fit one (the kernels' launch bounds).
 size_t resident(Width w, size_t hd) {
-  const size_t per_cu = w == kNarrow16 ? (hd <= 64 ? 3 : hd <= 128 ? 2 : 1) : hd <= 128 ? 2 : 1;
+  const size_t per_cu = w == kWide ? (hd <= 128 ? 2 : 1) : w == kNarrow16 && hd <= 64 ? 2 : 1;
   return 256 * per_cu;
 }
 
 // Cache rows of a part, per kernel: the fewest, in whole tiles, that leave no
 // more workgroups than run at once (a few left over for a second round would
-// take as long as all of the first), but no fewer than kLeast.
+// take as long as all of the first), but not so few that joining the parts
+// costs more than it saves: about 4 us, in which a narrow workgroup takes 512
+// rows and a wide one 128.
 Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd) {
-  constexpr size_t kLeast = 128;
   const size_t group = n_heads / n_kv;
   auto tiles = [&](size_t i) {
     const size_t rows = n_tree[i] * group;
@@ -904,8 +916,8 @@ Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_
     if (n_tree[i]) work[width_of(n_tree[i] * group, hd)] += (past[i] + n_tree[i]) * tiles(i);
   Plan p{};
   for (int w = 0; w < kWidths; w++) {
-    const size_t unit = w == kWide ? 64 : 128, most = resident(static_cast<Width>(w), hd);
-    size_t r = std::max(kLeast, (work[w] * n_kv / most + unit - 1) / unit * unit);
+    const size_t unit = w == kWide ? 64 : 32 * narrow_waves(static_cast<int>(hd)), most = resident(static_cast<Width>(w), hd);
+    size_t r = std::max<size_t>(w == kWide ? 128 : 512, (work[w] * n_kv / most + unit - 1) / unit * unit);
     for (int tries = 0; tries < 16; tries++) {
       size_t n = 0;
       for (size_t i = 0; i < n_seq; i++)
@@ -927,7 +939,7 @@ Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_
 
 template <int HDP, int BN>
 void launch_width(const TreeArgs& a, Width w, bool q8, uint32_t items, hipStream_t s) {
-  const dim3 grid(items * a.n_kv), nt(kTrNT);
+  const dim3 grid(items * a.n_kv), nt(w == kWide ? kTrNT : 64 * narrow_waves(HDP));
   if (w == kNarrow16) {
     if (q8)
       hipLaunchKernelGGL((tree_narrow_kernel<HDP, 1, true>), grid, nt, 0, s, a);
