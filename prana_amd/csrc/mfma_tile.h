@@ -19,6 +19,7 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Transposing LDS read of halves: the 16 lanes of a group read 4 rows of 16
@@ -61,16 +62,22 @@ __device__ __forceinline__ u32x4 only_finite(u32x4 v) {
   return u32x4{only_finite(v.x), only_finite(v.y), only_finite(v.z), only_finite(v.w)};
 }
 
-// An f32 as two halves, x = hi + lo to 22 bits (|x| under 65504; lo has steps
-// of at least 2^-24). x is opaque here: a product that feeds it would be fused
-// with the rounding to hi, but not with the one to lo, and the two would not
-// belong together where the product lies near a tie.
-__device__ __forceinline__ void split_half(float x, _Float16& hi, _Float16& lo) {
-  asm("" : "+v"(x));
-  hi = static_cast<_Float16>(x);
-  lo = static_cast<_Float16>(fmaf(static_cast<float>(hi), -1.0f, x));  // one instruction with its rounding
+// Two f32 as two halves each, x = hi + lo to 22 bits (|x| under 65504; lo has
+// steps of at least 2^-24): one conversion for the pair of hi, and one
+// instruction for each lo, x - hi rounded to a half. The values are opaque: a
+// product that feeds one would be fused with its rounding to hi, but not with
+// the one to lo, and the two would not belong together where the product lies
+// near a tie. The factor is, or the product with it would become a subtraction
+// and a rounding of its own.
+__device__ __forceinline__ void split_pair(float x0, float x1, half2v& hi, half2v& lo) {
+  float minus = -1.0f;
+  asm("" : "+v"(x0), "+v"(x1));
+  asm("" : "+s"(minus));
+  const f32x2 x = {x0, x1};
+  hi = __builtin_convertvector(x, half2v);
+  lo = half2v{static_cast<_Float16>(fmaf(static_cast<float>(hi.x), minus, x0)),
+              static_cast<_Float16>(fmaf(static_cast<float>(hi.y), minus, x1))};
 }
-
 // The power of two that brings amax into [2^9, 2^10), where both halves of a
 // split are far from their limits; 1 where amax is 0 or not finite.
 __device__ __forceinline__ float row_factor(float amax) {
@@ -127,11 +134,13 @@ struct QRow {
 #pragma unroll
       for (int s = 0; s < PIECES; s++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          _Float16 xh, xl;
-          split_half(__uint_as_float(raw[s][j]) * f * scale, xh, xl);
-          qh[s][j] = xh;
-          ql[s][j] = xl;
+        for (int j = 0; j < 8; j += 2) {
+          half2v xh, xl;
+          split_pair(__uint_as_float(raw[s][j]) * f * scale, __uint_as_float(raw[s][j + 1]) * f * scale, xh, xl);
+          qh[s][j] = xh.x;
+          qh[s][j + 1] = xh.y;
+          ql[s][j] = xl.x;
+          ql[s][j + 1] = xl.y;
         }
       return 1.0f / f;  // a power of two: exact
     }

@@ -242,16 +242,20 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
       for (int t = 0; t < 2; t++) {
         half8 ph, pl;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float p = exp2_hw(fmaf(s[b][t * 8 + j], c, -ms));
-          l += p;
-          if constexpr (HALF) {
-            ph[j] = static_cast<_Float16>(p);
-          } else {
-            _Float16 xh, xl;
-            split_half(p, xh, xl);
-            ph[j] = xh;
-            pl[j] = xl;
+        for (int j = 0; j < 8; j += 2) {
+          const float p0 = exp2_hw(fmaf(s[b][t * 8 + j], c, -ms)), p1 = exp2_hw(fmaf(s[b][t * 8 + j + 1], c, -ms));
+          l += p0;
+          l += p1;
+          half2v xh, xl;
+          if constexpr (HALF)
+            xh = __builtin_convertvector((f32x2{p0, p1}), half2v);
+          else
+            split_pair(p0, p1, xh, xl);
+          ph[j] = xh.x;
+          ph[j + 1] = xh.y;
+          if constexpr (!HALF) {
+            pl[j] = xl.x;
+            pl[j + 1] = xl.y;
           }
         }
         const uint16_t* vp = s_v + (b * 32 + t * 16 + 4 * h + ((lane & 15) >> 2)) * S::kLdV +
@@ -264,15 +268,15 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
         }
       }
     if (odd) {  // rare: the values left out, for the rows that see them (any weight gives the same result)
+      uint32_t last4 = hd - 4;  // (opaque: nothing of this is worth a register outside)
+      asm volatile("" : "+s"(last4));
       for (uint32_t r = k0; r < min(k0 + BN, len); r++) {
         if (r > tok) break;
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
           for (int g = 0; g < 4; g++) {
-            const uint32_t d = mb * 32 + 8 * g + 4 * h;
-            if (d >= hd) continue;
-            const half4 x = *reinterpret_cast<const half4*>(vb + r * a.ld_kv + d);
+            const half4 x = *reinterpret_cast<const half4*>(vb + r * a.ld_kv + min(mb * 32u + 8 * g + 4 * h, last4));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               const float v = static_cast<float>(x[j]);
@@ -403,16 +407,20 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
 #pragma unroll
     for (int b = 0; b < 2; b++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float p = exp2_hw(fmaf(s[b][i], c, -ms));
-        l += p;
-        if constexpr (HALF) {
-          ph[b * 4 + i] = static_cast<_Float16>(p);
-        } else {
-          _Float16 xh, xl;
-          split_half(p, xh, xl);
-          ph[b * 4 + i] = xh;
-          pl[b * 4 + i] = xl;
+      for (int i = 0; i < 4; i += 2) {
+        const float p0 = exp2_hw(fmaf(s[b][i], c, -ms)), p1 = exp2_hw(fmaf(s[b][i + 1], c, -ms));
+        l += p0;
+        l += p1;
+        half2v xh, xl;
+        if constexpr (HALF)
+          xh = __builtin_convertvector((f32x2{p0, p1}), half2v);
+        else
+          split_pair(p0, p1, xh, xl);
+        ph[b * 4 + i] = xh.x;
+        ph[b * 4 + i + 1] = xh.y;
+        if constexpr (!HALF) {
+          pl[b * 4 + i] = xl.x;
+          pl[b * 4 + i + 1] = xl.y;
         }
       }
     const uint16_t* vp = s_v + (4 * g + (n >> 2)) * S::kLdV + (n & 3) * 4;
@@ -423,12 +431,14 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
       if constexpr (!HALF) o[mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[mb], 0, 0, 0);
     }
     if (odd) {  // rare: the values left out, for the rows that see them
+      uint32_t last4 = hd - 4;
+      asm volatile("" : "+s"(last4));
       for (uint32_t r = k0; r < min(k0 + kWideBN, len); r++) {
         if (r > tok) break;
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++) {
           const uint32_t d = mb * 16 + 4 * g;
-          const half4 x = *reinterpret_cast<const half4*>(vb + r * a.ld_kv + min(d, hd - 4));
+          const half4 x = *reinterpret_cast<const half4*>(vb + r * a.ld_kv + min(d, last4));
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const float v = static_cast<float>(x[j]);

@@ -126,23 +126,40 @@ struct Piece<true> {
   __device__ __forceinline__ u32x4 halves() const { return i8_to_halves(w); }
 };
 
-// V scales of 8-bit caches are taken relative to a power of two no smaller
-// than any scale met so far, so that a probability times its scale stays below
-// 2^15 as the probability does.
+// Four values of a cache row.
+template <bool Q8>
+__device__ __forceinline__ void load_values(const unsigned char* p, float scale, float* x) {
+  if constexpr (Q8) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = static_cast<float>(static_cast<int8_t>(w >> (8 * j))) * scale;
+  } else {
+    const half4 v = *reinterpret_cast<const half4*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = static_cast<float>(v[j]);
+  }
+}
+
+// V scales of 8-bit caches are taken relative to 2^e, a power of two no smaller
+// than any scale met so far: probabilities are kept times 2^-e (through the
+// exponential's argument, in the sums too), so that one times its scale stays
+// below 2^15 as the probability itself does. A head whose scales pass 2^100
+// loses probabilities under 2^-26 to underflow.
 struct ScaleTop {
-  float top = 0x1p-100f, inv = 0x1p100f;
-  // v: this lane's scales of the tile. The factor for what was summed before.
+  float e = -60.0f, top = 0x1p-60f;
+  // v: this lane's scales of the tile (0 where they are not finite). The
+  // factor for what was summed before.
   __device__ __forceinline__ float raise(float v) {
-    float big = fabsf(v) < INFINITY ? fabsf(v) : 0.0f;
-    big = wave_max_f32(big);
+    const float big = wave_max_f32(fabsf(v));
     if (!(big > top)) return 1.0f;
-    const uint32_t e = min((__float_as_uint(big) >> 23) + 1, 253u);
-    const float nt = __uint_as_float(e << 23), f = top / nt;
+    const uint32_t x = min((__float_as_uint(big) >> 23) + 1, 253u);
+    const float nt = __uint_as_float(x << 23), f = top / nt;
     top = nt;
-    inv = 1.0f / nt;
+    e = static_cast<float>(static_cast<int>(x) - 127);
     return f;
   }
 };
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // ------------------------------------------------------------ narrow: up to 16 RB rows
 // Waves of a workgroup: eight, or four of heads that take more than half of a
@@ -323,6 +340,14 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
         }
       }
     }
+    if constexpr (Q8) {
+      // (so too a V scale: it would make every product with its row NaN)
+      if (edge) {
+        const bool bad = lane >= 32 && !finite(sc);
+        odd = __any(bad);
+        if (bad) sc = 0.0f;
+      }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the reads of the keys before come first)
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -332,15 +357,17 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
     }
     if constexpr (Q8) {
       s_scale[wave][lane] = sc;
-      const float v = lane < 32 ? 0.0f : sc;
+      const float v = lane < 32 || !finite(sc) ? 0.0f : sc;
       if (__any(fabsf(v) > top.top)) {
         const float f = top.raise(v);
 #pragma unroll
-        for (int r = 0; r < RB; r++)
+        for (int r = 0; r < RB; r++) {
+          l[r] *= f;
 #pragma unroll
           for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
             for (int j = 0; j < 4; j++) o[r][mb][j] *= f;
+        }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -384,8 +411,6 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
         const float4 y = *reinterpret_cast<const float4*>(&s_scale[wave][32 + b * 16 + 4 * g]);
         ks[b][0] = x.x; ks[b][1] = x.y; ks[b][2] = x.z; ks[b][3] = x.w;
         vs[b][0] = y.x; vs[b][1] = y.y; vs[b][2] = y.z; vs[b][3] = y.w;
-#pragma unroll
-        for (int j = 0; j < 4; j++) vs[b][j] *= top.inv;
       }
     }
     half8 ph[RB], pl[RB];
@@ -423,21 +448,24 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
 #pragma unroll
           for (int j = 0; j < 4; j++) o[r][mb][j] *= al;
       }
-      const float ms = m[r] == -INFINITY ? 0.0f : m[r] - kPShift;
+      const float ms = (m[r] == -INFINITY ? 0.0f : m[r] - kPShift) + (Q8 ? top.e : 0.0f);
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          float p = exp2_hw(fmaf(s[r][b][j], c[r], -ms));
-          l[r] += p;
+        for (int j = 0; j < 4; j += 2) {
+          float p0 = exp2_hw(fmaf(s[r][b][j], c[r], -ms)), p1 = exp2_hw(fmaf(s[r][b][j + 1], c[r], -ms));
+          l[r] += p0;
+          l[r] += p1;
           if constexpr (Q8) {
-            p *= vs[b][j];
-            if (edge && !(seen >> (b * 16 + j) & 1)) p = 0.0f;  // (its scale may be NaN)
+            p0 *= vs[b][j];
+            p1 *= vs[b][j + 1];
           }
-          _Float16 xh, xl;
-          split_half(p, xh, xl);
-          ph[r][b * 4 + j] = xh;
-          pl[r][b * 4 + j] = xl;
+          half2v xh, xl;
+          split_pair(p0, p1, xh, xl);
+          ph[r][b * 4 + j] = xh.x;
+          ph[r][b * 4 + j + 1] = xh.y;
+          pl[r][b * 4 + j] = xl.x;
+          pl[r][b * 4 + j + 1] = xl.y;
         }
     }
     const uint16_t* vp = s_v + (4 * g + (n >> 2)) * S::kLdV + (n & 3) * 4;
@@ -450,22 +478,27 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
         o[r][mb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[r], o[r][mb], 0, 0, 0);
       }
     }
-    if (odd) {  // rare
-      for (uint32_t t = k0; t < min(k0 + 32, kend); t++)
+    if (odd) {  // rare (and opaque: nothing of it is worth a register outside)
+      uint32_t last4 = hd - 4;
+      asm volatile("" : "+s"(last4));
+      for (uint32_t t = k0; t < min(k0 + 32, kend); t++) {
+        float scale = 1.0f;
+        if constexpr (Q8) {
+          scale = sq.vs[static_cast<size_t>(t) * a.n_kv + kvh];
+          if (finite(scale)) continue;
+        }
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++) {
-          const uint32_t d = mb * 16 + 4 * g;
-          if (d >= hd) continue;
-          const half4 x = *reinterpret_cast<const half4*>(vbase + (t * ld + d) * kSize);
+          float x[4];
+          load_values<Q8>(vbase + (t * ld + min(mb * 16u + 4 * g, last4)) * kSize, scale, x);
 #pragma unroll
-          for (int r = 0; r < RB; r++)
+          for (int r = 0; r < RB; r++) {
+            const bool sees = seen_from(word[r], static_cast<int>(t) - static_cast<int>(sq.past)) & 1;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const float v = static_cast<float>(x[j]);
-              if (!(fabsf(v) < INFINITY) && (seen_from(word[r], static_cast<int>(t) - static_cast<int>(sq.past)) & 1))
-                o[r][mb][j] += v;
-            }
+            for (int j = 0; j < 4; j++) o[r][mb][j] += sees && !finite(x[j]) ? x[j] : 0.0f;
+          }
         }
+      }
     }
   }
 
@@ -474,6 +507,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
   for (int r = 0; r < RB; r++) {
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
+    if constexpr (Q8) l[r] *= top.top;
     if (g == 0) {
       s_m[wave][r * 16 + n] = m[r];
       s_l[wave][r * 16 + n] = l[r];
@@ -608,9 +642,13 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
 #pragma unroll
     for (int mb = 0; mb < S::kDimBlocks; mb++) keep_accumulator<(HDP > 128)>(o[mb]);
     const bool edge = k0 + BN > min(sq.past, kend);
-    bool odd = false;
-    if (!Q8 && edge) {
-      if constexpr (!Q8) {
+    bool odd = false;  // (as in the narrow kernel)
+    if (edge) {
+      if constexpr (Q8) {
+        const bool bad = tid / BN % 2 == 1 && !finite(sc);
+        odd = __syncthreads_or(bad);
+        if (bad) sc = 0.0f;
+      } else {
         uint32_t bits = 0;
 #pragma unroll
         for (int p = 0; p < S::kLoads; p++) bits |= odd_halves(vr[p].w);
@@ -651,9 +689,11 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[t], s[b], 0, 0, 0);
       }
     if constexpr (Q8) {
-      const float v = lane < BN ? s_scale[1][lane] : 0.0f;
+      float v = lane < BN ? s_scale[1][lane] : 0.0f;
+      if (!finite(v)) v = 0.0f;
       if (__any(fabsf(v) > top.top)) {
         const float f = top.raise(v);
+        l *= f;
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
@@ -700,7 +740,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
     }
 #pragma unroll
     for (int mb = 0; mb < S::kDimBlocks; mb++) keep_accumulator<(HDP > 128)>(o[mb]);
-    const float ms = m == -INFINITY ? 0.0f : m - kPShift;
+    const float ms = (m == -INFINITY ? 0.0f : m - kPShift) + (Q8 ? top.e : 0.0f);
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
 #pragma unroll
@@ -712,18 +752,21 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
           if constexpr (Q8) vs = *reinterpret_cast<const float4*>(&s_scale[1][b * 32 + 16 * t + 8 * gg + 4 * h]);
           const float v4[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
+          for (int j = 0; j < 4; j += 2) {
             const int reg = t * 8 + gg * 4 + j;
-            float p = exp2_hw(fmaf(s[b][reg], c, -ms));
-            l += p;
+            float p0 = exp2_hw(fmaf(s[b][reg], c, -ms)), p1 = exp2_hw(fmaf(s[b][reg + 1], c, -ms));
+            l += p0;
+            l += p1;
             if constexpr (Q8) {
-              p *= v4[j] * top.inv;
-              if (edge && !(seen >> (b * 32 + 8 * (reg / 4) + reg % 4) & 1)) p = 0.0f;
+              p0 *= v4[j];
+              p1 *= v4[j + 1];
             }
-            _Float16 xh, xl;
-            split_half(p, xh, xl);
-            ph[gg * 4 + j] = xh;
-            pl[gg * 4 + j] = xl;
+            half2v xh, xl;
+            split_pair(p0, p1, xh, xl);
+            ph[gg * 4 + j] = xh.x;
+            ph[gg * 4 + j + 1] = xh.y;
+            pl[gg * 4 + j] = xl.x;
+            pl[gg * 4 + j + 1] = xl.y;
           }
         }
         const uint16_t* vp = s_v + (b * 32 + t * 16 + 4 * h + ((lane & 15) >> 2)) * S::kLdV +
@@ -735,42 +778,45 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
           o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[mb], 0, 0, 0);
         }
       }
-    if (odd) {  // rare
+    if (odd) {  // rare (and opaque: nothing of it is worth a register outside)
+      uint32_t last4 = hd - 4;
+      asm volatile("" : "+s"(last4));
       for (uint32_t t = k0; t < min(k0 + BN, kend); t++) {
+        float scale = 1.0f;
+        if constexpr (Q8) {
+          scale = sq.vs[static_cast<size_t>(t) * a.n_kv + kvh];
+          if (finite(scale)) continue;
+        }
         if (!(seen_from(word, static_cast<int>(t) - static_cast<int>(sq.past)) & 1)) continue;
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
           for (int g = 0; g < 4; g++) {
-            const uint32_t d = mb * 32 + 8 * g + 4 * h;
-            if (d >= hd) continue;
-            const half4 x = *reinterpret_cast<const half4*>(vbase + (t * ld + d) * kSize);
+            float x[4];
+            load_values<Q8>(vbase + (t * ld + min(mb * 32u + 8 * g + 4 * h, last4)) * kSize, scale, x);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const float v = static_cast<float>(x[j]);
-              if (!(fabsf(v) < INFINITY)) o[mb][4 * g + j] += v;
-            }
+            for (int j = 0; j < 4; j++) o[mb][4 * g + j] += finite(x[j]) ? 0.0f : x[j];
           }
       }
     }
   }
   l += __shfl_xor(l, 32, 64);
   if (row0 + wave * 32 + n >= rows) return;
-  float f = 1.0f;
+  float f;
   float* dst;
   if (sq.splits == 1) {
     f = l == 0.0f ? 0.0f : 1.0f / l;
     dst = a.out + (static_cast<size_t>(sq.tok0) * a.n_heads + qrow) * hd;
   } else {
     const size_t pr = sq.part0 + qrow * sq.splits + split;
+    f = Q8 ? top.top : 1.0f;
     dst = a.part + pr * hd;
     if (h == 0) {
       float* ml = a.part + a.part_rows * hd + pr * 2;
       ml[0] = m;
-      ml[1] = l;
+      ml[1] = l * f;
     }
   }
-  if constexpr (Q8) f *= top.top;
 #pragma unroll
   for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
