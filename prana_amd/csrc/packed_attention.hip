@@ -75,16 +75,16 @@ struct TileFetch {
   static constexpr bool kEven = kPkNT % CHUNKS == 0;  // a workgroup's pieces are whole rows
   const unsigned char *kb, *vb;
   size_t ld;  // bytes
-  uint32_t len, hd;
+  uint32_t len, hd, tid;
   uint32_t off[kEven ? 1 : kLoads];
   __device__ __forceinline__ uint32_t offset(uint32_t e, uint32_t last) const {
     return min(e / CHUNKS, last) * static_cast<uint32_t>(ld) + min(e % CHUNKS * 8, hd - 8) * 2;
   }
-  __device__ __forceinline__ TileFetch(const uint16_t* k, const uint16_t* v, size_t ld_, uint32_t len_, uint32_t hd_)
+  __device__ __forceinline__ TileFetch(const uint16_t* k, const uint16_t* v, size_t ld_, uint32_t len_, uint32_t hd_, uint32_t tid_)
       : kb(reinterpret_cast<const unsigned char*>(k)), vb(reinterpret_cast<const unsigned char*>(v)), ld(ld_ * 2),
-        len(len_), hd(hd_) {
+        len(len_), hd(hd_), tid(tid_) {
 #pragma unroll
-    for (int i = 0; i < (kEven ? 1 : kLoads); i++) off[i] = offset(i * kPkNT + threadIdx.x, BN);
+    for (int i = 0; i < (kEven ? 1 : kLoads); i++) off[i] = offset(i * kPkNT + tid, BN);
   }
   __device__ __forceinline__ void operator()(uint32_t k0, u32x4* kr, u32x4* vr) const {
     const unsigned char* kp = kb + k0 * ld;
@@ -101,7 +101,7 @@ struct TileFetch {
       const uint32_t last = len - 1 - k0;
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
-        const uint32_t e = i * kPkNT + threadIdx.x, at = offset(e, last);
+        const uint32_t e = i * kPkNT + tid, at = offset(e, last);
         kr[i] = *reinterpret_cast<const u32x4*>(kp + at);
         vr[i] = u32x4{0, 0, 0, 0};
         if (e / CHUNKS <= last) vr[i] = *reinterpret_cast<const u32x4*>(vp + at);
@@ -116,7 +116,7 @@ struct TileFetch {
 // stay out of the tile, and true is returned, for them to be added to the rows
 // that see them.
 template <int BN, int CHUNKS, int LD_K, int LD_V>
-__device__ __forceinline__ bool stage_tile(uint16_t* s_k, uint16_t* s_v, u32x4* kr, u32x4* vr, bool edge) {
+__device__ __forceinline__ bool stage_tile(uint16_t* s_k, uint16_t* s_v, u32x4* kr, u32x4* vr, int tid, bool edge) {
   constexpr int kLoads = BN * CHUNKS / kPkNT;
   bool odd = false;
   if (edge) {
@@ -133,7 +133,7 @@ __device__ __forceinline__ bool stage_tile(uint16_t* s_k, uint16_t* s_v, u32x4* 
   }
 #pragma unroll
   for (int i = 0; i < kLoads; i++) {
-    const int e = i * kPkNT + threadIdx.x;
+    const int e = i * kPkNT + tid;
     const int r = e / CHUNKS, d = (e % CHUNKS) * 8;
     *reinterpret_cast<u32x4*>(s_k + r * LD_K + d) = kr[i];
     *reinterpret_cast<u32x4*>(s_v + r * LD_V + d) = vr[i];
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
   const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   u32x4 kr[S::kLoads], vr[S::kLoads];
-  const TileFetch<BN, S::kChunks> fetch(kb, vb, a.ld_kv, len, hd);
+  const TileFetch<BN, S::kChunks> fetch(kb, vb, a.ld_kv, len, hd, tid);
   fetch(0, kr, vr);
   half8 qh[S::kStepsQK], ql[HALF ? 1 : S::kStepsQK];
   const float c = q.halves(a.scale, h * 8, hd, qh, ql);
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
 
   for (uint32_t k0 = 0; k0 <= tok_last_wg; k0 += BN) {
     const bool odd =
-        stage_tile<BN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, k0 + BN - 1 > tok_first_wg);
+        stage_tile<BN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, tid, k0 + BN - 1 > tok_first_wg);
     if (k0 + BN <= tok_last_wg) fetch(k0 + BN, kr, vr);
     if (k0 > tok_last) continue;  // (the wave's rows see nothing of this tile)
     f32x16 s[S::kKeyBlocks];
@@ -303,9 +303,11 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
 // ------------------------------------------------------------ heads wider than 128
 // 32 rows of such heads would fill the registers of a wave that runs alone on
 // its unit, with nothing to hide its waits behind. So a wave takes 16 rows
-// (16x16x32 products, twice the LDS reads per product) and a workgroup 64,
-// three of which run side by side; tiles of 32 keys.
-constexpr int kWideRows = 64, kWideBN = 32;
+// (16x16x32 products, twice the LDS reads per product) and four waves 64;
+// tiles of 32 keys. Such heads often share one KV head, and 64 rows of it are
+// few workgroups that walk long prompts alone, so each has two such groups of
+// waves, which take the tiles in turn and join their sums at the end.
+constexpr int kWideRows = 64, kWideBN = 32, kWideGroups = 2;
 
 template <int HDP>
 struct PkWideShape {
@@ -313,15 +315,21 @@ struct PkWideShape {
   static constexpr int kLdK = HDP + 8;
   static constexpr int kLdV = HDP + 16;  // 32-byte pieces of 8 rows on different banks
   static constexpr int kLoads = kWideBN * kChunks / kPkNT;
+  static constexpr int kTile = kWideBN * (kLdK + kLdV);  // halves of a group's K and V
+  static constexpr int kLdO = HDP + 4;                   // joining the groups: floats per row
+  static_assert(kWideRows * kLdO * 4 <= kWideGroups * kTile * 2, "a group's sums fit the tiles");
 };
 
 template <int HDP, bool HALF>
-__global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
+__global__ __launch_bounds__(kWideGroups* kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
   using S = PkWideShape<HDP>;
   static_assert(kWideBN * S::kChunks % kPkNT == 0, "a tile is a whole number of pieces per lane");
-  __shared__ __attribute__((aligned(16))) uint16_t s_k[kWideBN * S::kLdK];
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[kWideBN * S::kLdV];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ __attribute__((aligned(16))) uint16_t s_tiles[kWideGroups * S::kTile];
+  __shared__ float s_ml[2][kWideRows];
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kPkNT);
+  const int tid = threadIdx.x % kPkNT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint16_t* const s_k = s_tiles + group * S::kTile;
+  uint16_t* const s_v = s_k + kWideBN * S::kLdK;
   const int n = lane & 15, g = lane >> 4;
   const uint32_t kvh = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv;
   const int sq = table_find(a.tile0, a.n_seq, tile);
@@ -343,8 +351,8 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
   const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   u32x4 kr[S::kLoads], vr[S::kLoads];
-  const TileFetch<kWideBN, S::kChunks> fetch(kb, vb, a.ld_kv, len, hd);
-  fetch(0, kr, vr);
+  const TileFetch<kWideBN, S::kChunks> fetch(kb, vb, a.ld_kv, len, hd, tid);
+  if (group * kWideBN <= tok_last_wg) fetch(group * kWideBN, kr, vr);
   half8 qh[S::kSteps], ql[HALF ? 1 : S::kSteps];
   const float c = q.halves(a.scale, g * 8, hd, qh, ql);
 
@@ -355,10 +363,12 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
     for (int i = 0; i < 4; i++) o[mb][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  for (uint32_t k0 = 0; k0 <= tok_last_wg; k0 += kWideBN) {
-    const bool odd = stage_tile<kWideBN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr,
-                                                                       k0 + kWideBN - 1 > tok_first_wg);
-    if (k0 + kWideBN <= tok_last_wg) fetch(k0 + kWideBN, kr, vr);
+  constexpr uint32_t kRound = kWideGroups * kWideBN;
+  for (uint32_t r0 = 0; r0 <= tok_last_wg; r0 += kRound) {
+    const uint32_t k0 = r0 + group * kWideBN;
+    const bool odd = stage_tile<kWideBN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, tid,
+                                                                       r0 + kRound - 1 > tok_first_wg);
+    if (k0 + kRound <= tok_last_wg) fetch(k0 + kRound, kr, vr);
     if (k0 > tok_last) continue;  // (the wave's rows see nothing of this tile)
 
     f32x4 s[2], s2[2];  // (two chains of products each)
@@ -450,14 +460,32 @@ __global__ __launch_bounds__(kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  if (row_w + n >= rows) return;
-  const float inv = 1.0f / l;
+  // join the groups: the second leaves its sums in LDS
+  float* const s_o = reinterpret_cast<float*>(s_tiles) + (wave * 16 + n) * S::kLdO;
+  __syncthreads();
+  if (group == 1) {
+    if (g == 0) {
+      s_ml[0][wave * 16 + n] = m;
+      s_ml[1][wave * 16 + n] = l;
+    }
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++)
+      *reinterpret_cast<f32x4*>(s_o + mb * 16 + 4 * g) = o[mb];
+  }
+  __syncthreads();
+  if (group == 1 || row_w + n >= rows) return;
+  // (Every row sees the first key, so the first group's maximum is a number. A
+  // row's maximum in the second is one from its first tile on: 32 tokens are
+  // whole blocks of 16 rows, so a wave's rows see a tile's first key together.)
+  const float m2 = s_ml[0][wave * 16 + n], l2 = s_ml[1][wave * 16 + n], top = fmaxf(m, m2);
+  const float f1 = exp2_hw(m - top), f2 = exp2_hw(m2 - top);
+  const float inv = 1.0f / fmaf(l, f1, l2 * f2);
 #pragma unroll
   for (int mb = 0; mb < S::kDimBlocks; mb++) {
     const uint32_t d = mb * 16 + 4 * g;
     if (d < hd) {
-      const size_t at = (base + tok) * a.ld_out + static_cast<size_t>(head) * hd + d;
-      store4<HALF>(a.out, at, o[mb][0] * inv, o[mb][1] * inv, o[mb][2] * inv, o[mb][3] * inv);
+      const f32x4 y = (o[mb] * f1 + *reinterpret_cast<const f32x4*>(s_o + d) * f2) * inv;
+      store4<HALF>(a.out, (base + tok) * a.ld_out + static_cast<size_t>(head) * hd + d, y[0], y[1], y[2], y[3]);
     }
   }
 }
@@ -472,9 +500,9 @@ void launch_shape(const PackedArgs& a, bool half, uint32_t tiles, hipStream_t s)
       hipLaunchKernelGGL((packed_kernel<HDP, 64, false>), grid, nt, 0, s, a);
   } else {
     if (half)
-      hipLaunchKernelGGL((packed_wide_kernel<HDP, true>), grid, nt, 0, s, a);
+      hipLaunchKernelGGL((packed_wide_kernel<HDP, true>), grid, dim3(kWideGroups * kPkNT), 0, s, a);
     else
-      hipLaunchKernelGGL((packed_wide_kernel<HDP, false>), grid, nt, 0, s, a);
+      hipLaunchKernelGGL((packed_wide_kernel<HDP, false>), grid, dim3(kWideGroups * kPkNT), 0, s, a);
   }
 }
 
