@@ -8,13 +8,17 @@
 // its products: the scale of a K row multiplies its score, that of a V row its
 // probability, and the i8 values go to the matrix cores as they are.
 //
-// Both kernels move each byte once and are bound by memory. A lane holds 8
-// values of a head (two 16-byte loads of f32, one 8-byte store of i8), the
-// lanes of a head find its maximum among them, and a lane takes kItems heads
-// whose loads are in flight together.
+// Both kernels move each byte once and are bound by memory. Writing, a lane
+// holds 8 values of a head (two 16-byte loads of f32, one 8-byte store of i8),
+// the lanes of a head find its maximum among them, and a lane takes kItems
+// heads whose loads are in flight together. What is read or written once
+// passes the caches by (nontemporal); the quantized rows do not, attention
+// reads them next.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
+#include "mfma_tile.h"
 #include "seq_table.h"
 #include "serving.h"
 
@@ -24,6 +28,8 @@ namespace {
 
 constexpr int kKvNT = 256;
 constexpr int kItems = 4;  // heads of a lane group, loads in flight together
+// Values a lane writes when a cache is read back.
+__host__ __device__ constexpr int read_values(bool half) { return half ? 8 : 4; }
 
 struct KvArgs {
   const void* k;  // the packed side
@@ -97,9 +103,9 @@ __global__ __launch_bounds__(kKvNT) void kv_write_kernel(KvArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; j++) x[it][j] = 0.0f;
     if (item < n_items && live) {
-      const float4* p = reinterpret_cast<const float4*>(src + (static_cast<size_t>(sq.src) + row) * a.ld +
+      const f32x4* p = reinterpret_cast<const f32x4*>(src + (static_cast<size_t>(sq.src) + row) * a.ld +
                                                         static_cast<size_t>(head) * a.hd + sub * 8);
-      const float4 u = p[0], w = p[1];
+      const f32x4 u = __builtin_nontemporal_load(p), w = __builtin_nontemporal_load(p + 1);
       x[it][0] = u.x; x[it][1] = u.y; x[it][2] = u.z; x[it][3] = u.w;
       x[it][4] = w.x; x[it][5] = w.y; x[it][6] = w.z; x[it][7] = w.w;
     }
@@ -150,26 +156,30 @@ __global__ __launch_bounds__(kKvNT) void kv_write_kernel(KvArgs a) {
   }
 }
 
+// The rows written by kv_write_kernel. A lane moves the values of one 16-byte
+// store: 8 halves or 4 floats (a lane of 8 floats would leave its lines half
+// written between two stores).
 template <int LPH, bool HALF>
 __global__ __launch_bounds__(kKvNT) void kv_read_kernel(KvArgs a) {
-  constexpr int kGroups = kKvNT / LPH;
+  constexpr int kGroups = kKvNT / LPH, kPer = read_values(HALF);
+  using Word = std::conditional_t<HALF, u32x2, uint32_t>;
   const KvSeq sq = this_seq(a);
   const int8_t* src = static_cast<const int8_t*>(sq.cache);
   void* dst = const_cast<void*>(blockIdx.y ? a.v : a.k);
   const int sub = threadIdx.x % LPH, grp = threadIdx.x / LPH;
-  if (sub * 8u >= a.hd) return;
+  if (sub * static_cast<uint32_t>(kPer) >= a.hd) return;
   const uint64_t n_items = static_cast<uint64_t>(sq.rows) * a.n_kv;
   const uint64_t item0 = static_cast<uint64_t>(blockIdx.x - sq.block0) * (kGroups * kItems) + grp;
-  uint2 w[kItems];
+  Word w[kItems];
   float scale[kItems];
 #pragma unroll
   for (int it = 0; it < kItems; it++) {
     const uint64_t item = item0 + it * kGroups;
-    w[it] = make_uint2(0, 0);
+    w[it] = Word{};
     scale[it] = 0.0f;
     if (item < n_items) {
       const size_t at = static_cast<size_t>(sq.first) * a.n_kv + item;  // (row, head) of the cache
-      w[it] = *reinterpret_cast<const uint2*>(src + at * a.hd + sub * 8);
+      w[it] = *reinterpret_cast<const Word*>(src + at * a.hd + sub * kPer);
       scale[it] = sq.scales[at];
     }
   }
@@ -178,31 +188,33 @@ __global__ __launch_bounds__(kKvNT) void kv_read_kernel(KvArgs a) {
     const uint64_t item = item0 + it * kGroups;
     if (item >= n_items) continue;
     const uint32_t row = static_cast<uint32_t>(item / a.n_kv), head = static_cast<uint32_t>(item % a.n_kv);
-    const size_t at = (static_cast<size_t>(sq.src) + row) * a.ld + static_cast<size_t>(head) * a.hd + sub * 8;
-    float y[8];
+    const size_t at = (static_cast<size_t>(sq.src) + row) * a.ld + static_cast<size_t>(head) * a.hd + sub * kPer;
+    float y[kPer];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const uint32_t word = j < 4 ? w[it].x : w[it].y;
+    for (int j = 0; j < kPer; j++) {
+      uint32_t word;
+      if constexpr (HALF)
+        word = j < 4 ? w[it].x : w[it].y;
+      else
+        word = w[it];
       y[j] = static_cast<float>(static_cast<int8_t>(word >> (8 * (j % 4)))) * scale[it];
     }
     if constexpr (HALF) {
-      uint32_t h[4];
+      u32x4 h;
 #pragma unroll
       for (int j = 0; j < 4; j++)
         h[j] = static_cast<uint32_t>(f32_to_f16(y[2 * j])) | static_cast<uint32_t>(f32_to_f16(y[2 * j + 1])) << 16;
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst) + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      __builtin_nontemporal_store(h, reinterpret_cast<u32x4*>(static_cast<uint16_t*>(dst) + at));
     } else {
-      float4* o = reinterpret_cast<float4*>(static_cast<float*>(dst) + at);
-      o[0] = make_float4(y[0], y[1], y[2], y[3]);
-      o[1] = make_float4(y[4], y[5], y[6], y[7]);
+      __builtin_nontemporal_store(f32x4{y[0], y[1], y[2], y[3]}, reinterpret_cast<f32x4*>(static_cast<float*>(dst) + at));
     }
   }
 }
 
-// Lanes of a head: the power of two that holds its 8-value pieces.
-int lanes_per_head(size_t hd) {
+// Lanes of a head: the power of two that holds its pieces of `per` values.
+int lanes_per_head(size_t hd, int per) {
   int n = 1;
-  while (n * 8 < static_cast<int>(hd)) n *= 2;
+  while (n * per < static_cast<int>(hd)) n *= 2;
   return n;
 }
 
@@ -211,17 +223,19 @@ enum class Move { kWrite, kRead32, kRead16 };
 template <int LPH>
 void launch_move(Move m, const KvArgs& a, uint32_t blocks, hipStream_t s) {
   const dim3 grid(blocks, 2), nt(kKvNT);
-  if (m == Move::kWrite)
-    hipLaunchKernelGGL((kv_write_kernel<LPH>), grid, nt, 0, s, a);
-  else if (m == Move::kRead32)
+  if (m == Move::kRead32) {
     hipLaunchKernelGGL((kv_read_kernel<LPH, false>), grid, nt, 0, s, a);
-  else
-    hipLaunchKernelGGL((kv_read_kernel<LPH, true>), grid, nt, 0, s, a);
+  } else if constexpr (LPH <= 32) {
+    if (m == Move::kWrite)
+      hipLaunchKernelGGL((kv_write_kernel<LPH>), grid, nt, 0, s, a);
+    else
+      hipLaunchKernelGGL((kv_read_kernel<LPH, true>), grid, nt, 0, s, a);
+  }
 }
 
 int launch_moves(Move m, const void* k, const void* v, size_t ld, const prana_kv* kv, const size_t* first_rows,
                  const size_t* n_rows, size_t n_seq, size_t n_kv, size_t hd, hipStream_t s) {
-  const int lph = lanes_per_head(hd);
+  const int lph = lanes_per_head(hd, m == Move::kRead32 ? read_values(false) : 8);
   const size_t per_block = static_cast<size_t>(kKvNT / lph) * kItems;
   KvArgs a{};
   a.k = k;
@@ -239,7 +253,8 @@ int launch_moves(Move m, const void* k, const void* v, size_t ld, const prana_kv
       case 4: launch_move<4>(m, a, b, s); break;
       case 8: launch_move<8>(m, a, b, s); break;
       case 16: launch_move<16>(m, a, b, s); break;
-      default: launch_move<32>(m, a, b, s); break;
+      case 32: launch_move<32>(m, a, b, s); break;
+      default: launch_move<64>(m, a, b, s); break;
     }
     PRANA_LAUNCH_CHECK();
     a.n_seq = 0;
