@@ -147,16 +147,16 @@ __device__ __forceinline__ void load_values(const unsigned char* p, float scale,
 // loses probabilities under 2^-26 to underflow.
 struct ScaleTop {
   float e = -60.0f, top = 0x1p-60f;
-  // v: this lane's scales of the tile (0 where they are not finite). The
-  // factor for what was summed before.
-  __device__ __forceinline__ float raise(float v) {
+  // v: this lane's scales of the tile (0 where they are not finite). The power
+  // of two that what was summed before is to be multiplied with (as an
+  // exponent: it can lie beyond a float's).
+  __device__ __forceinline__ int raise(float v) {
     const float big = wave_max_f32(fabsf(v));
-    if (!(big > top)) return 1.0f;
-    const uint32_t x = min((__float_as_uint(big) >> 23) + 1, 253u);
-    const float nt = __uint_as_float(x << 23), f = top / nt;
-    top = nt;
-    e = static_cast<float>(static_cast<int>(x) - 127);
-    return f;
+    if (!(big > top)) return 0;
+    const int x = min((__float_as_uint(big) >> 23) + 1, 253u), was = static_cast<int>(e);
+    top = __uint_as_float(static_cast<uint32_t>(x) << 23);
+    e = static_cast<float>(x - 127);
+    return was - (x - 127);
   }
 };
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
@@ -359,14 +359,14 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
       s_scale[wave][lane] = sc;
       const float v = lane < 32 || !finite(sc) ? 0.0f : sc;
       if (__any(fabsf(v) > top.top)) {
-        const float f = top.raise(v);
+        const int f = top.raise(v);
 #pragma unroll
         for (int r = 0; r < RB; r++) {
-          l[r] *= f;
+          l[r] = ldexpf(l[r], f);
 #pragma unroll
           for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[r][mb][j] *= f;
+            for (int j = 0; j < 4; j++) o[r][mb][j] = ldexpf(o[r][mb][j], f);
         }
       }
     }
@@ -692,12 +692,12 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
       float v = lane < BN ? s_scale[1][lane] : 0.0f;
       if (!finite(v)) v = 0.0f;
       if (__any(fabsf(v) > top.top)) {
-        const float f = top.raise(v);
-        l *= f;
+        const int f = top.raise(v);
+        l = ldexpf(l, f);
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
-          for (int j = 0; j < 16; j++) o[mb][j] *= f;
+          for (int j = 0; j < 16; j++) o[mb][j] = ldexpf(o[mb][j], f);
       }
 #pragma unroll
       for (int b = 0; b < S::kKeyBlocks; b++)
@@ -881,8 +881,9 @@ __global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
     if (s != s0) load(s);
 #pragma unroll
     for (int k = 0; k < kBatch; k++) {
-      if (s + k * kPG >= ns || ms[k] == -INFINITY) continue;  // (a part that saw nothing holds zeros)
-      const float f = exp2_hw(ms[k] - M);
+      if (s + k * kPG >= ns) continue;
+      // a part without a maximum holds zeros (it saw nothing) or NaN (so were all its scores), which stays
+      const float f = ms[k] == -INFINITY ? 0.0f : exp2_hw(ms[k] - M);
       y.x = fmaf(x[k].x, f, y.x);
       y.y = fmaf(x[k].y, f, y.y);
       y.z = fmaf(x[k].z, f, y.z);

@@ -186,6 +186,74 @@ def test_matches_split_decode_and_the_same_call_twice(kind):
         assert np.all(np.abs(s - a) <= bound + 1e-4 * np.abs(want) + 2e-6)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("past,tokens,group", [(37, 5, 2), (6000, 5, 2), (6000, 12, 2), (6000, 40, 4)])
+def test_a_query_that_is_not_a_number_spoils_its_row_alone(kind, past, tokens, group):
+    # (the longer caches in parts, each without a maximum for that row)
+    w = 64
+    q, caches, _, _ = make(3, kind, [past], [tokens], 2 * group, 2, w)
+    clean = P.attention_tree(q, caches, [past], [tokens], 2 * group, 2, w)
+    q[3, w + 5] = np.nan
+    got = P.attention_tree(q, caches, [past], [tokens], 2 * group, 2, w)
+    assert np.isnan(got[3, w:2 * w]).all()
+    got[3, w:2 * w] = clean[3, w:2 * w]
+    assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("past,tokens", [(600, 3), (3000, 40)])
+def test_q8_value_scales_beyond_a_floats_square(past, tokens):
+    # V scales from 2^-66 to 2^80, the small ones first: what is summed before
+    # the large ones come stays in the sum that divides
+    w = 64
+    q, caches, ks, vs = make(32, "q8", [past], [tokens], 4, 1, w)
+    s = caches[0].v_scales.to_host()
+    f = np.where(np.arange(len(s)) < past // 2, np.float32(2.0 ** -62), np.float32(2.0 ** 84))[:, None]
+    s2 = (s * f).astype(np.float32)
+    P.check(_lib.load().prana_memcpy_h2d(caches[0].v_scales.ptr, C.c_void_p(s2.ctypes.data), s2.nbytes))
+    vs[0] = vs[0] * f.astype(np.float64)  # (a power of two: exact)
+    got = P.attention_tree(q, caches, [past], [tokens], 4, 1, w)
+    want, bound = SO.tree(q, ks, vs, [past], [tokens], None, 4, 1, w)
+    ok, worst = SO.within(got, want, bound)
+    assert ok, worst
+
+
+def test_one_call_of_all_widths():
+    # single tokens, small trees and large ones over short and long caches in one call
+    check("f16", [5000, 0, 77, 4000, 300, 2], [1, 64, 9, 30, 3, 1], 8, 2, 128)
+    check("q8", [5000, 0, 77, 4000, 300, 2], [1, 64, 9, 30, 3, 1], 8, 2, 128)
+
+
+def test_offsets_past_32_bits():
+    # a cache whose last rows lie 4 GiB behind its first; K and V share it
+    kv_heads, w, rows, past = 8, 256, (1 << 20) + 300, (1 << 20) + 290
+    q = np.zeros((2, kv_heads * w), np.float32)
+    c = P.DeviceArray.from_host(np.zeros((rows, kv_heads * w), np.uint16))
+    lib = _lib.load()
+    r = np.random.default_rng(0)
+    some = {t: r.standard_normal(kv_heads * w).astype(np.float16) for t in (5, past - 3, past + 1)}
+    for t, x in some.items():
+        P.check(lib.prana_memcpy_h2d(C.c_void_p(c.ptr.value + t * kv_heads * w * 2), C.c_void_p(x.ctypes.data), x.nbytes))
+    # scores of 20 there and 0 elsewhere
+    for i, t in ((0, past - 3), (1, past + 1)):
+        for h in range(kv_heads):
+            x = some[t][h * w:(h + 1) * w].astype(np.float64)
+            q[i, h * w:(h + 1) * w] = 20 * np.sqrt(w) * x / (x @ x)
+    got = P.attention_tree(q, [P.KvF16(c, c)], [past], [2], kv_heads, kv_heads, w)
+    for i in range(2):
+        for h in range(kv_heads):
+            a = slice(h * w, (h + 1) * w)
+            t = [t for t in some if t <= past + i]
+            k = np.stack([some[x][a].astype(np.float64) for x in t])
+            s = k @ q[i, a].astype(np.float64) / np.sqrt(w)
+            p = np.exp(s)
+            den = p.sum() + (past + 1 + i - len(t))  # the rows of zeros
+            want = p @ k / den
+            # as derived in serving_oracle.py, with n rows of which only these have values
+            ds = ((w + 8) * SO.U * (np.abs(k) @ np.abs(q[i, a].astype(np.float64))) / np.sqrt(w) + 4 * SO.U * np.abs(s)).max()
+            bound = (p @ np.abs(k) / den) * (2 * ds + 8 * SO.U + 2 * past * SO.U) + 2.0 ** -31 * len(t) * np.abs(k).max()
+            assert (np.abs(got[i, a] - want) <= bound).all()
+
+
 def test_empty_calls():
     lib = _lib.load()
     P.init()
