@@ -35,8 +35,8 @@ namespace {
 constexpr int kPkNT = 256;     // lanes of a workgroup
 constexpr int kPkRows = 128;   // rows of a workgroup
 constexpr float kLag = 8.0f;   // how far (log2) scores may pass the kept maximum
-constexpr float kPShift = 7.0f;  // f32 form: probabilities are kept times 2^7 (at most 2^15), so that
-                                 // the smaller half of one resolves 2^-32 of the largest
+constexpr float kPShift = 7.0f;  // probabilities are kept times 2^7 (at most 2^15), so that a half (the smaller
+                                 // half of two) resolves 2^-32 of the largest
 
 struct PackedArgs {
   const void* q;
@@ -145,8 +145,10 @@ __device__ __forceinline__ bool stage_tile(uint16_t* s_k, uint16_t* s_v, u32x4* 
 template <bool HALF>
 __device__ __forceinline__ void store4(void* out, size_t at, float a, float b, float c, float d) {
   if constexpr (HALF) {
-    const half4 y = {static_cast<_Float16>(a), static_cast<_Float16>(b), static_cast<_Float16>(c),
-                     static_cast<_Float16>(d)};
+    // A weighted mean of halves is no larger than they are, but the roundings
+    // of its weights (2^-11) can carry one at the end of their range past it.
+    auto half = [](float x) { return static_cast<_Float16>(fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x); };
+    const half4 y = {half(a), half(b), half(c), half(d)};
     *reinterpret_cast<half4*>(static_cast<uint16_t*>(out) + at) = y;
   } else {
     *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(a, b, c, d);
@@ -235,7 +237,7 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
 #pragma unroll
         for (int i = 0; i < 16; i++) o[mb][i] *= al;
     }
-    const float ms = HALF ? m : m - kPShift;
+    const float ms = m - kPShift;
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
 #pragma unroll
@@ -412,7 +414,7 @@ __global__ __launch_bounds__(kWideGroups* kPkNT, 2) void packed_wide_kernel(Pack
 #pragma unroll
         for (int i = 0; i < 4; i++) o[mb][i] *= al;
     }
-    const float ms = HALF ? m : m - kPShift;
+    const float ms = m - kPShift;
     half8 ph, pl;
 #pragma unroll
     for (int b = 0; b < 2; b++)
@@ -535,7 +537,8 @@ int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v,
   // the longest first: a workgroup's work grows with its place in its sequence
   std::stable_sort(seqs.begin(), seqs.end(), [](const Seq& x, const Seq& y) { return x.len > y.len; });
   const size_t tile_rows = head_dim <= 128 ? kPkRows : kWideRows;
-  const size_t most = 0x7fffffffu / n_kv_heads;  // tiles of one grid
+  // Tiles of one grid: its lanes are to fit 32 bits (one sequence's do, by the length check).
+  const size_t most = (size_t{1} << 22) / n_kv_heads;
   for (size_t i = 0; i < seqs.size();) {
     size_t tiles = 0;
     a.n_seq = 0;

@@ -10,7 +10,7 @@ namespace prana {
 
 namespace {
 
-constexpr size_t kMaxRows = size_t{1} << 30;  // rows of one sequence: row and key indices fit 32 bits
+constexpr size_t kMaxRows = size_t{1} << 30;  // rows (times heads) of one sequence: indices and grids fit 32 bits
 
 constexpr size_t kMaxStride = size_t{1} << 24;  // row strides: 63 rows' bytes fit 32 bits
 
@@ -38,7 +38,7 @@ int check_attention_packed(const void* q, const uint16_t* k, const uint16_t* v, 
   if (n_seq && !seq_lens) return refuse(what, "null seq_lens");
   size_t total = 0;
   for (size_t i = 0; i < n_seq; i++) {
-    if (seq_lens[i] > kMaxRows || seq_lens[i] * (n_heads / n_kv_heads) > kMaxRows)
+    if (seq_lens[i] > kMaxRows || seq_lens[i] * n_heads > kMaxRows)
       return refuse(what, "sequence " + std::to_string(i) + " is too long");
     total += seq_lens[i];
     if (total > 0xffffffffu) return refuse(what, "more than 2^32 - 1 rows");

@@ -147,6 +147,73 @@ def test_f32_queries_beyond_halves(size):
     assert ok, worst
 
 
+@pytest.mark.parametrize("w", [64, 256])
+def test_f16_results_at_the_end_of_their_range(w):
+    # means of +-65504 and of it alone: no rounding of a weight carries one past it
+    n = 150
+    q, k, v = inputs(5, n, 2, 1, w, True)
+    v[:] = np.float16(65504)
+    v[:, 1::2] = np.float16(-65504)
+    got = P.attention_packed(q, k, v, [n], 2, 1, w).reshape(n, 2, w)
+    # off by the weights' roundings (2^-11) and the result's own, and never past the end
+    assert np.isfinite(got).all() and (np.abs(got.astype(np.float64)) >= 65504 * (1 - 2.0 ** -10)).all()
+    assert (got[..., 0::2] > 0).all() and (got[..., 1::2] < 0).all()
+    v[7, 3] = np.inf  # but an infinity that a row sees is one
+    got = P.attention_packed(q, k, v, [n], 2, 1, w).reshape(n, 2, w)
+    assert not np.isfinite(got[7:, :, 3]).any() and np.isfinite(got[:7]).all()
+    assert np.isfinite(np.delete(got, 3, 2)).all()
+
+
+@pytest.mark.parametrize("w", [8, 136])
+def test_many_small_probabilities_of_an_f16_call_are_not_lost(w):
+    # the first key outweighs each other one by 2^25: 20000 of those are 6e-4 of
+    # the result. A probability is off by at most 2^-32 of the largest, the rest
+    # are the roundings of a probability and of the result (2^-11 each, 2^-25).
+    n = 20000
+    q, k, v = np.zeros((n, w), np.float16), np.zeros((n, w), np.float16), np.zeros((n, w), np.float16)
+    s0 = 25 * np.log(2)
+    q[:, 0] = 4
+    k[0, 0] = s0 * np.sqrt(w) / 4
+    v[1:] = 1
+    got = P.attention_packed(q, k, v, [n], 1, 1, w).astype(np.float64)
+    p = np.exp(-float(k[0, 0]) * 4 / np.sqrt(w))
+    i = np.arange(n)[:, None]
+    want = i * p / (1 + i * p)
+    assert (np.abs(got - want) <= want * 2.0 ** -10 + 2.0 ** -25 + i * 2.0 ** -32 + want * n * 2.0 ** -23).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("w", [64, 256])
+def test_a_query_that_is_not_a_number_spoils_its_row_alone(half, w):
+    q, k, v = inputs(9, 200, 4, 2, w, half)
+    clean = P.attention_packed(q, k, v, [200], 4, 2, w)
+    q[70, w + 5] = np.nan
+    got = P.attention_packed(q, k, v, [200], 4, 2, w)
+    assert np.isnan(got[70, w:2 * w]).all()
+    got[70, w:2 * w] = clean[70, w:2 * w]
+    assert np.array_equal(got, clean)
+
+
+def test_offsets_past_32_bits():
+    # f16 rows of a fused buffer 2^24 values apart: q, k and v beside one another,
+    # the second prompt 4 GiB behind the first
+    heads, w, ld, lens = 1, 8, 1 << 24, [130, 7]
+    n = sum(lens)
+    q, k, v = inputs(4, n, heads, heads, w, True)
+    lib = _lib.load()
+    buf = P.DeviceArray((n * ld,), np.uint16)
+    host = np.ascontiguousarray(np.concatenate([q, k, v], 1))
+    for i in range(n):
+        P.check(lib.prana_memcpy_h2d(C.c_void_p(buf.ptr.value + i * ld * 2), C.c_void_p(host[i].ctypes.data), 48))
+    out = P.DeviceArray((n, w), np.float16)
+    at = [C.c_void_p(buf.ptr.value + 16 * i) for i in range(3)]
+    P.check(lib.prana_attention_packed(at[0], at[1], at[2], P.F16, (C.c_size_t * 2)(*lens), 2, heads, heads, w, ld, ld,
+                                       w, out.ptr, None))
+    want, bound = SO.packed(q, k, v, lens, heads, heads, w)
+    ok, worst = SO.within(out.to_host(), want, bound)
+    assert ok, worst
+
+
 def test_empty_calls():
     lib = _lib.load()
     P.init()
