@@ -340,6 +340,12 @@ def attention_prefill(q, k, v, seq, n_heads, n_kv_heads, head_dim):
 
 
 # ---------------------------------------------------------------- serving
+def _halves(a):
+    a = np.ascontiguousarray(a)
+    _want(a.dtype.itemsize == 2, "halves (f16 values or their bits) are expected")
+    return a.view(np.uint16)
+
+
 class KvF16:
     """One sequence's f16 K/V cache on the device: [rows, n_kv_heads*head_dim]
     halves (host arrays are copied; DeviceArrays are used in place)."""
@@ -347,9 +353,10 @@ class KvF16:
     kind = KV_F16
 
     def __init__(self, k, v):
-        self.k, self.v = (c if isinstance(c, DeviceArray)
-                          else DeviceArray.from_host(np.ascontiguousarray(c).view(np.uint16)) for c in (k, v))
-        self.rows = self.k.shape[0]
+        self.k, self.v = (c if isinstance(c, DeviceArray) else DeviceArray.from_host(_halves(c)) for c in (k, v))
+        _want(self.k.shape == self.v.shape and len(self.k.shape) == 2, "k and v are [rows, values] of one shape")
+        _want(self.k.dtype.itemsize == self.v.dtype.itemsize == 2, "k and v are halves")
+        self.rows, self.width = self.k.shape
 
     def struct(self):
         return PranaKv(self.k.ptr, self.v.ptr, None, None, self.rows)
@@ -362,7 +369,7 @@ class KvQ8:
     kind = KV_Q8
 
     def __init__(self, rows, n_kv_heads, head_dim):
-        self.rows, self.n_kv_heads, self.head_dim = rows, n_kv_heads, head_dim
+        self.rows, self.n_kv_heads, self.head_dim, self.width = rows, n_kv_heads, head_dim, n_kv_heads * head_dim
         self.k, self.v = (DeviceArray.from_host(np.zeros((rows, n_kv_heads * head_dim), np.int8)) for _ in "kv")
         self.k_scales, self.v_scales = (DeviceArray.from_host(np.ones((rows, n_kv_heads), np.float32)) for _ in "kv")
 
@@ -378,32 +385,58 @@ def _kv_structs(caches):
     return (PranaKv * max(len(caches), 1))(*[c.struct() for c in caches])
 
 
+# The library takes the shapes on trust; these are what it cannot see.
+def _want(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _check_caches(caches, kinds, width, *per_seq):
+    _want(len({c.kind for c in caches}) <= 1 and all(c.kind in kinds for c in caches), "caches of another kind")
+    _want(all(c.width == width for c in caches), f"a cache's rows are not {width} values")
+    _want(all(len(x) == len(caches) for x in per_seq), "one size per cache")
+    _want(all(int(x) >= 0 for sizes in per_seq for x in sizes), "a negative size")
+
+
 def kv_write_q8(caches, k, v, first_rows, n_rows):
     """Quantize the packed f32 rows of k and v into KvQ8 caches: the next
     n_rows[s] rows become rows first_rows[s].. of caches[s]."""
-    dk, dv = DeviceArray.from_host(np.asarray(k, np.float32)), DeviceArray.from_host(np.asarray(v, np.float32))
+    if not caches:
+        return
+    k, v = np.asarray(k, np.float32), np.asarray(v, np.float32)
+    heads, w = caches[0].n_kv_heads, caches[0].head_dim
+    _check_caches(caches, (KV_Q8,), heads * w, first_rows, n_rows)
+    _want(all(c.n_kv_heads == heads for c in caches), "caches of other heads")
+    _want(k.shape == v.shape == (sum(n_rows), heads * w), "k and v hold the rows of n_rows, one after another")
+    dk, dv = DeviceArray.from_host(k), DeviceArray.from_host(v)
     check(load().prana_kv_write_q8(dk.ptr, dv.ptr, dk.shape[1], _kv_structs(caches), _sizes(first_rows),
-                                   _sizes(n_rows), len(caches), caches[0].n_kv_heads, caches[0].head_dim, None))
+                                   _sizes(n_rows), len(caches), heads, w, None))
     check(load().prana_synchronize())
 
 
 def kv_read_q8(caches, first_rows, n_rows, half=False):
-    """Rows of KvQ8 caches as values, packed: (k, v) in f32, or in f16."""
-    width = caches[0].n_kv_heads * caches[0].head_dim
-    dk, dv = (DeviceArray((int(sum(n_rows)), width), np.float16 if half else np.float32) for _ in "kv")
-    check(load().prana_kv_read_q8(_kv_structs(caches), _sizes(first_rows), _sizes(n_rows), len(caches),
-                                  caches[0].n_kv_heads, caches[0].head_dim, F16 if half else F32, dk.ptr, dv.ptr,
-                                  width, None))
+    """Rows of KvQ8 caches (at least one cache) as values, packed: (k, v) in
+    f32, or in f16."""
+    _want(len(caches) > 0, "no cache")
+    heads, w = caches[0].n_kv_heads, caches[0].head_dim
+    _check_caches(caches, (KV_Q8,), heads * w, first_rows, n_rows)
+    _want(all(c.n_kv_heads == heads for c in caches), "caches of other heads")
+    dk, dv = (DeviceArray((int(sum(n_rows)), heads * w), np.float16 if half else np.float32) for _ in "kv")
+    check(load().prana_kv_read_q8(_kv_structs(caches), _sizes(first_rows), _sizes(n_rows), len(caches), heads, w,
+                                  F16 if half else F32, dk.ptr, dv.ptr, heads * w, None))
     return dk.to_host(), dv.to_host()
 
 
 def attention_packed(q, k, v, seq_lens, n_heads, n_kv_heads, head_dim):
     """Causal attention of whole prompts packed behind one another: q [rows,
     n_heads*head_dim] in f32 or f16 (the result has its type), k / v f16 rows."""
-    q = np.ascontiguousarray(q)
-    kind = {np.dtype(np.float32): F32, np.dtype(np.float16): F16}[q.dtype]
-    dq = DeviceArray.from_host(q)
-    dk, dv = (DeviceArray.from_host(np.ascontiguousarray(x).view(np.uint16)) for x in (k, v))
+    q, k, v = np.ascontiguousarray(q), _halves(k), _halves(v)
+    kind = {np.dtype(np.float32): F32, np.dtype(np.float16): F16}.get(q.dtype)
+    _want(kind is not None, "q is f32 or f16")
+    _want(all(int(n) >= 0 for n in seq_lens), "a negative size")
+    _want(q.shape == (sum(seq_lens), n_heads * head_dim), "q holds the rows of seq_lens, one after another")
+    _want(k.shape == v.shape == (sum(seq_lens), n_kv_heads * head_dim), "k and v hold the rows of seq_lens")
+    dq, dk, dv = (DeviceArray.from_host(x) for x in (q, k, v))
     do = DeviceArray(q.shape, q.dtype)
     check(load().prana_attention_packed(dq.ptr, dk.ptr, dv.ptr, kind, _sizes(seq_lens), len(seq_lens), n_heads,
                                         n_kv_heads, head_dim, q.shape[1], dk.shape[1], q.shape[1], do.ptr, None))
@@ -412,6 +445,7 @@ def attention_packed(q, k, v, seq_lens, n_heads, n_kv_heads, head_dim):
 
 def attention_tree_workspace(past, n_tree, n_heads, n_kv_heads, head_dim):
     """Bytes of device scratch attention_tree needs for these sizes."""
+    _want(len(past) == len(n_tree) and all(int(x) >= 0 for x in [*past, *n_tree]), "one size per sequence")
     n = C.c_size_t()
     check(load().prana_attention_tree_workspace(_sizes(past), _sizes(n_tree), len(past), n_heads, n_kv_heads,
                                                 head_dim, C.byref(n)))
@@ -422,7 +456,14 @@ def attention_tree(q, caches, past, n_tree, n_heads, n_kv_heads, head_dim, mask=
     """Attention of drafted tokens, a tree per sequence, over KvF16 or KvQ8
     caches: q [sum(n_tree), n_heads*head_dim] f32, mask one word per drafted
     token (bit j: it sees drafted token j of its sequence; None = a chain)."""
-    dq = DeviceArray.from_host(np.asarray(q, np.float32))
+    q = np.asarray(q, np.float32)
+    _check_caches(caches, (KV_F16, KV_Q8), n_kv_heads * head_dim, past, n_tree)
+    _want(all(c.kind != KV_Q8 or c.n_kv_heads == n_kv_heads for c in caches), "caches of other heads")
+    _want(q.shape == (sum(n_tree), n_heads * head_dim), "q holds the rows of n_tree, one after another")
+    _want(mask is None or np.shape(mask) == (sum(n_tree),), "one mask word per drafted token")
+    if not caches:
+        return q.copy()
+    dq = DeviceArray.from_host(q)
     dm = DeviceArray.from_host(np.asarray(mask, np.uint64)) if mask is not None else None
     work = DeviceArray((attention_tree_workspace(past, n_tree, n_heads, n_kv_heads, head_dim),), np.uint8)
     do = DeviceArray(dq.shape, np.float32)

@@ -262,8 +262,8 @@ int launch_moves(Move m, const void* k, const void* v, size_t ld, const prana_kv
     return kOk;
   };
   for (size_t i = 0; i < n_seq; i++) {
-    // a launch's grid stays far from 2^31 workgroups: long sequences go in parts
-    constexpr size_t kPartBlocks = size_t{1} << 24;
+    // a launch's lanes fit 32 bits: long sequences go in parts
+    constexpr size_t kPartBlocks = size_t{1} << 22;
     const size_t part = std::max<size_t>(1, kPartBlocks * per_block / n_kv);
     for (size_t r = 0; r < n_rows[i]; r += part) {
       const size_t rows = std::min(part, n_rows[i] - r);

@@ -108,6 +108,22 @@ def test_strided_rows_many_sequences_and_nothing_outside():
     assert np.all(got[:total, 2 * heads * w:] == 7) and np.all(got[total] == 7)
 
 
+def test_offsets_past_32_bits():
+    # rows that lie 4 GiB behind the cache's first
+    heads, w, rows = 8, 256, (1 << 21) + 40
+    c = P.KvQ8.__new__(P.KvQ8)
+    c.rows, c.n_kv_heads, c.head_dim, c.width = rows, heads, w, heads * w
+    c.k, c.v = (P.DeviceArray((rows, heads * w), np.int8) for _ in "kv")
+    c.k_scales, c.v_scales = (P.DeviceArray((rows, heads), np.float32) for _ in "kv")
+    r = np.random.default_rng(0)
+    k, v = (r.standard_normal((50, heads * w)).astype(np.float32) for _ in "kv")
+    P.kv_write_q8([c, c], k, v, [rows - 40, 3], [40, 10])
+    for got, x in zip(P.kv_read_q8([c, c], [rows - 40, 3], [40, 10]), (k, v)):
+        q, s = SO.quantize(x, heads, w)
+        want = (q.reshape(50, heads, w) * s[..., None]).reshape(50, heads * w)
+        assert (np.abs(got - want) <= np.abs(want) * 2.0 ** -22).all()
+
+
 def test_empty_calls():
     lib = _lib.load()
     P.init()

@@ -3,6 +3,7 @@ device is touched, so none of these calls needs a GPU, and no pointer here is
 ever followed."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 import prana_amd as P
@@ -175,3 +176,48 @@ def test_tree_mask():
     for bad in ([0], [-1, 1], [-1, -2]):
         with pytest.raises(ValueError):
             P.tree_mask(bad)
+
+
+class Cache:
+    """A cache that is never touched: the shapes are refused first."""
+
+    def __init__(self, kind=P.KV_Q8, n_kv_heads=2, head_dim=8, rows=9):
+        self.kind, self.n_kv_heads, self.head_dim, self.rows = kind, n_kv_heads, head_dim, rows
+        self.width = n_kv_heads * head_dim
+
+
+def rows(n, width, dtype=np.float32):
+    return np.zeros((n, width), dtype)
+
+
+@pytest.mark.parametrize("call,says", [
+    (lambda: P.attention_packed(rows(5, 32), rows(5, 16, np.float16), rows(5, 16, np.float16), [2, 2], 4, 2, 8), "q holds"),
+    (lambda: P.attention_packed(rows(4, 32), rows(4, 16, np.float16), rows(3, 16, np.float16), [4], 4, 2, 8), "k and v hold"),
+    (lambda: P.attention_packed(rows(4, 32), rows(4, 16), rows(4, 16), [4], 4, 2, 8), "halves"),
+    (lambda: P.attention_packed(rows(4, 32, np.float64), *[rows(4, 16, np.float16)] * 2, [4], 4, 2, 8), "f32 or f16"),
+    (lambda: P.attention_packed(rows(4, 32), *[rows(4, 16, np.float16)] * 2, [5, -1], 4, 2, 8), "negative"),
+    (lambda: P.kv_write_q8([Cache()], rows(4, 16), rows(4, 16), [0], [3]), "k and v hold"),
+    (lambda: P.kv_write_q8([Cache()], rows(3, 8), rows(3, 8), [0], [3]), "k and v hold"),
+    (lambda: P.kv_write_q8([Cache()] * 2, rows(3, 16), rows(3, 16), [0], [3]), "one size"),
+    (lambda: P.kv_write_q8([Cache(P.KV_F16)], rows(3, 16), rows(3, 16), [0], [3]), "another kind"),
+    (lambda: P.kv_write_q8([Cache(), Cache(n_kv_heads=1, head_dim=16)], rows(3, 16), rows(3, 16), [0, 0], [1, 2]),
+     "other heads"),
+    (lambda: P.kv_read_q8([], [], []), "no cache"),
+    (lambda: P.kv_read_q8([Cache()], [0, 1], [3]), "one size"),
+    (lambda: P.kv_read_q8([Cache(), Cache(head_dim=16)], [0, 1], [3, 3]), "not 16 values"),
+    (lambda: P.attention_tree(rows(3, 32), [Cache(), Cache(P.KV_F16)], [2, 2], [1, 2], 4, 2, 8), "another kind"),
+    (lambda: P.attention_tree(rows(3, 32), [Cache(head_dim=16)], [2], [3], 4, 2, 8), "not 16 values"),
+    (lambda: P.attention_tree(rows(3, 32), [Cache(n_kv_heads=1, head_dim=16)], [2], [3], 4, 2, 8), "other heads"),
+    (lambda: P.attention_tree(rows(3, 32), [Cache()], [2], [2], 4, 2, 8), "q holds"),
+    (lambda: P.attention_tree(rows(3, 32), [Cache()], [2, 2], [3], 4, 2, 8), "one size"),
+    (lambda: P.attention_tree(rows(3, 32), [Cache()], [2], [3], 4, 2, 8, mask=[1, 3]), "one mask word"),
+    (lambda: P.attention_tree_workspace([1, 2], [1], 4, 2, 8), "one size"),
+])
+def test_shapes_that_do_not_belong_together(call, says):
+    with pytest.raises(ValueError, match=says):
+        call()
+
+
+def test_a_sequence_of_more_than_2_to_30_rows_and_heads():
+    assert packed(lens=((1 << 27) + 1,)) == INVALID and "sequence 0 is too long" in message()
+    assert packed(lens=(1 << 27,), q=None) == INVALID and "null buffer" in message()  # (its length is taken)
