@@ -192,10 +192,14 @@ int prana_attention_prefill(const float *q, const float *k, const float *v, size
  * host arrays that are read before the call returns. They are asynchronous on
  * `stream` (NULL = the library's), allocate nothing and keep nothing between
  * calls, so they may be captured into a HIP graph; a replay repeats the call
- * with the sizes and pointers it was captured with. Results are f32-accurate
- * (not the scalar tier's bits). Device pointers lie on 16 bytes (scales on 4),
- * row strides are multiples of 16 bytes and head_dim is a multiple of 8 up to
- * 256; anything else is PRANA_ERR_INVALID. Outputs do not overlap inputs. */
+ * with the sizes and pointers it was captured with. f32 results are
+ * f32-accurate (not the scalar tier's bits); an f16 result rounds its
+ * probabilities and itself to halves. Equal calls give equal bits. Device
+ * pointers lie on 16 bytes (scales on 4), row strides are multiples of 16 bytes
+ * and at most 2^24 elements, head_dim is a multiple of 8 up to 256; anything
+ * else is PRANA_ERR_INVALID. Outputs do not overlap inputs or one another. In
+ * attention, an infinity or NaN that a row sees makes what it reaches of that
+ * row infinite or NaN, and no other row's. */
 
 /* Causal attention of whole prompts: sequence s is the next seq_lens[s] rows
  * (0 allowed) of q, k, v and out, and its row i attends to its rows 0..=i. q
@@ -245,7 +249,8 @@ int prana_kv_read_q8(const prana_kv *kv, const size_t *first_rows, const size_t 
  * to q. What masked rows and rows past the drafted ones hold (infinities and
  * NaN too) does not reach the result. workspace: device scratch of the size
  * prana_attention_tree_workspace gives for the same sizes (it may be 0, then
- * workspace may be NULL); calls that may run at the same time need one each. */
+ * workspace may be NULL); calls that may run at the same time (also replays of
+ * two captured graphs) need one each. 8-bit: values up to 2^64 in magnitude. */
 int prana_attention_tree(const float *q, int kv_type, const prana_kv *kv, const size_t *past, const size_t *n_tree,
                          size_t n_seq, const uint64_t *mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
                          float *out, void *workspace, size_t workspace_bytes, prana_stream_t stream);
