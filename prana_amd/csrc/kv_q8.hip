@@ -151,8 +151,8 @@ __global__ __launch_bounds__(kKvNT) void kv_write_kernel(KvArgs a) {
     if (!finite) scale = __uint_as_float(0x7fc00000u);  // reads back as NaN
     const size_t r = static_cast<size_t>(sq.first) + row;
     if (live)
-      *reinterpret_cast<uint2*>(dst + (r * a.n_kv + head) * a.hd + sub * 8) = make_uint2(w[0], w[1]);
-    if (sub == 0) sq.scales[r * a.n_kv + head] = scale;
+      *(device_t<u32x2>*)(dst + (r * a.n_kv + head) * a.hd + sub * 8) = u32x2{w[0], w[1]};
+    if (sub == 0) *(device_t<float>*)(sq.scales + r * a.n_kv + head) = scale;
   }
 }
 
@@ -179,8 +179,8 @@ __global__ __launch_bounds__(kKvNT) void kv_read_kernel(KvArgs a) {
     scale[it] = 0.0f;
     if (item < n_items) {
       const size_t at = static_cast<size_t>(sq.first) * a.n_kv + item;  // (row, head) of the cache
-      w[it] = *reinterpret_cast<const Word*>(src + at * a.hd + sub * kPer);
-      scale[it] = sq.scales[at];
+      w[it] = load_at<Word>(src + at * a.hd + sub * kPer);
+      scale[it] = load_at<float>(sq.scales + at);
     }
   }
 #pragma unroll

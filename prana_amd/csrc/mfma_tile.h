@@ -22,6 +22,19 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// A value in device memory, at a byte offset from a base. Said outright: a
+// pointer that came through a register exchange or an opaque assembly statement
+// may point anywhere for all the compiler knows, and its generic loads count
+// as LDS accesses too, so that each wait for LDS would wait for the loads of the
+// next tile with it (4 prompts up to 1025, 8/1 x 256: 39.1 us with them, 37.3
+// without; 9 prompts up to 8192: 828, 816).
+template <class T>
+using device_t = __attribute__((address_space(1))) T;
+template <class T>
+__device__ __forceinline__ T load_at(const void* base, uint32_t off = 0) {
+  return *(const device_t<T>*)((const device_t<unsigned char>*)(base) + off);
+}
+
 // Transposing LDS read of halves: the 16 lanes of a group read 4 rows of 16
 // (lane l the four at row l / 4, column 4 (l % 4)), and lane l gets column l,
 // rows 0..3.

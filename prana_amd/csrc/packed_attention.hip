@@ -94,17 +94,17 @@ struct TileFetch {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         const size_t up = kEven ? i * (kPkNT / CHUNKS) * ld : 0;
-        kr[i] = *reinterpret_cast<const u32x4*>(kp + up + off[kEven ? 0 : i]);
-        vr[i] = *reinterpret_cast<const u32x4*>(vp + up + off[kEven ? 0 : i]);
+        kr[i] = load_at<u32x4>(kp + up, off[kEven ? 0 : i]);
+        vr[i] = load_at<u32x4>(vp + up, off[kEven ? 0 : i]);
       }
     } else {  // keys past the end: K repeats the last (and is masked), V is 0
       const uint32_t last = len - 1 - k0;
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         const uint32_t e = i * kPkNT + tid, at = offset(e, last);
-        kr[i] = *reinterpret_cast<const u32x4*>(kp + at);
+        kr[i] = load_at<u32x4>(kp, at);
         vr[i] = u32x4{0, 0, 0, 0};
-        if (e / CHUNKS <= last) vr[i] = *reinterpret_cast<const u32x4*>(vp + at);
+        if (e / CHUNKS <= last) vr[i] = load_at<u32x4>(vp, at);
       }
     }
   }

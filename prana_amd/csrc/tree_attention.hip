@@ -112,7 +112,7 @@ struct Piece {
   u32x4 w;
   __device__ __forceinline__ void zero() { w = u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ void load(const unsigned char* base, uint32_t off) {
-    w = *reinterpret_cast<const u32x4*>(base + off);
+    w = load_at<u32x4>(base, off);
   }
   __device__ __forceinline__ u32x4 halves() const { return w; }
 };
@@ -121,7 +121,7 @@ struct Piece<true> {
   u32x2 w;
   __device__ __forceinline__ void zero() { w = u32x2{0, 0}; }
   __device__ __forceinline__ void load(const unsigned char* base, uint32_t off) {
-    w = *reinterpret_cast<const u32x2*>(base + off);
+    w = load_at<u32x2>(base, off);
   }
   __device__ __forceinline__ u32x4 halves() const { return i8_to_halves(w); }
 };
@@ -130,11 +130,11 @@ struct Piece<true> {
 template <bool Q8>
 __device__ __forceinline__ void load_values(const unsigned char* p, float scale, float* x) {
   if constexpr (Q8) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    const uint32_t w = load_at<uint32_t>(p);
 #pragma unroll
     for (int j = 0; j < 4; j++) x[j] = static_cast<float>(static_cast<int8_t>(w >> (8 * j))) * scale;
   } else {
-    const half4 v = *reinterpret_cast<const half4*>(p);
+    const half4 v = load_at<half4>(p);
 #pragma unroll
     for (int j = 0; j < 4; j++) x[j] = static_cast<float>(v[j]);
   }
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
 #pragma unroll
       for (int p = 0; p < S::kPieces; p++)
         vr[p].load(kEvenRows ? vp + p * (64 / kRowPieces) * ld * kSize : vp, voff[kEvenRows ? 0 : p]);
-      if constexpr (Q8) sr = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
+      if constexpr (Q8) sr = load_at<float>(scales + static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv);
     } else {  // keys past the end: V is 0
       const uint32_t last = kend - 1 - k0;
 #pragma unroll
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
       }
       if constexpr (Q8) {
         sr = 0.0f;
-        if ((lane & 31u) <= last) sr = scales[static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv];
+        if ((lane & 31u) <= last) sr = load_at<float>(scales + static_cast<size_t>(k0 + (lane & 31u)) * a.n_kv);
       }
     }
   };
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
       for (uint32_t t = k0; t < min(k0 + 32, kend); t++) {
         float scale = 1.0f;
         if constexpr (Q8) {
-          scale = sq.vs[static_cast<size_t>(t) * a.n_kv + kvh];
+          scale = load_at<float>(sq.vs + static_cast<size_t>(t) * a.n_kv + kvh);
           if (finite(scale)) continue;
         }
 #pragma unroll
@@ -609,7 +609,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
     const unsigned char* vp = vbase + k0 * ld * kSize;
     const bool whole = k0 + BN <= kend;
     const uint32_t last = whole ? BN - 1 : kend - 1 - k0;  // keys past the end repeat the last
-    if constexpr (Q8) sc = scales[static_cast<size_t>(k0 + min(tid % BN + 0u, last)) * a.n_kv];
+    if constexpr (Q8) sc = load_at<float>(scales + static_cast<size_t>(k0 + min(tid % BN + 0u, last)) * a.n_kv);
 #pragma unroll
     for (int p = 0; p < S::kLoads; p++) {
       const uint32_t e = p * kTrNT + tid, r = e / S::kChunks;
@@ -784,7 +784,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
       for (uint32_t t = k0; t < min(k0 + BN, kend); t++) {
         float scale = 1.0f;
         if constexpr (Q8) {
-          scale = sq.vs[static_cast<size_t>(t) * a.n_kv + kvh];
+          scale = load_at<float>(sq.vs + static_cast<size_t>(t) * a.n_kv + kvh);
           if (finite(scale)) continue;
         }
         if (!(seen_from(word, static_cast<int>(t) - static_cast<int>(sq.past)) & 1)) continue;
