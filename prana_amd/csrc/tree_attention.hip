@@ -180,14 +180,6 @@ struct NarrowShape {
   static constexpr int kBytes = kWaves * std::max(kWaveHalves * 2, 16 * kLdO * 4);
 };
 
-template <bool FIRST, class T>
-__device__ __forceinline__ T& pick_pieces(T& a, T& b) {
-  if constexpr (FIRST)
-    return a;
-  else
-    return b;
-}
-
 template <int HDP, int RB, bool Q8>
 __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
   using S = NarrowShape<HDP>;
@@ -305,25 +297,9 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
   for (int r = 0; r < RB; r++) c[r] = s_c[r * 16 + n];
   ScaleTop top;
   for (; k0 < kend; k0 += S::kRound) {
-    // One block of rows: the next keys are under way while these are computed.
-    // Two leave no registers for that: the next ones follow as these are used.
+    // the next keys follow into the registers as these leave them
     const bool more = k0 + S::kRound < kend;
-    Piece<Q8> kc[2][S::kSteps], vc[S::kPieces];
     float sc = sr;
-    if constexpr (RB == 1) {
-#pragma unroll
-      for (int p = 0; p < S::kPieces; p++) vc[p] = vr[p];
-#pragma unroll
-      for (int b = 0; b < 2; b++)
-#pragma unroll
-        for (int s = 0; s < S::kSteps; s++) kc[b][s] = kr[b][s];
-      if (more) {
-        fetch_v(k0 + S::kRound);
-        fetch_k(k0 + S::kRound);
-      }
-    }
-    Piece<Q8>* const vu = RB == 1 ? vc : vr;
-    auto& ku = pick_pieces<RB == 1>(kc, kr);
     const bool edge = k0 + 32 > min(sq.past, kend);  // not every row sees every key
     bool odd = false;
     if constexpr (!Q8) {
@@ -332,11 +308,11 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
       if (edge) {
         uint32_t bits = 0;
 #pragma unroll
-        for (int p = 0; p < S::kPieces; p++) bits |= odd_halves(vu[p].w);
+        for (int p = 0; p < S::kPieces; p++) bits |= odd_halves(vr[p].w);
         odd = __any((bits & kOddBits) != 0);
         if (odd) {
 #pragma unroll
-          for (int p = 0; p < S::kPieces; p++) vu[p].w = only_finite(vu[p].w);
+          for (int p = 0; p < S::kPieces; p++) vr[p].w = only_finite(vr[p].w);
         }
       }
     }
@@ -353,7 +329,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
 #pragma unroll
     for (int p = 0; p < S::kPieces; p++) {
       const int e = p * 64 + lane;
-      *reinterpret_cast<u32x4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vu[p].halves();
+      *reinterpret_cast<u32x4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vr[p].halves();
     }
     if constexpr (Q8) {
       s_scale[wave][lane] = sc;
@@ -373,8 +349,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 
-    if constexpr (RB > 1)
-      if (more) fetch_v(k0 + S::kRound);
+    if (more) fetch_v(k0 + S::kRound);
     f32x4 s[RB][2], s2[RB][2];  // from both halves of q
 #pragma unroll
     for (int r = 0; r < RB; r++)
@@ -386,7 +361,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
     for (int b = 0; b < 2; b++)
 #pragma unroll
       for (int t = 0; t < S::kSteps; t++) {
-        const half8 kf = __builtin_bit_cast(half8, ku[b][t].halves());
+        const half8 kf = __builtin_bit_cast(half8, kr[b][t].halves());
 #pragma unroll
         for (int r = 0; r < RB; r++) {
           const uint16_t* qp = s_q[0] + (r * 16 + n) * S::kLdQ + t * 32 + g * 8;
@@ -396,8 +371,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
           s2[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql, s2[r][b], 0, 0, 0);
         }
       }
-    if constexpr (RB > 1)
-      if (more) fetch_k(k0 + S::kRound);
+    if (more) fetch_k(k0 + S::kRound);
 #pragma unroll
     for (int r = 0; r < RB; r++)
 #pragma unroll
