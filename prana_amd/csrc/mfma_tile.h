@@ -48,6 +48,21 @@ __device__ __forceinline__ half8 join(half4 a, half4 b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// For a stretch of N LDS reads that feed M products each: two reads first, then
+// one after each read's products, so that a read's wait is behind those of the
+// one before. (On its own the compiler waits for pairs where registers are few.)
+template <int N, int M>
+__device__ __forceinline__ void reads_ahead() {
+  constexpr int kProduct = 0x008, kRead = 0x100;
+  __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+#pragma unroll
+  for (int i = 0; i < N - 2; i++) {
+    __builtin_amdgcn_sched_group_barrier(kProduct, M, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kProduct, 2 * M, 0);
+}
+
 // Accumulators wider than the 256 directly addressed registers leave room for:
 // keeps one in the accumulation registers here, where the products use it in
 // place. (Without this the compiler moves all of them there and back around

@@ -6,7 +6,7 @@
 // cores. The rows of a sequence are its (token, query head of the group)
 // pairs, so the heads that share a KV head share its tiles too; a workgroup
 // takes 128 rows (32 per wave) and walks the keys up to its last token in
-// tiles of kBN, staged through registers into LDS while the tile before is
+// tiles of 64 or 32, staged through registers into LDS while the tile before is
 // computed. Per tile and wave, with 32x32x16 products:
 //   S^T = K Q^T : a lane holds one row's scores, 16 of each 32 keys, so the
 //                 maximum and sum of a row are taken inside two lanes;
@@ -155,8 +155,14 @@ __device__ __forceinline__ void store4(void* out, size_t at, float a, float b, f
   }
 }
 
-template <int HDP, int BN, bool HALF>
+// Keys of a tile: 64, or 32 in the f32 form of heads wider than 96, which 64
+// would make spill (5 prompts up to 700 and 3000, 32/8 x 128: 44 and 663 us with
+// 64, 37 and 641 with 32).
+constexpr int packed_keys(int hdp, bool half) { return half || hdp <= 96 ? 64 : 32; }
+
+template <int HDP, bool HALF>
 __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(PackedArgs a) {
+  constexpr int BN = packed_keys(HDP, HALF);
   using S = PkShape<HDP, BN>;
   static_assert(BN * S::kChunks % kPkNT == 0, "a tile is a whole number of pieces per lane");
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
@@ -497,9 +503,9 @@ void launch_shape(const PackedArgs& a, bool half, uint32_t tiles, hipStream_t s)
   const dim3 grid(tiles * a.n_kv), nt(kPkNT);
   if constexpr (HDP <= 128) {
     if (half)
-      hipLaunchKernelGGL((packed_kernel<HDP, 64, true>), grid, nt, 0, s, a);
+      hipLaunchKernelGGL((packed_kernel<HDP, true>), grid, nt, 0, s, a);
     else
-      hipLaunchKernelGGL((packed_kernel<HDP, 64, false>), grid, nt, 0, s, a);
+      hipLaunchKernelGGL((packed_kernel<HDP, false>), grid, nt, 0, s, a);
   } else {
     if (half)
       hipLaunchKernelGGL((packed_wide_kernel<HDP, true>), grid, dim3(kWideGroups * kPkNT), 0, s, a);

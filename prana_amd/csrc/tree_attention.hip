@@ -19,7 +19,7 @@
 //     from memory straight into the operand's registers, V through a corner of
 //     LDS that only its wave uses, so no wave waits for another until the end.
 //   wide (more rows): bound by the products. Four waves of 32 rows share tiles
-//     of 64 keys in LDS.
+//     of 64 or 32 keys in LDS.
 // In both S^T = K Q^T leaves a row's scores in the lanes of one column, whose
 // registers are, as halves, the operand of O^T += V^T P^T; V comes out of LDS
 // transposed to match. The kept maximum lags the scores by up to 2^8 before
@@ -542,6 +542,11 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
 // ------------------------------------------------------------ wide: 128 rows a workgroup
 constexpr int kWideRows = 128;
 
+// Keys of a tile: 64, or 32 of heads wider than 96, whose scores and keys on
+// their way would spill with 64 (8 trees of 64 over up to 16385, 32/8 x 128:
+// 202 us with 64, 195 with 32; 6 of 48 over up to 9000, 24/6 x 192: 125, 113).
+constexpr int wide_keys(int hdp) { return hdp <= 96 ? 64 : 32; }
+
 template <int HDP, int BN>
 struct WideShape {
   static constexpr int kStepsQK = HDP / 16, kDimBlocks = HDP / 32, kKeyBlocks = BN / 32;
@@ -551,8 +556,9 @@ struct WideShape {
   static constexpr int kLoads = BN * kChunks / kTrNT;
 };
 
-template <int HDP, int BN, bool Q8>
+template <int HDP, bool Q8>
 __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(TreeArgs a) {
+  constexpr int BN = wide_keys(HDP);
   using S = WideShape<HDP, BN>;
   static_assert(BN * S::kChunks % kTrNT == 0, "a tile is a whole number of pieces per lane");
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
@@ -662,6 +668,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[t], s[b], 0, 0, 0);
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[t], s[b], 0, 0, 0);
       }
+    reads_ahead<S::kStepsQK * S::kKeyBlocks, 2>();
     if constexpr (Q8) {
       float v = lane < BN ? s_scale[1][lane] : 0.0f;
       if (!finite(v)) v = 0.0f;
@@ -958,7 +965,7 @@ Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_
   return p;
 }
 
-template <int HDP, int BN>
+template <int HDP>
 void launch_width(const TreeArgs& a, Width w, bool q8, uint32_t items, hipStream_t s) {
   const dim3 grid(items * a.n_kv), nt(w == kWide ? kTrNT : 64 * narrow_waves(HDP));
   if (w == kNarrow16) {
@@ -975,9 +982,9 @@ void launch_width(const TreeArgs& a, Width w, bool q8, uint32_t items, hipStream
     }
   } else {
     if (q8)
-      hipLaunchKernelGGL((tree_wide_kernel<HDP, BN, true>), grid, nt, 0, s, a);
+      hipLaunchKernelGGL((tree_wide_kernel<HDP, true>), grid, nt, 0, s, a);
     else
-      hipLaunchKernelGGL((tree_wide_kernel<HDP, BN, false>), grid, nt, 0, s, a);
+      hipLaunchKernelGGL((tree_wide_kernel<HDP, false>), grid, nt, 0, s, a);
   }
 }
 
@@ -1016,15 +1023,15 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
       if (a.n_seq) {
         const uint32_t it = static_cast<uint32_t>(items);
         if (head_dim <= 64)
-          launch_width<64, 64>(a, static_cast<Width>(w), q8, it, s);
+          launch_width<64>(a, static_cast<Width>(w), q8, it, s);
         else if (head_dim <= 96)
-          launch_width<96, 64>(a, static_cast<Width>(w), q8, it, s);
+          launch_width<96>(a, static_cast<Width>(w), q8, it, s);
         else if (head_dim <= 128)
-          launch_width<128, 64>(a, static_cast<Width>(w), q8, it, s);
+          launch_width<128>(a, static_cast<Width>(w), q8, it, s);
         else if (head_dim <= 192)
-          launch_width<192, 64>(a, static_cast<Width>(w), q8, it, s);
+          launch_width<192>(a, static_cast<Width>(w), q8, it, s);
         else
-          launch_width<256, 32>(a, static_cast<Width>(w), q8, it, s);
+          launch_width<256>(a, static_cast<Width>(w), q8, it, s);
         PRANA_LAUNCH_CHECK();
       }
       if (j.n_seq) {
