@@ -48,7 +48,8 @@ struct TreeArgs {
   float* part;  // [partial row][hd] weighted sums, then [partial row][2] maximum and sum
   size_t part_rows;
   uint32_t n_seq, n_heads, n_kv, group, hd;
-  uint32_t rows_per_split;
+  uint32_t whole;           // a cache of up to this many rows is one part
+  uint32_t rows_per_split;  // of a longer one
   float scale;  // log2(e) / sqrt(hd)
   const void* k[kTableSeqs];
   const void* v[kTableSeqs];
@@ -72,7 +73,8 @@ __device__ __forceinline__ TreeSeq this_seq(const TreeArgs& a, uint32_t item) {
   const int s = table_find(a.item0, a.n_seq, item);
   TreeSeq q{table_at(a.k, s),      table_at(a.v, s),    table_at(a.ks, s),    table_at(a.vs, s),   table_at(a.past, s),
             table_at(a.tokens, s), table_at(a.tok0, s), table_at(a.item0, s), table_at(a.part0, s), 0};
-  q.splits = (q.past + q.tokens + a.rows_per_split - 1) / a.rows_per_split;
+  const uint32_t total = q.past + q.tokens;
+  q.splits = total <= a.whole ? 1 : (total + a.rows_per_split - 1) / a.rows_per_split;
   return q;
 }
 
@@ -194,7 +196,7 @@ __global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : 
   const TreeSeq sq = this_seq(a, item);
   const uint32_t split = item - sq.item0, hd = a.hd;
   const uint32_t rows = sq.tokens * a.group, total = sq.past + sq.tokens;
-  const uint32_t kbeg = split * a.rows_per_split, kend = min(total, kbeg + a.rows_per_split);
+  const uint32_t kbeg = split * a.rows_per_split, kend = sq.splits == 1 ? total : min(total, kbeg + a.rows_per_split);
 
   // Pieces past the head's width repeat its last one: q is 0 there for K, and
   // V columns there are never stored.
@@ -571,7 +573,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   const uint32_t hd = a.hd, rows = sq.tokens * a.group, total = sq.past + sq.tokens;
   const uint32_t row_tiles = (rows + kWideRows - 1) / kWideRows;
   const uint32_t split = (item - sq.item0) / row_tiles, row0 = (item - sq.item0) % row_tiles * kWideRows;
-  const uint32_t kbeg = split * a.rows_per_split, kend = min(total, kbeg + a.rows_per_split);
+  const uint32_t kbeg = split * a.rows_per_split, kend = sq.splits == 1 ? total : min(total, kbeg + a.rows_per_split);
   const bool idle = row0 + wave * 32 >= rows;  // the wave has no rows: it only stages
   const uint32_t row = min(row0 + wave * 32 + n, rows - 1), i = row / a.group;
   const size_t qrow = static_cast<size_t>(i) * a.n_heads + kvh * a.group + row % a.group;
@@ -908,17 +910,24 @@ void launch_join(const JoinArgs& j, hipStream_t s) {
 }
 
 // ------------------------------------------------------------ plan
-// Kernel of a sequence, by its rows per KV head.
+// Kernel of a sequence, by its rows per KV head. Two blocks of narrow rows only
+// over 8-bit caches of heads up to 128 wide, which leave them the registers:
+// 10 tokens in four sequences, 12/4 x 128, caches up to 4000 and 20000, take
+// 16.7 and 28.6 us there and 18.1 and 35 on the wide kernel (three quarters of
+// it idle), but 17.9 and 34 against 13.6 and 29 in f16.
 enum Width { kNarrow16, kNarrow32, kWide, kWidths };
-// (32 narrow rows of heads wider than 128 would not fit the registers.)
-Width width_of(size_t rows, size_t hd) {
-  return rows <= 16 ? kNarrow16 : rows <= 32 && hd <= 128 ? kNarrow32 : kWide;
+Width width_of(size_t rows, size_t hd, bool q8) {
+  return rows <= 16 ? kNarrow16 : rows <= 32 && hd <= 128 && q8 ? kNarrow32 : kWide;
 }
 
 struct Plan {
-  size_t rows_per_split[kWidths];
+  size_t whole[kWidths];           // caches of up to this many rows are one part
+  size_t rows_per_split[kWidths];  // of longer ones
   size_t part_rows;
   size_t floats;
+  size_t parts(int w, size_t total) const {
+    return total <= whole[w] ? 1 : (total + rows_per_split[w] - 1) / rows_per_split[w];
+  }
 };
 
 // Workgroups that run at once: 256 compute units times those whose registers
@@ -930,36 +939,39 @@ size_t resident(Width w, size_t hd) {
 
 // Cache rows of a part, per kernel: the fewest, in whole tiles, that leave no
 // more workgroups than run at once (a few left over for a second round would
-// take as long as all of the first), but not so few that joining the parts
-// costs more than it saves: about 4 us, in which a narrow workgroup takes 512
-// rows and a wide one 128.
-Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd) {
+// take as long as all of the first), and at least one round of a narrow
+// workgroup's waves (256 rows) or 128 rows of a wide one's tiles: one token over
+// 4000 rows, 12/4 x 128, takes 11.3 us with parts of 256 rows, 12.5 with 512 and
+// 17.1 with 1024; 32 tokens over two caches of up to 3000 21.3 with 64, 18.1
+// with 128 and 19.7 with 256. Joining parts costs about 3 us, and a narrow round
+// 1.9, so two rounds are one part (one token over 511 rows: 8.9 us; three, where
+// other sequences of the call have parts: 15.4 against 11.0).
+Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd, bool q8) {
   const size_t group = n_heads / n_kv;
-  auto tiles = [&](size_t i) {
-    const size_t rows = n_tree[i] * group;
-    return width_of(rows, hd) == kWide ? (rows + kWideRows - 1) / kWideRows : 1;
-  };
+  auto width = [&](size_t i) { return width_of(n_tree[i] * group, hd, q8); };
+  auto tiles = [&](size_t i) { return width(i) == kWide ? (n_tree[i] * group + kWideRows - 1) / kWideRows : 1; };
   size_t work[kWidths] = {};  // cache rows times row tiles
   for (size_t i = 0; i < n_seq; i++)
-    if (n_tree[i]) work[width_of(n_tree[i] * group, hd)] += (past[i] + n_tree[i]) * tiles(i);
+    if (n_tree[i]) work[width(i)] += (past[i] + n_tree[i]) * tiles(i);
   Plan p{};
   for (int w = 0; w < kWidths; w++) {
-    const size_t unit = w == kWide ? 64 : 32 * narrow_waves(static_cast<int>(hd)), most = resident(static_cast<Width>(w), hd);
-    size_t r = std::max<size_t>(w == kWide ? 128 : 512, (work[w] * n_kv / most + unit - 1) / unit * unit);
+    const size_t round = 32 * narrow_waves(static_cast<int>(hd)), most = resident(static_cast<Width>(w), hd);
+    const size_t unit = w == kWide ? 64 : round, least = w == kWide ? 128 : round;
+    size_t r = std::max(least, (work[w] * n_kv / most + unit - 1) / unit * unit);
+    p.whole[w] = w == kWide ? least : 2 * round;
     for (int tries = 0; tries < 16; tries++) {
+      p.rows_per_split[w] = r;
       size_t n = 0;
       for (size_t i = 0; i < n_seq; i++)
-        if (n_tree[i] && width_of(n_tree[i] * group, hd) == w) n += (past[i] + n_tree[i] + r - 1) / r * tiles(i);
+        if (n_tree[i] && width(i) == w) n += p.parts(w, past[i] + n_tree[i]) * tiles(i);
       if (n * n_kv <= most) break;
       r += std::max(unit, r / 16 / unit * unit);
     }
-    p.rows_per_split[w] = r;
   }
   for (size_t i = 0; i < n_seq; i++) {
     if (!n_tree[i]) continue;
-    const size_t rps = p.rows_per_split[width_of(n_tree[i] * group, hd)];
-    const size_t splits = (past[i] + n_tree[i] + rps - 1) / rps;
-    if (splits > 1) p.part_rows += n_tree[i] * n_heads * splits;
+    const size_t parts = p.parts(width(i), past[i] + n_tree[i]);
+    if (parts > 1) p.part_rows += n_tree[i] * n_heads * parts;
   }
   p.floats = p.part_rows * (hd + 2);
   return p;
@@ -974,12 +986,7 @@ void launch_width(const TreeArgs& a, Width w, bool q8, uint32_t items, hipStream
     else
       hipLaunchKernelGGL((tree_narrow_kernel<HDP, 1, false>), grid, nt, 0, s, a);
   } else if (w == kNarrow32) {
-    if constexpr (HDP <= 128) {
-      if (q8)
-        hipLaunchKernelGGL((tree_narrow_kernel<HDP, 2, true>), grid, nt, 0, s, a);
-      else
-        hipLaunchKernelGGL((tree_narrow_kernel<HDP, 2, false>), grid, nt, 0, s, a);
-    }
+    if constexpr (HDP <= 128) hipLaunchKernelGGL((tree_narrow_kernel<HDP, 2, true>), grid, nt, 0, s, a);
   } else {
     if (q8)
       hipLaunchKernelGGL((tree_wide_kernel<HDP, true>), grid, nt, 0, s, a);
@@ -992,13 +999,14 @@ void launch_width(const TreeArgs& a, Width w, bool q8, uint32_t items, hipStream
 
 size_t attention_tree_floats(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads,
                              size_t n_kv_heads, size_t head_dim) {
-  return make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim).floats;
+  return std::max(make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim, false).floats,
+                  make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim, true).floats);
 }
 
 int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const size_t* past, const size_t* n_tree,
                           size_t n_seq, const uint64_t* mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
                           float* out, float* workspace, hipStream_t s) {
-  const Plan plan = make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim);
+  const Plan plan = make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim, q8);
   TreeArgs a{};
   a.q = q;
   a.mask = mask;
@@ -1017,6 +1025,7 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
   j.hd = a.hd;
   size_t part0 = 0;
   for (int w = 0; w < kWidths; w++) {
+    a.whole = static_cast<uint32_t>(plan.whole[w]);
     a.rows_per_split = static_cast<uint32_t>(std::min<size_t>(plan.rows_per_split[w], 0x7fffffff));
     size_t tok0 = 0, items = 0, most_splits = 0;
     auto flush = [&]() -> int {
@@ -1048,8 +1057,8 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
     for (size_t i = 0; i < n_seq; tok0 += n_tree[i], i++) {
       if (!n_tree[i]) continue;
       const size_t rows = n_tree[i] * a.group;
-      if (width_of(rows, head_dim) != w) continue;
-      const size_t splits = (past[i] + n_tree[i] + plan.rows_per_split[w] - 1) / plan.rows_per_split[w];
+      if (width_of(rows, head_dim, q8) != w) continue;
+      const size_t splits = plan.parts(w, past[i] + n_tree[i]);
       if (a.n_seq == kTableSeqs)
         if (int rc = flush()) return rc;
       const uint32_t e = a.n_seq++;
