@@ -921,6 +921,7 @@ Width width_of(size_t rows, size_t hd, bool q8) {
 }
 
 struct Plan {
+  Width as[kWidths];               // the kernel that a width's sequences run on in this call
   size_t whole[kWidths];           // caches of up to this many rows are one part
   size_t rows_per_split[kWidths];  // of longer ones
   size_t part_rows;
@@ -946,14 +947,32 @@ size_t resident(Width w, size_t hd) {
 // with 128 and 19.7 with 256. Joining parts costs about 3 us, and a narrow round
 // 1.9, so two rounds are one part (one token over 511 rows: 8.9 us; three, where
 // other sequences of the call have parts: 15.4 against 11.0).
+//
+// A kernel's launch and its joining cost a call that has sequences of several
+// widths about 8 us each, so few cache rows of a smaller width go along on the
+// wider kernel, where reading them, with most of it idle, costs less than that:
+// up to 2^26 values of an f16 cache, 2^24 of an 8-bit one (trees of 4 to 8
+// tokens in four sequences, 12/4 x 128: caches of up to 4000 25.4 us on two
+// kernels and 15.3 on one, 8-bit 28.3 and 16.5; 16 single tokens over up to
+// 20000 8-bit rows 43 us narrow and 74 wide).
 Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd, bool q8) {
   const size_t group = n_heads / n_kv;
-  auto width = [&](size_t i) { return width_of(n_tree[i] * group, hd, q8); };
+  Plan p{};
+  size_t rows[kWidths] = {};  // cache rows of each width
+  for (size_t i = 0; i < n_seq; i++)
+    if (n_tree[i]) rows[width_of(n_tree[i] * group, hd, q8)] += past[i] + n_tree[i];
+  const size_t few = (q8 ? size_t{1} << 24 : size_t{1} << 26) / (n_kv * hd);
+  int wider = -1;
+  for (int w = kWide; w >= 0; w--) {
+    if (!rows[w]) continue;
+    wider = wider >= 0 && rows[w] <= few ? wider : w;
+    p.as[w] = static_cast<Width>(wider);
+  }
+  auto width = [&](size_t i) { return p.as[width_of(n_tree[i] * group, hd, q8)]; };
   auto tiles = [&](size_t i) { return width(i) == kWide ? (n_tree[i] * group + kWideRows - 1) / kWideRows : 1; };
   size_t work[kWidths] = {};  // cache rows times row tiles
   for (size_t i = 0; i < n_seq; i++)
     if (n_tree[i]) work[width(i)] += (past[i] + n_tree[i]) * tiles(i);
-  Plan p{};
   for (int w = 0; w < kWidths; w++) {
     const size_t round = 32 * narrow_waves(static_cast<int>(hd)), most = resident(static_cast<Width>(w), hd);
     const size_t unit = w == kWide ? 64 : round, least = w == kWide ? 128 : round;
@@ -1057,7 +1076,7 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
     for (size_t i = 0; i < n_seq; tok0 += n_tree[i], i++) {
       if (!n_tree[i]) continue;
       const size_t rows = n_tree[i] * a.group;
-      if (width_of(rows, head_dim, q8) != w) continue;
+      if (plan.as[width_of(rows, head_dim, q8)] != w) continue;
       const size_t splits = plan.parts(w, past[i] + n_tree[i]);
       if (a.n_seq == kTableSeqs)
         if (int rc = flush()) return rc;
