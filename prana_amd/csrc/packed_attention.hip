@@ -18,7 +18,16 @@
 // passes it by more than 2^8, so probabilities are at most 256.
 //
 // f32 form: q * log2(e)/sqrt(w), normalised per row by a power of two, and the
-// probabilities go in as two halves each (22 bits), twice the products.
+// probabilities go in as two halves each (22 bits), twice the products. The
+// f16 form rounds a probability to a half (2^-11), as its result is.
+//
+// Measured: two prompts of up to 8191, 32/8 x 128, f16: 800 us, 898 TFLOP/s (a
+// library's f16 product reaches 1155; both run at 1.5 to 1.7 GHz); matrix cores
+// busy 45 % and vector ALU 41 % of the cycles, seldom both. Nine of up to 1501,
+// 14/2 x 64, f32: 51.5 us, 316 TFLOP/s, twice that with both halves' products.
+// Computing scores a tile ahead (1044 us instead of 806) and groups of waves that
+// take products and softmax in turn (904 instead of 827) cost more registers and
+// barriers than they hide.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -314,7 +323,10 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
 // (16x16x32 products, twice the LDS reads per product) and four waves 64;
 // tiles of 32 keys. Such heads often share one KV head, and 64 rows of it are
 // few workgroups that walk long prompts alone, so each has two such groups of
-// waves, which take the tiles in turn and join their sums at the end.
+// waves, which take the tiles in turn and join their sums at the end. Four
+// prompts of up to 1025, 8/1 x 256, f16: 37.3 us, 279 TFLOP/s (32-row waves 59,
+// one group of 16-row waves 48); bound by LDS, from which a wave reads every
+// operand for 16 rows only.
 constexpr int kWideRows = 64, kWideBN = 32, kWideGroups = 2;
 
 template <int HDP>

@@ -24,6 +24,17 @@
 // registers are, as halves, the operand of O^T += V^T P^T; V comes out of LDS
 // transposed to match. The kept maximum lags the scores by up to 2^8 before
 // the sums are rescaled.
+//
+// Measured, 32/8 heads x 128. Narrow: one token in each of 8 sequences over up
+// to 32767 8-bit rows 98 us, 4.0 TB/s of cache (a bare loop over such 128-byte
+// pieces of rows reads 5.4); the vector ALU is busy 46 % of the time, half of
+// that with turning i8 into halves, the matrix cores 16 %. Twelve waves instead
+// of eight spill (110 us); 16-byte loads of i8 gain 0.5 %. Wide: trees of up to
+// 64 in 8 sequences over up to 16385 f16 rows 196 us, 378 TFLOP/s, twice that
+// with both halves' products (a library's f16 product reaches 1155), 11 of it
+// joining; matrix cores busy 42 %, vector ALU 29 %, the rest waits for LDS and
+// at barriers. Short calls are launches and trips to memory one after another:
+// one token over 511 rows 9 us, four trees of 13 over up to 4099 rows 12.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -164,8 +175,8 @@ struct ScaleTop {
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // ------------------------------------------------------------ narrow: up to 16 RB rows
-// Waves of a workgroup: eight, or four of heads that take more than half of a
-// unit's registers.
+// Waves of a workgroup: eight, or four of heads whose rows take more than half
+// of a unit's registers (one wave of such heads runs on a unit).
 constexpr int narrow_waves(int hdp) { return hdp <= 128 ? 8 : 4; }
 
 template <int HDP>
@@ -826,7 +837,9 @@ struct JoinArgs {
 // A row: M = max m_s, out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), by
 // T lanes (a wave, or a workgroup where a row has many parts). A part's row is
 // read by LANES lanes, 16 bytes each, T / LANES parts at a time; kBatch loads
-// of a lane are in flight together, the first ones before M is known.
+// of a lane are in flight together, the first ones before M is known. (Parts of
+// 20000 rows, one token, 12/4 x 128: a wave a row 16.5 us for the whole call, a
+// workgroup 14.9; up to 16 parts the two take the same.)
 template <int T, int LANES>
 __global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
   constexpr int kBatch = 8, kPG = T / LANES, kWaves = T / 64;
