@@ -63,15 +63,6 @@ __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(kProduct, 2 * M, 0);
 }
 
-// Accumulators wider than the 256 directly addressed registers leave room for:
-// keeps one in the accumulation registers here, where the products use it in
-// place. (Without this the compiler moves all of them there and back around
-// every tile, because the rare rescaling needs them in ordinary ones.)
-template <bool ACC>
-__device__ __forceinline__ void keep_accumulator(f32x16& x) {
-  if constexpr (ACC) asm("" : "+a"(x));
-}
-
 // 2^x as the hardware computes it (1 ulp; results under 2^-126 are 0).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

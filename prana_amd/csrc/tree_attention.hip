@@ -577,6 +577,10 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
   __shared__ __attribute__((aligned(16))) uint16_t s_v[BN * S::kLdV];
   __shared__ __attribute__((aligned(16))) float s_scale[2][64];
+  // The smaller halves of q, in LDS where the registers would spill (6 trees of
+  // 48 over up to 9000 f16 rows, 24/6 x 256: 212 us in registers, 140 in LDS).
+  constexpr bool kLowInLds = HDP > 192;
+  __shared__ __attribute__((aligned(16))) half8 s_ql[kLowInLds ? S::kStepsQK * kTrNT : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = lane & 31, h = lane >> 5;
   const uint32_t kvh = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
@@ -623,6 +627,10 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   fetch(kbeg);
   half8 qh[S::kStepsQK], ql[S::kStepsQK];
   const float c = q.halves(a.scale, h * 8, hd, qh, ql);
+  if constexpr (kLowInLds) {
+#pragma unroll
+    for (int t = 0; t < S::kStepsQK; t++) s_ql[t * kTrNT + tid] = ql[t];
+  }
   f32x16 o[S::kDimBlocks];
 #pragma unroll
   for (int mb = 0; mb < S::kDimBlocks; mb++)
@@ -632,8 +640,6 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   ScaleTop top;
 
   for (uint32_t k0 = kbeg; k0 < kend; k0 += BN) {
-#pragma unroll
-    for (int mb = 0; mb < S::kDimBlocks; mb++) keep_accumulator<(HDP > 128)>(o[mb]);
     const bool edge = k0 + BN > min(sq.past, kend);
     bool odd = false;  // (as in the narrow kernel)
     if (edge) {
@@ -679,9 +685,10 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
       for (int b = 0; b < S::kKeyBlocks; b++) {
         const half8 kf = *reinterpret_cast<const half8*>(s_k + (b * 32 + n) * S::kLdK + t * 16 + h * 8);
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[t], s[b], 0, 0, 0);
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[t], s[b], 0, 0, 0);
+        const half8 low = kLowInLds ? s_ql[t * kTrNT + tid] : ql[t];
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, low, s[b], 0, 0, 0);
       }
-    reads_ahead<S::kStepsQK * S::kKeyBlocks, 2>();
+    if constexpr (!kLowInLds) reads_ahead<S::kStepsQK * S::kKeyBlocks, 2>();
     if constexpr (Q8) {
       float v = lane < BN ? s_scale[1][lane] : 0.0f;
       if (!finite(v)) v = 0.0f;
@@ -732,8 +739,6 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
 #pragma unroll
         for (int j = 0; j < 16; j++) o[mb][j] *= al;
     }
-#pragma unroll
-    for (int mb = 0; mb < S::kDimBlocks; mb++) keep_accumulator<(HDP > 128)>(o[mb]);
     const float ms = (m == -INFINITY ? 0.0f : m - kPShift) + (Q8 ? top.e : 0.0f);
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
