@@ -7,7 +7,8 @@
 // pairs, so the heads that share a KV head share its tiles too; a workgroup
 // takes 128 rows (32 per wave) and walks the keys up to its last token in
 // tiles of 64 or 32, staged through registers into LDS while the tile before is
-// computed. Per tile and wave, with 32x32x16 products:
+// computed; where few rows leave the walk over the keys as the bound, groups of
+// waves take a workgroup's tiles in turn. Per tile and wave, with 32x32x16 products:
 //   S^T = K Q^T : a lane holds one row's scores, 16 of each 32 keys, so the
 //                 maximum and sum of a row are taken inside two lanes;
 //   O^T += V^T P^T : the scores' registers are, as halves, the operand of
@@ -41,8 +42,6 @@ namespace prana {
 
 namespace {
 
-constexpr int kPkNT = 256;     // lanes of a workgroup
-constexpr int kPkRows = 128;   // rows of a workgroup
 constexpr float kLag = 8.0f;   // how far (log2) scores may pass the kept maximum
 constexpr float kPShift = 7.0f;  // probabilities are kept times 2^7 (at most 2^15), so that a half (the smaller
                                  // half of two) resolves 2^-32 of the largest
@@ -60,7 +59,7 @@ struct PackedArgs {
 };
 
 // HDP: head width rounded up; the lanes past the real one hold zeros.
-template <int HDP, int BN>
+template <int HDP, int BN, int NT>
 struct PkShape {
   static constexpr int kStepsQK = HDP / 16, kDimBlocks = HDP / 32, kKeyBlocks = BN / 32;
   static constexpr int kChunks = HDP / 8;  // 16-byte pieces of a row
@@ -69,7 +68,9 @@ struct PkShape {
   // 64-byte pieces of 4 rows that a transposing read takes.
   static constexpr int kLdK = HDP + 8;
   static constexpr int kLdV = HDP % 128 == 96 ? HDP : HDP + 32;
-  static constexpr int kLoads = BN * kChunks / kPkNT;  // 16-byte pieces a lane stages of K (and of V)
+  static constexpr int kLoads = BN * kChunks / NT;  // 16-byte pieces a lane stages of K (and of V)
+  static constexpr int kTile = BN * (kLdK + kLdV);  // halves of a tile of K and V
+  static constexpr int kLdO = HDP + 4;              // joining groups of waves: floats per row
 };
 
 // The pieces of K and V rows k0 .. k0+BN-1 (of len) that a lane stages.
@@ -78,10 +79,10 @@ struct PkShape {
 // would take two registers a piece and as many additions). Pieces past the
 // head's width repeat its last one (q is 0 there for K, and V columns there
 // are never stored).
-template <int BN, int CHUNKS>
+template <int BN, int CHUNKS, int NT>
 struct TileFetch {
-  static constexpr int kLoads = BN * CHUNKS / kPkNT;
-  static constexpr bool kEven = kPkNT % CHUNKS == 0;  // a workgroup's pieces are whole rows
+  static constexpr int kLoads = BN * CHUNKS / NT;
+  static constexpr bool kEven = NT % CHUNKS == 0;  // a group's pieces are whole rows
   const unsigned char *kb, *vb;
   size_t ld;  // bytes
   uint32_t len, hd, tid;
@@ -93,7 +94,7 @@ struct TileFetch {
       : kb(reinterpret_cast<const unsigned char*>(k)), vb(reinterpret_cast<const unsigned char*>(v)), ld(ld_ * 2),
         len(len_), hd(hd_), tid(tid_) {
 #pragma unroll
-    for (int i = 0; i < (kEven ? 1 : kLoads); i++) off[i] = offset(i * kPkNT + tid, BN);
+    for (int i = 0; i < (kEven ? 1 : kLoads); i++) off[i] = offset(i * NT + tid, BN);
   }
   __device__ __forceinline__ void operator()(uint32_t k0, u32x4* kr, u32x4* vr) const {
     const unsigned char* kp = kb + k0 * ld;
@@ -102,7 +103,7 @@ struct TileFetch {
     if (k0 + BN <= len) {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
-        const size_t up = kEven ? i * (kPkNT / CHUNKS) * ld : 0;
+        const size_t up = kEven ? i * (NT / CHUNKS) * ld : 0;
         kr[i] = load_at<u32x4>(kp + up, off[kEven ? 0 : i]);
         vr[i] = load_at<u32x4>(vp + up, off[kEven ? 0 : i]);
       }
@@ -110,7 +111,7 @@ struct TileFetch {
       const uint32_t last = len - 1 - k0;
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
-        const uint32_t e = i * kPkNT + tid, at = offset(e, last);
+        const uint32_t e = i * NT + tid, at = offset(e, last);
         kr[i] = load_at<u32x4>(kp, at);
         vr[i] = u32x4{0, 0, 0, 0};
         if (e / CHUNKS <= last) vr[i] = load_at<u32x4>(vp, at);
@@ -124,9 +125,9 @@ struct TileFetch {
 // that is not finite must not meet that row's zero probability: such values
 // stay out of the tile, and true is returned, for them to be added to the rows
 // that see them.
-template <int BN, int CHUNKS, int LD_K, int LD_V>
+template <int BN, int CHUNKS, int NT, int LD_K, int LD_V>
 __device__ __forceinline__ bool stage_tile(uint16_t* s_k, uint16_t* s_v, u32x4* kr, u32x4* vr, int tid, bool edge) {
-  constexpr int kLoads = BN * CHUNKS / kPkNT;
+  constexpr int kLoads = BN * CHUNKS / NT;
   bool odd = false;
   if (edge) {
     uint32_t bits = 0;
@@ -142,7 +143,7 @@ __device__ __forceinline__ bool stage_tile(uint16_t* s_k, uint16_t* s_v, u32x4* 
   }
 #pragma unroll
   for (int i = 0; i < kLoads; i++) {
-    const int e = i * kPkNT + tid;
+    const int e = i * NT + tid;
     const int r = e / CHUNKS, d = (e % CHUNKS) * 8;
     *reinterpret_cast<u32x4*>(s_k + r * LD_K + d) = kr[i];
     *reinterpret_cast<u32x4*>(s_v + r * LD_V + d) = vr[i];
@@ -166,30 +167,39 @@ __device__ __forceinline__ void store4(void* out, size_t at, float a, float b, f
 
 // Keys of a tile: 64, or 32 in the f32 form of heads wider than 96, which 64
 // would make spill (5 prompts up to 700 and 3000, 32/8 x 128: 44 and 663 us with
-// 64, 37 and 641 with 32).
-constexpr int packed_keys(int hdp, bool half) { return half || hdp <= 96 ? 64 : 32; }
+// 64, 37 and 641 with 32), and where two waves stage a tile of heads wider
+// than 64.
+constexpr int packed_keys(int hdp, bool half, int waves) {
+  return hdp <= 64 || (waves == 4 && (half || hdp <= 96)) ? 64 : 32;
+}
 
-template <int HDP, bool HALF>
-__global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(PackedArgs a) {
-  constexpr int BN = packed_keys(HDP, HALF);
-  using S = PkShape<HDP, BN>;
-  static_assert(BN * S::kChunks % kPkNT == 0, "a tile is a whole number of pieces per lane");
-  __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[BN * S::kLdV];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// WAVES waves take 32 rows each and share tiles; GROUPS such groups of a
+// workgroup take the tiles in turn and join their sums at the end.
+template <int HDP, bool HALF, int WAVES, int GROUPS>
+__global__ __launch_bounds__(64 * WAVES * GROUPS, GROUPS == 1 && HDP <= 64 ? 3 : 2) void packed_kernel(PackedArgs a) {
+  constexpr int NT = 64 * WAVES, BN = packed_keys(HDP, HALF, WAVES), kRows = 32 * WAVES;
+  using S = PkShape<HDP, BN, NT>;
+  static_assert(BN * S::kChunks % NT == 0, "a tile is a whole number of pieces per lane");
+  constexpr int kTiles = GROUPS * S::kTile, kSums = (GROUPS - 1) * kRows * S::kLdO * 2;  // halves
+  __shared__ __attribute__((aligned(16))) uint16_t s_tiles[kTiles > kSums ? kTiles : kSums];
+  __shared__ float s_ml[GROUPS][2][kRows];
+  const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const int tid = threadIdx.x % NT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  uint16_t* const s_k = s_tiles + group * S::kTile;
+  uint16_t* const s_v = s_k + BN * S::kLdK;
   const int n = lane & 31, h = lane >> 5;
   const uint32_t kvh = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv;
   const int sq = table_find(a.tile0, a.n_seq, tile);
   const uint32_t len = table_at(a.len, sq), rows = len * a.group;
-  const uint32_t n_tiles = (rows + kPkRows - 1) / kPkRows;
+  const uint32_t n_tiles = (rows + kRows - 1) / kRows;
   // the last tiles see the most keys: they go first
-  const uint32_t row0 = (n_tiles - 1 - (tile - table_at(a.tile0, sq))) * kPkRows;
+  const uint32_t row0 = (n_tiles - 1 - (tile - table_at(a.tile0, sq))) * kRows;
   const size_t base = table_at(a.start, sq);
   const uint32_t row_w = row0 + wave * 32;                       // the wave's first row
   const uint32_t row = min(row_w + n, rows - 1);                 // (rows past the end repeat the last one)
   const uint32_t tok = row / a.group, head = kvh * a.group + row % a.group;
   const uint32_t tok_first_wg = row0 / a.group;
-  const uint32_t tok_last_wg = (min(row0 + kPkRows, rows) - 1) / a.group;
+  const uint32_t tok_last_wg = (min(row0 + kRows, rows) - 1) / a.group;
   const uint32_t tok_first = min(row_w, rows - 1) / a.group;      // of the wave
   const uint32_t tok_last = min(row_w + 31, rows - 1) / a.group;
   const uint32_t hd = a.hd;
@@ -199,8 +209,8 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
   const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   u32x4 kr[S::kLoads], vr[S::kLoads];
-  const TileFetch<BN, S::kChunks> fetch(kb, vb, a.ld_kv, len, hd, tid);
-  fetch(0, kr, vr);
+  const TileFetch<BN, S::kChunks, NT> fetch(kb, vb, a.ld_kv, len, hd, tid);
+  if (group * BN <= tok_last_wg) fetch(group * BN, kr, vr);
   half8 qh[S::kStepsQK], ql[HALF ? 1 : S::kStepsQK];
   const float c = q.halves(a.scale, h * 8, hd, qh, ql);
 
@@ -211,10 +221,12 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
     for (int i = 0; i < 16; i++) o[mb][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;  // kept maximum (log2 units) and this lane's share of the sum
 
-  for (uint32_t k0 = 0; k0 <= tok_last_wg; k0 += BN) {
-    const bool odd =
-        stage_tile<BN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, tid, k0 + BN - 1 > tok_first_wg);
-    if (k0 + BN <= tok_last_wg) fetch(k0 + BN, kr, vr);
+  constexpr uint32_t kRound = GROUPS * BN;
+  for (uint32_t r0 = 0; r0 <= tok_last_wg; r0 += kRound) {
+    const uint32_t k0 = r0 + group * BN;
+    const bool odd = stage_tile<BN, S::kChunks, NT, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, tid,
+                                                                      r0 + kRound - 1 > tok_first_wg);
+    if (k0 + kRound <= tok_last_wg) fetch(k0 + kRound, kr, vr);
     if (k0 > tok_last) continue;  // (the wave's rows see nothing of this tile)
     f32x16 s[S::kKeyBlocks];
 #pragma unroll
@@ -304,6 +316,54 @@ __global__ __launch_bounds__(kPkNT, HDP <= 64 ? 3 : 2) void packed_kernel(Packed
     }
   }
   l += __shfl_xor(l, 32, 64);
+  if constexpr (GROUPS > 1) {
+    // the other groups leave their sums in LDS, for the first to join
+    const int row_wg = wave * 32 + n;
+    __syncthreads();
+    if (h == 0) {
+      s_ml[group][0][row_wg] = m;
+      s_ml[group][1][row_wg] = l;
+    }
+    float* const s_o = reinterpret_cast<float*>(s_tiles) + row_wg * S::kLdO + 4 * h;
+    if (group > 0) {
+#pragma unroll
+      for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+          *reinterpret_cast<float4*>(s_o + (group - 1) * kRows * S::kLdO + mb * 32 + 8 * g) =
+              make_float4(o[mb][4 * g], o[mb][4 * g + 1], o[mb][4 * g + 2], o[mb][4 * g + 3]);
+    }
+    __syncthreads();
+    if (group > 0) return;
+    // Every row sees the first key, so the first group's maximum is a number (or
+    // the row's scores are not). In another group a row's is one from its first
+    // tile on: a tile's tokens are whole blocks of rows, so a wave's rows see its
+    // first key together.
+    const float mine = m;
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) m = fmaxf(m, s_ml[i][0][row_wg]);
+    const float f0 = exp2_hw(mine - m);
+    l *= f0;
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[mb][i] *= f0;
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) {
+      const float f = exp2_hw(s_ml[i][0][row_wg] - m);
+      l = fmaf(s_ml[i][1][row_wg], f, l);
+#pragma unroll
+      for (int mb = 0; mb < S::kDimBlocks; mb++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const float4 x = *reinterpret_cast<const float4*>(s_o + (i - 1) * kRows * S::kLdO + mb * 32 + 8 * g);
+          o[mb][4 * g] = fmaf(x.x, f, o[mb][4 * g]);
+          o[mb][4 * g + 1] = fmaf(x.y, f, o[mb][4 * g + 1]);
+          o[mb][4 * g + 2] = fmaf(x.z, f, o[mb][4 * g + 2]);
+          o[mb][4 * g + 3] = fmaf(x.w, f, o[mb][4 * g + 3]);
+        }
+    }
+  }
   if (row_w + n >= rows) return;
   const float inv = 1.0f / l;
 #pragma unroll
@@ -331,37 +391,39 @@ constexpr int kWideRows = 64, kWideBN = 32, kWideGroups = 2;
 
 template <int HDP>
 struct PkWideShape {
+  static constexpr int kNT = 4 * kWideRows;  // lanes of a group
   static constexpr int kSteps = HDP / 32, kDimBlocks = HDP / 16, kChunks = HDP / 8;
   static constexpr int kLdK = HDP + 8;
   static constexpr int kLdV = HDP + 16;  // 32-byte pieces of 8 rows on different banks
-  static constexpr int kLoads = kWideBN * kChunks / kPkNT;
+  static constexpr int kLoads = kWideBN * kChunks / kNT;
   static constexpr int kTile = kWideBN * (kLdK + kLdV);  // halves of a group's K and V
   static constexpr int kLdO = HDP + 4;                   // joining the groups: floats per row
-  static_assert(kWideRows * kLdO * 4 <= kWideGroups * kTile * 2, "a group's sums fit the tiles");
+  static_assert((kWideGroups - 1) * kWideRows * kLdO * 4 <= kWideGroups * kTile * 2, "the groups' sums fit the tiles");
 };
 
 template <int HDP, bool HALF>
-__global__ __launch_bounds__(kWideGroups* kPkNT, 2) void packed_wide_kernel(PackedArgs a) {
+__global__ __launch_bounds__(kWideGroups * 4 * kWideRows, 2) void packed_wide_kernel(PackedArgs a) {
   using S = PkWideShape<HDP>;
-  static_assert(kWideBN * S::kChunks % kPkNT == 0, "a tile is a whole number of pieces per lane");
-  __shared__ __attribute__((aligned(16))) uint16_t s_tiles[kWideGroups * S::kTile];
-  __shared__ float s_ml[2][kWideRows];
-  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kPkNT);
-  const int tid = threadIdx.x % kPkNT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int NT = S::kNT, kRows = kWideRows, GROUPS = kWideGroups;
+  static_assert(kWideBN * S::kChunks % NT == 0, "a tile is a whole number of pieces per lane");
+  __shared__ __attribute__((aligned(16))) uint16_t s_tiles[GROUPS * S::kTile];
+  __shared__ float s_ml[GROUPS][2][kRows];
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  const int tid = threadIdx.x % NT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint16_t* const s_k = s_tiles + group * S::kTile;
   uint16_t* const s_v = s_k + kWideBN * S::kLdK;
   const int n = lane & 15, g = lane >> 4;
   const uint32_t kvh = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv;
   const int sq = table_find(a.tile0, a.n_seq, tile);
   const uint32_t len = table_at(a.len, sq), rows = len * a.group;
-  const uint32_t n_tiles = (rows + kWideRows - 1) / kWideRows;
-  const uint32_t row0 = (n_tiles - 1 - (tile - table_at(a.tile0, sq))) * kWideRows;
+  const uint32_t n_tiles = (rows + kRows - 1) / kRows;
+  const uint32_t row0 = (n_tiles - 1 - (tile - table_at(a.tile0, sq))) * kRows;
   const size_t base = table_at(a.start, sq);
   const uint32_t row_w = row0 + wave * 16;
   const uint32_t row = min(row_w + n, rows - 1);
   const uint32_t tok = row / a.group, head = kvh * a.group + row % a.group;
   const uint32_t tok_first_wg = row0 / a.group;
-  const uint32_t tok_last_wg = (min(row0 + kWideRows, rows) - 1) / a.group;
+  const uint32_t tok_last_wg = (min(row0 + kRows, rows) - 1) / a.group;
   const uint32_t tok_first = min(row_w, rows - 1) / a.group;
   const uint32_t tok_last = min(row_w + 15, rows - 1) / a.group;
   const uint32_t hd = a.hd;
@@ -371,7 +433,7 @@ __global__ __launch_bounds__(kWideGroups* kPkNT, 2) void packed_wide_kernel(Pack
   const uint16_t* kb = a.k + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   const uint16_t* vb = a.v + base * a.ld_kv + static_cast<size_t>(kvh) * hd;
   u32x4 kr[S::kLoads], vr[S::kLoads];
-  const TileFetch<kWideBN, S::kChunks> fetch(kb, vb, a.ld_kv, len, hd, tid);
+  const TileFetch<kWideBN, S::kChunks, NT> fetch(kb, vb, a.ld_kv, len, hd, tid);
   if (group * kWideBN <= tok_last_wg) fetch(group * kWideBN, kr, vr);
   half8 qh[S::kSteps], ql[HALF ? 1 : S::kSteps];
   const float c = q.halves(a.scale, g * 8, hd, qh, ql);
@@ -383,11 +445,11 @@ __global__ __launch_bounds__(kWideGroups* kPkNT, 2) void packed_wide_kernel(Pack
     for (int i = 0; i < 4; i++) o[mb][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  constexpr uint32_t kRound = kWideGroups * kWideBN;
+  constexpr uint32_t kRound = GROUPS * kWideBN;
   for (uint32_t r0 = 0; r0 <= tok_last_wg; r0 += kRound) {
     const uint32_t k0 = r0 + group * kWideBN;
-    const bool odd = stage_tile<kWideBN, S::kChunks, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, tid,
-                                                                       r0 + kRound - 1 > tok_first_wg);
+    const bool odd = stage_tile<kWideBN, S::kChunks, NT, S::kLdK, S::kLdV>(s_k, s_v, kr, vr, tid,
+                                                                           r0 + kRound - 1 > tok_first_wg);
     if (k0 + kRound <= tok_last_wg) fetch(k0 + kRound, kr, vr);
     if (k0 > tok_last) continue;  // (the wave's rows see nothing of this tile)
 
@@ -480,50 +542,100 @@ __global__ __launch_bounds__(kWideGroups* kPkNT, 2) void packed_wide_kernel(Pack
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  // join the groups: the second leaves its sums in LDS
-  float* const s_o = reinterpret_cast<float*>(s_tiles) + (wave * 16 + n) * S::kLdO;
+  // the other groups leave their sums in LDS, for the first to join
+  const int row_wg = wave * 16 + n;
+  float* const s_o = reinterpret_cast<float*>(s_tiles) + row_wg * S::kLdO + 4 * g;
   __syncthreads();
-  if (group == 1) {
-    if (g == 0) {
-      s_ml[0][wave * 16 + n] = m;
-      s_ml[1][wave * 16 + n] = l;
-    }
+  if (g == 0) {
+    s_ml[group][0][row_wg] = m;
+    s_ml[group][1][row_wg] = l;
+  }
+  if (group > 0) {
 #pragma unroll
     for (int mb = 0; mb < S::kDimBlocks; mb++)
-      *reinterpret_cast<f32x4*>(s_o + mb * 16 + 4 * g) = o[mb];
+      *reinterpret_cast<f32x4*>(s_o + (group - 1) * kRows * S::kLdO + mb * 16) = o[mb];
   }
   __syncthreads();
-  if (group == 1 || row_w + n >= rows) return;
-  // (Every row sees the first key, so the first group's maximum is a number. A
-  // row's maximum in the second is one from its first tile on: 32 tokens are
-  // whole blocks of 16 rows, so a wave's rows see a tile's first key together.)
-  const float m2 = s_ml[0][wave * 16 + n], l2 = s_ml[1][wave * 16 + n], top = fmaxf(m, m2);
-  const float f1 = exp2_hw(m - top), f2 = exp2_hw(m2 - top);
-  const float inv = 1.0f / fmaf(l, f1, l2 * f2);
+  if (group > 0 || row_w + n >= rows) return;
+  // (the maxima are numbers as in the kernel above)
+  const float mine = m;
+#pragma unroll
+  for (int i = 1; i < GROUPS; i++) m = fmaxf(m, s_ml[i][0][row_wg]);
+  const float f0 = exp2_hw(mine - m);
+  l *= f0;
+#pragma unroll
+  for (int mb = 0; mb < S::kDimBlocks; mb++) o[mb] *= f0;
+#pragma unroll
+  for (int i = 1; i < GROUPS; i++) {
+    const float f = exp2_hw(s_ml[i][0][row_wg] - m);
+    l = fmaf(s_ml[i][1][row_wg], f, l);
+#pragma unroll
+    for (int mb = 0; mb < S::kDimBlocks; mb++)
+      o[mb] += *reinterpret_cast<const f32x4*>(s_o + (i - 1) * kRows * S::kLdO + mb * 16) * f;
+  }
+  const float inv = 1.0f / l;
 #pragma unroll
   for (int mb = 0; mb < S::kDimBlocks; mb++) {
     const uint32_t d = mb * 16 + 4 * g;
     if (d < hd) {
-      const f32x4 y = (o[mb] * f1 + *reinterpret_cast<const f32x4*>(s_o + d) * f2) * inv;
+      const f32x4 y = o[mb] * inv;
       store4<HALF>(a.out, (base + tok) * a.ld_out + static_cast<size_t>(head) * hd + d, y[0], y[1], y[2], y[3]);
     }
   }
 }
 
-template <int HDP>
-void launch_shape(const PackedArgs& a, bool half, uint32_t tiles, hipStream_t s) {
-  const dim3 grid(tiles * a.n_kv), nt(kPkNT);
-  if constexpr (HDP <= 128) {
-    if (half)
-      hipLaunchKernelGGL((packed_kernel<HDP, true>), grid, nt, 0, s, a);
-    else
-      hipLaunchKernelGGL((packed_kernel<HDP, false>), grid, nt, 0, s, a);
-  } else {
-    if (half)
-      hipLaunchKernelGGL((packed_wide_kernel<HDP, true>), grid, dim3(kWideGroups * kPkNT), 0, s, a);
-    else
-      hipLaunchKernelGGL((packed_wide_kernel<HDP, false>), grid, dim3(kWideGroups * kPkNT), 0, s, a);
+struct Seq {
+  size_t start, len;
+};
+
+// Rows of a workgroup.
+size_t tile_rows(size_t head_dim, bool divided) {
+  return head_dim > 128 ? kWideRows : divided && head_dim <= 96 ? 64 : 128;
+}
+
+// Whether workgroups divide the keys among groups of waves: four groups of two
+// waves (64 rows) for heads up to 96 wide, two of four for heads up to 128. That
+// shortens the longest walk over the keys, which bounds a call of few rows, but
+// such a workgroup has a compute unit to itself (and joins its groups, so
+// not for short walks: 300 tokens, 8/2 x 128, 12.4 us whole,
+// 12.8 divided; 6/6 x 48 8.4, 7.7). In units of a tile of 64 keys
+// (1.1 to 1.4 us), the longest walk is len / 64; divided workgroups cost about
+// 3 each and 0.45 (0.8 with two groups) per tile of their walks, on 256 units.
+// One prompt of 1500, 14/2 x 64, f32: 36 us whole, 22 divided; two of up to
+// 3500, 6/6 x 48: 81 and 59; one of 1500, 32/8 x 128: 63 and 52; but eight of up
+// to 600, 14/2 x 64: 20 and 25, and one of 3500, 32/8 x 128: 212 and 217.
+bool divide(const std::vector<Seq>& seqs, size_t group, size_t n_kv, size_t head_dim) {  // seqs: the longest first
+  if (head_dim > 128 || seqs.empty() || seqs[0].len < (head_dim <= 96 ? 256 : 512)) return false;
+  const size_t rows = tile_rows(head_dim, true);
+  const double per_tile = head_dim <= 96 ? 0.45 : 0.8;
+  double cost = 0;
+  for (const Seq& q : seqs) {
+    const double wgs = static_cast<double>((q.len * group + rows - 1) / rows * n_kv);
+    cost += wgs * (3 + per_tile * static_cast<double>(q.len) / 128);  // (half of len on average)
   }
+  return cost / 256 < static_cast<double>(seqs[0].len) / 64;
+}
+
+template <int HDP, bool HALF>
+void launch_shape(const PackedArgs& a, bool divided, uint32_t tiles, hipStream_t s) {
+  const dim3 grid(tiles * a.n_kv);
+  if constexpr (HDP <= 128) {
+    constexpr int kWaves = HDP <= 96 ? 2 : 4;
+    if (divided)
+      hipLaunchKernelGGL((packed_kernel<HDP, HALF, kWaves, 8 / kWaves>), grid, dim3(512), 0, s, a);
+    else
+      hipLaunchKernelGGL((packed_kernel<HDP, HALF, 4, 1>), grid, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((packed_wide_kernel<HDP, HALF>), grid, dim3(512), 0, s, a);
+  }
+}
+
+template <int HDP>
+void launch_type(const PackedArgs& a, bool half, bool divided, uint32_t tiles, hipStream_t s) {
+  if (half)
+    launch_shape<HDP, true>(a, divided, tiles, s);
+  else
+    launch_shape<HDP, false>(a, divided, tiles, s);
 }
 
 }  // namespace
@@ -543,9 +655,6 @@ int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v,
   a.group = static_cast<uint32_t>(n_heads / n_kv_heads);
   a.hd = static_cast<uint32_t>(head_dim);
   a.scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_dim)));
-  struct Seq {
-    size_t start, len;
-  };
   std::vector<Seq> seqs;
   size_t at = 0;
   for (size_t i = 0; i < n_seq; i++) {
@@ -554,14 +663,15 @@ int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v,
   }
   // the longest first: a workgroup's work grows with its place in its sequence
   std::stable_sort(seqs.begin(), seqs.end(), [](const Seq& x, const Seq& y) { return x.len > y.len; });
-  const size_t tile_rows = head_dim <= 128 ? kPkRows : kWideRows;
+  const bool divided = divide(seqs, a.group, n_kv_heads, head_dim);
+  const size_t rows = tile_rows(head_dim, divided);
   // Tiles of one grid: its lanes are to fit 32 bits (one sequence's do, by the length check).
   const size_t most = (size_t{1} << 22) / n_kv_heads;
   for (size_t i = 0; i < seqs.size();) {
     size_t tiles = 0;
     a.n_seq = 0;
     while (i < seqs.size() && a.n_seq < kTableSeqs) {
-      const size_t t = (seqs[i].len * a.group + tile_rows - 1) / tile_rows;
+      const size_t t = (seqs[i].len * a.group + rows - 1) / rows;
       if (a.n_seq && tiles + t > most) break;
       a.start[a.n_seq] = static_cast<uint32_t>(seqs[i].start);
       a.len[a.n_seq] = static_cast<uint32_t>(seqs[i].len);
@@ -571,15 +681,15 @@ int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v,
     }
     const uint32_t t = static_cast<uint32_t>(tiles);
     if (head_dim <= 64)
-      launch_shape<64>(a, half, t, s);
+      launch_type<64>(a, half, divided, t, s);
     else if (head_dim <= 96)
-      launch_shape<96>(a, half, t, s);
+      launch_type<96>(a, half, divided, t, s);
     else if (head_dim <= 128)
-      launch_shape<128>(a, half, t, s);
+      launch_type<128>(a, half, divided, t, s);
     else if (head_dim <= 192)
-      launch_shape<192>(a, half, t, s);
+      launch_type<192>(a, half, divided, t, s);
     else
-      launch_shape<256>(a, half, t, s);
+      launch_type<256>(a, half, divided, t, s);
     PRANA_LAUNCH_CHECK();
   }
   return kOk;

@@ -214,6 +214,29 @@ def test_offsets_past_32_bits():
     assert ok, worst
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,w", [(2, 2, 48), (6, 2, 64), (3, 1, 80), (5, 1, 96), (7, 1, 128), (2, 2, 104)])
+def test_few_rows_over_long_prompts(heads, kv_heads, w, half):
+    # the keys of a workgroup divided among groups of waves, some of which see
+    # nothing: prompts that end in the first group's tile, at and past a round's end
+    lens = [700, 3, 0, 257, 64, 65, 129, 1]
+    n = sum(lens)
+    q, k, v = inputs(13, n, heads, kv_heads, w, half)
+    check(q, k, v, lens, heads, kv_heads, w)
+    # values that are not finite stay with the rows that see them: row 600 of the first prompt
+    clean = P.attention_packed(q, k, v, lens, heads, kv_heads, w)
+    v[600, 5], k[690, 7] = np.inf, np.nan  # (KV head 0)
+    q[650, 3] = np.nan  # (head 0)
+    got = P.attention_packed(q, k, v, lens, heads, kv_heads, w)
+    group = heads // kv_heads
+    hit = np.zeros(got.shape, bool)
+    for h in range(group):
+        hit[600:700, h * w + 5] = True
+        hit[690:700, h * w:(h + 1) * w] = True
+    hit[650, :w] = True
+    assert not np.isfinite(got[hit]).any() and np.array_equal(got[~hit], clean[~hit])
+
+
 def test_empty_calls():
     lib = _lib.load()
     P.init()
