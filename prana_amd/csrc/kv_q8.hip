@@ -213,7 +213,8 @@ __global__ __launch_bounds__(kKvNT) void kv_read_kernel(KvArgs a) {
         h[j] = static_cast<uint32_t>(f32_to_f16(y[2 * j])) | static_cast<uint32_t>(f32_to_f16(y[2 * j + 1])) << 16;
       __builtin_nontemporal_store(h, reinterpret_cast<u32x4*>(static_cast<uint16_t*>(dst) + at));
     } else {
-      __builtin_nontemporal_store(f32x4{y[0], y[1], y[2], y[3]}, reinterpret_cast<f32x4*>(static_cast<float*>(dst) + at));
+      const f32x4 f = {y[0], y[1], y[2], y[3]};
+      __builtin_nontemporal_store(f, reinterpret_cast<f32x4*>(static_cast<float*>(dst) + at));
     }
   }
 }

@@ -90,7 +90,8 @@ struct TileFetch {
   __device__ __forceinline__ uint32_t offset(uint32_t e, uint32_t last) const {
     return min(e / CHUNKS, last) * static_cast<uint32_t>(ld) + min(e % CHUNKS * 8, hd - 8) * 2;
   }
-  __device__ __forceinline__ TileFetch(const uint16_t* k, const uint16_t* v, size_t ld_, uint32_t len_, uint32_t hd_, uint32_t tid_)
+  __device__ __forceinline__ TileFetch(const uint16_t* k, const uint16_t* v, size_t ld_, uint32_t len_, uint32_t hd_,
+                                       uint32_t tid_)
       : kb(reinterpret_cast<const unsigned char*>(k)), vb(reinterpret_cast<const unsigned char*>(v)), ld(ld_ * 2),
         len(len_), hd(hd_), tid(tid_) {
 #pragma unroll
@@ -157,7 +158,9 @@ __device__ __forceinline__ void store4(void* out, size_t at, float a, float b, f
   if constexpr (HALF) {
     // A weighted mean of halves is no larger than they are, but the roundings
     // of its weights (2^-11) can carry one at the end of their range past it.
-    auto half = [](float x) { return static_cast<_Float16>(fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x); };
+    auto half = [](float x) {
+      return static_cast<_Float16>(fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x);
+    };
     const half4 y = {half(a), half(b), half(c), half(d)};
     *reinterpret_cast<half4*>(static_cast<uint16_t*>(out) + at) = y;
   } else {

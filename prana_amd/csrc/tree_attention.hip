@@ -194,7 +194,8 @@ struct NarrowShape {
 };
 
 template <int HDP, int RB, bool Q8>
-__global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : HDP <= 128 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * narrow_waves(HDP), HDP <= 64 && RB == 1 ? 4 : HDP <= 128 ? 2 : 1)
+void tree_narrow_kernel(TreeArgs a) {
   using S = NarrowShape<HDP>;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[S::kBytes];
   __shared__ __attribute__((aligned(16))) uint16_t s_q[2][16 * RB * S::kLdQ];  // the halves of q
@@ -848,7 +849,8 @@ struct JoinArgs {
 template <int T, int LANES>
 __global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
   constexpr int kBatch = 8, kPG = T / LANES, kWaves = T / 64;
-  const uint32_t r = blockIdx.x * (256 / T) + __builtin_amdgcn_readfirstlane(threadIdx.x / T), tid = threadIdx.x % T, lane = threadIdx.x & 63;
+  const uint32_t r = blockIdx.x * (256 / T) + __builtin_amdgcn_readfirstlane(threadIdx.x / T);
+  const uint32_t tid = threadIdx.x % T, lane = threadIdx.x & 63;
   if (r >= a.n_rows) return;  // (whole waves; with T = 256 never)
   const int si = table_find(a.row0, a.n_seq, r);
   const uint32_t row = r - table_at(a.row0, si), ns = table_at(a.splits, si);
@@ -973,7 +975,8 @@ size_t resident(Width w, size_t hd) {
 // tokens in four sequences, 12/4 x 128: caches of up to 4000 25.4 us on two
 // kernels and 15.3 on one, 8-bit 28.3 and 16.5; 16 single tokens over up to
 // 20000 8-bit rows 43 us narrow and 74 wide).
-Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd, bool q8) {
+Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd,
+               bool q8) {
   const size_t group = n_heads / n_kv;
   Plan p{};
   size_t rows[kWidths] = {};  // cache rows of each width
