@@ -153,25 +153,34 @@ __device__ __forceinline__ void load_values(const unsigned char* p, float scale,
   }
 }
 
-// V scales of 8-bit caches are taken relative to 2^e, a power of two no smaller
-// than any scale met so far: probabilities are kept times 2^-e (through the
-// exponential's argument, in the sums too), so that one times its scale stays
-// below 2^15 as the probability itself does. A head whose scales pass 2^100
-// loses probabilities under 2^-26 to underflow.
-struct ScaleTop {
-  float e = -60.0f, top = 0x1p-60f;
-  // v: this lane's scales of the tile (0 where they are not finite). The power
-  // of two that what was summed before is to be multiplied with (as an
-  // exponent: it can lie beyond a float's).
-  __device__ __forceinline__ int raise(float v) {
-    const float big = wave_max_f32(fabsf(v));
-    if (!(big > top)) return 0;
-    const int x = min((__float_as_uint(big) >> 23) + 1, 253u), was = static_cast<int>(e);
-    top = __uint_as_float(static_cast<uint32_t>(x) << 23);
-    e = static_cast<float>(x - 127);
-    return was - (x - 127);
-  }
-};
+// V scales of 8-bit caches. A row's reference follows the largest product of a
+// weight and its V scale among the keys that the row itself sees. The largest
+// product then lies between 2^6 and 2^15, where two halves hold 22 bits, whatever
+// scales the keys have that the row does not see or gives no weight. With 2^x
+// above a key's scale, what is compared is score + x (log2 units); the weights
+// and their sum count from the reference. (One power of two for all rows of a
+// wave, over all scales met, took 8 single tokens over up to 32767 rows 3 us less
+// of 98, but a masked row of large scale took the other rows' bits.)
+constexpr float kTop = kLag + kPShift;  // products of weights and scales stay under 2^kTop
+constexpr float kUnseen = -3e38f;       // the reference of a row that has seen nothing
+// x, at least -80: weights stay under 2^(80 + 15), and 2^30 of them under a float's end.
+__device__ __forceinline__ float scale_log2(float v) {
+  return static_cast<float>(max(static_cast<int>(__float_as_uint(v) >> 23 & 255u) - 126, -80));
+}
+// A sum of weights, x powers of two up (x <= 0): in two steps, for references that
+// lie further apart than a float's range. (Weighted sums of values then vanish
+// beside what raised the reference; the weights need not, their scales were small.)
+__device__ __forceinline__ float shift_sum(float l, float x) {
+  const float half = exp2_hw(0.5f * x);
+  return l * half * half;
+}
+// The reference for a largest score + x of mx. Past 2^22 that sum is rounded to
+// halves and more: two steps up keep every product under 2^kTop.
+__device__ __forceinline__ bool coarse(float mx) { return fabsf(mx) >= 0x1p22f; }
+__device__ __forceinline__ float reference(float mx) {
+  const float r = mx - kPShift;
+  return coarse(mx) ? fmaf(fabsf(r), 0x1p-22f, r) : r;
+}
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // ------------------------------------------------------------ narrow: up to 16 RB rows
@@ -201,7 +210,8 @@ void tree_narrow_kernel(TreeArgs a) {
   using S = NarrowShape<HDP>;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[S::kBytes];
   __shared__ __attribute__((aligned(16))) uint16_t s_q[2][16 * RB * S::kLdQ];  // the halves of q
-  __shared__ __attribute__((aligned(16))) float s_scale[S::kWaves][64];  // per wave: K scales of 32 keys, V scales
+  // per wave: K scales of 32 keys, V scales and their scale_log2
+  __shared__ __attribute__((aligned(16))) float s_scale[S::kWaves][96];
   __shared__ float s_c[16 * RB], s_m[S::kWaves][16 * RB], s_l[S::kWaves][16 * RB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -301,7 +311,7 @@ void tree_narrow_kernel(TreeArgs a) {
   for (int r = 0; r < RB; r++) {
     const uint32_t i = min(r * 16u + n, rows - 1) / a.group;
     word[r] = mask_word(a, sq, i);
-    m[r] = -INFINITY;
+    m[r] = Q8 ? kUnseen : -INFINITY;
     l[r] = 0.0f;
 #pragma unroll
     for (int mb = 0; mb < S::kDimBlocks; mb++)
@@ -311,7 +321,6 @@ void tree_narrow_kernel(TreeArgs a) {
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < RB; r++) c[r] = s_c[r * 16 + n];
-  ScaleTop top;
   for (; k0 < kend; k0 += S::kRound) {
     // the next keys follow into the registers as these leave them
     const bool more = k0 + S::kRound < kend;
@@ -349,18 +358,7 @@ void tree_narrow_kernel(TreeArgs a) {
     }
     if constexpr (Q8) {
       s_scale[wave][lane] = sc;
-      const float v = lane < 32 || !finite(sc) ? 0.0f : sc;
-      if (__any(fabsf(v) > top.top)) {
-        const int f = top.raise(v);
-#pragma unroll
-        for (int r = 0; r < RB; r++) {
-          l[r] = ldexpf(l[r], f);
-#pragma unroll
-          for (int mb = 0; mb < S::kDimBlocks; mb++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) o[r][mb][j] = ldexpf(o[r][mb][j], f);
-        }
-      }
+      if (lane >= 32) s_scale[wave][32 + lane] = scale_log2(sc);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -393,14 +391,16 @@ void tree_narrow_kernel(TreeArgs a) {
 #pragma unroll
       for (int b = 0; b < 2; b++) s[r][b] += s2[r][b];
 
-    float ks[2][4], vs[2][4];
+    float ks[2][4], vs[2][4], vx[2][4];
     if constexpr (Q8) {
 #pragma unroll
       for (int b = 0; b < 2; b++) {
         const float4 x = *reinterpret_cast<const float4*>(&s_scale[wave][b * 16 + 4 * g]);
         const float4 y = *reinterpret_cast<const float4*>(&s_scale[wave][32 + b * 16 + 4 * g]);
+        const float4 z = *reinterpret_cast<const float4*>(&s_scale[wave][64 + b * 16 + 4 * g]);
         ks[b][0] = x.x; ks[b][1] = x.y; ks[b][2] = x.z; ks[b][3] = x.w;
         vs[b][0] = y.x; vs[b][1] = y.y; vs[b][2] = y.z; vs[b][3] = y.w;
+        vx[b][0] = z.x; vx[b][1] = z.y; vx[b][2] = z.z; vx[b][3] = z.w;
       }
     }
     half8 ph[RB], pl[RB];
@@ -424,21 +424,43 @@ void tree_narrow_kernel(TreeArgs a) {
           for (int j = 0; j < 4; j++)
             if (!(seen >> (b * 16 + j) & 1)) s[r][b][j] = -INFINITY;
       }
-      float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
-                       fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c[r];
-      if (__any(mx > m[r] + kLag)) {
-        const float mn = fmaxf(m[r], mx);
-        const float al = mn == -INFINITY ? 1.0f : exp2_hw(m[r] - mn);  // (a row that has seen nothing yet)
+      auto rescale = [&](float mn, float al) {
+        l[r] = Q8 ? shift_sum(l[r], m[r] - mn) : l[r] * al;
         m[r] = mn;
-        l[r] *= al;
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
           for (int j = 0; j < 4; j++) o[r][mb][j] *= al;
+      };
+      float ms;
+      if constexpr (Q8) {
+        auto largest = [&](auto of) {  // over the row's keys, of a score and its scale's exponent
+          float x = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) x = fmaxf(x, of(s[r][b][j], vx[b][j]));
+          x = fmaxf(x, __shfl_xor(x, 16, 64));
+          return fmaxf(x, __shfl_xor(x, 32, 64));
+        };
+        const float mx = largest([&](float score, float x) { return fmaf(score, c[r], x); });
+        if (__any(mx - m[r] > kTop || coarse(mx))) {
+          const float past = largest([&](float score, float x) { return fmaf(score, c[r], -m[r]) + x; });
+          const float mn = past > kTop ? reference(mx) : m[r];
+          rescale(mn, exp2_hw(m[r] - mn));
+        }
+        ms = m[r];
+      } else {
+        float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
+                         fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c[r];
+        if (__any(mx > m[r] + kLag)) {
+          const float mn = fmaxf(m[r], mx);
+          rescale(mn, mn == -INFINITY ? 1.0f : exp2_hw(m[r] - mn));  // (a row that has seen nothing yet)
+        }
+        ms = m[r] == -INFINITY ? 0.0f : m[r] - kPShift;
       }
-      const float ms = (m[r] == -INFINITY ? 0.0f : m[r] - kPShift) + (Q8 ? top.e : 0.0f);
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -497,7 +519,6 @@ void tree_narrow_kernel(TreeArgs a) {
   for (int r = 0; r < RB; r++) {
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
-    if constexpr (Q8) l[r] *= top.top;
     if (g == 0) {
       s_m[wave][r * 16 + n] = m[r];
       s_l[wave][r * 16 + n] = l[r];
@@ -512,8 +533,7 @@ void tree_narrow_kernel(TreeArgs a) {
     float M = s_m[0][i];
 #pragma unroll
     for (int w = 1; w < S::kWaves; w++) M = fmaxf(M, s_m[w][i]);
-    float f = m[r] == -INFINITY ? 0.0f : exp2_hw(m[r] - M);
-    if constexpr (Q8) f *= top.top;
+    const float f = m[r] == -INFINITY ? 0.0f : exp2_hw(m[r] - M);
 #pragma unroll
     for (int mb = 0; mb < S::kDimBlocks; mb++) {
       // a wave that saw nothing of this row holds zeros
@@ -535,7 +555,10 @@ void tree_narrow_kernel(TreeArgs a) {
       for (int w = 0; w < S::kWaves; w++) {
         const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 16 + rr) * S::kLdO + d);
         y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
-        if (s_m[w][ri] != -INFINITY) L = fmaf(s_l[w][ri], exp2_hw(s_m[w][ri] - top_m), L);
+        if constexpr (Q8)
+          L += shift_sum(s_l[w][ri], s_m[w][ri] - top_m);
+        else if (s_m[w][ri] != -INFINITY)
+          L = fmaf(s_l[w][ri], exp2_hw(s_m[w][ri] - top_m), L);
       }
       const size_t qrow = static_cast<size_t>(row / a.group) * a.n_heads + kvh * a.group + row % a.group;
       if (sq.splits == 1) {
@@ -579,7 +602,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   static_assert(BN * S::kChunks % kTrNT == 0, "a tile is a whole number of pieces per lane");
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
   __shared__ __attribute__((aligned(16))) uint16_t s_v[BN * S::kLdV];
-  __shared__ __attribute__((aligned(16))) float s_scale[2][64];
+  __shared__ __attribute__((aligned(16))) float s_scale[3][64];  // K scales, V scales, their scale_log2
   // The smaller halves of q, in LDS where the registers would spill (6 trees of
   // 48 over up to 9000 f16 rows, 24/6 x 256: 212 us in registers, 140 in LDS).
   constexpr bool kLowInLds = HDP > 192;
@@ -639,8 +662,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
     for (int j = 0; j < 16; j++) o[mb][j] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  ScaleTop top;
+  float m = Q8 ? kUnseen : -INFINITY, l = 0.0f;
 
   for (uint32_t k0 = kbeg; k0 < kend; k0 += BN) {
     const bool edge = k0 + BN > min(sq.past, kend);
@@ -672,6 +694,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
     }
     if constexpr (Q8) {
       if (tid < 2 * BN) s_scale[tid / BN][tid % BN] = sc;
+      if (tid >= BN && tid < 2 * BN) s_scale[2][tid % BN] = scale_log2(sc);
     }
     __syncthreads();
     if (k0 + BN < kend) fetch(k0 + BN);
@@ -693,16 +716,6 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
       }
     if constexpr (!kLowInLds) reads_ahead<S::kStepsQK * S::kKeyBlocks, 2>();
     if constexpr (Q8) {
-      float v = lane < BN ? s_scale[1][lane] : 0.0f;
-      if (!finite(v)) v = 0.0f;
-      if (__any(fabsf(v) > top.top)) {
-        const int f = top.raise(v);
-        l = ldexpf(l, f);
-#pragma unroll
-        for (int mb = 0; mb < S::kDimBlocks; mb++)
-#pragma unroll
-          for (int j = 0; j < 16; j++) o[mb][j] = ldexpf(o[mb][j], f);
-      }
 #pragma unroll
       for (int b = 0; b < S::kKeyBlocks; b++)
 #pragma unroll
@@ -726,23 +739,49 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
         for (int j = 0; j < 16; j++)
           if (!(seen >> (b * 32 + 8 * (j / 4) + j % 4) & 1)) s[b][j] = -INFINITY;
     }
-    float mx = s[0][0];
-#pragma unroll
-    for (int b = 0; b < S::kKeyBlocks; b++)
-#pragma unroll
-      for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-    if (__any(mx > m + kLag)) {
-      const float mn = fmaxf(m, mx);
-      const float al = mn == -INFINITY ? 1.0f : exp2_hw(m - mn);
+    auto rescale = [&](float mn, float al) {
+      l = Q8 ? shift_sum(l, m - mn) : l * al;
       m = mn;
-      l *= al;
 #pragma unroll
       for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
         for (int j = 0; j < 16; j++) o[mb][j] *= al;
+    };
+    float ms;
+    if constexpr (Q8) {  // (as in the narrow kernel)
+      auto largest = [&](auto of) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const float4 vx = *reinterpret_cast<const float4*>(&s_scale[2][b * 32 + 8 * g + 4 * h]);
+            const float v4[4] = {vx.x, vx.y, vx.z, vx.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) x = fmaxf(x, of(s[b][4 * g + j], v4[j]));
+          }
+        return fmaxf(x, __shfl_xor(x, 32, 64));
+      };
+      const float mx = largest([&](float score, float x) { return fmaf(score, c, x); });
+      if (__any(mx - m > kTop || coarse(mx))) {
+        const float past = largest([&](float score, float x) { return fmaf(score, c, -m) + x; });
+        const float mn = past > kTop ? reference(mx) : m;
+        rescale(mn, exp2_hw(m - mn));
+      }
+      ms = m;
+    } else {
+      float mx = s[0][0];
+#pragma unroll
+      for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+      if (__any(mx > m + kLag)) {
+        const float mn = fmaxf(m, mx);
+        rescale(mn, mn == -INFINITY ? 1.0f : exp2_hw(m - mn));
+      }
+      ms = m == -INFINITY ? 0.0f : m - kPShift;
     }
-    const float ms = (m == -INFINITY ? 0.0f : m - kPShift) + (Q8 ? top.e : 0.0f);
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
 #pragma unroll
@@ -811,12 +850,12 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
     dst = a.out + (static_cast<size_t>(sq.tok0) * a.n_heads + qrow) * hd;
   } else {
     const size_t pr = sq.part0 + qrow * sq.splits + split;
-    f = Q8 ? top.top : 1.0f;
+    f = 1.0f;
     dst = a.part + pr * hd;
     if (h == 0) {
       float* ml = a.part + a.part_rows * hd + pr * 2;
       ml[0] = m;
-      ml[1] = l * f;
+      ml[1] = l;
     }
   }
 #pragma unroll
@@ -836,6 +875,7 @@ struct JoinArgs {
   size_t part_rows;
   float* out;
   uint32_t n_seq, n_rows, hd;
+  bool q8;                     // the parts' references: of an 8-bit cache (shift_sum)
   uint32_t row0[kTableSeqs];  // first (token, head) row of the sequence in this launch
   uint32_t out0[kTableSeqs];  // its first row of out
   uint32_t splits[kTableSeqs];
@@ -878,7 +918,10 @@ __global__ __launch_bounds__(256) void tree_join_kernel(JoinArgs a) {
   float L = 0.0f;
   for (uint32_t s = lane; s < ns; s += 64) {
     const float2 v = ml[s];
-    if (v.x != -INFINITY) L = fmaf(v.y, exp2_hw(v.x - M), L);
+    if (a.q8)
+      L += shift_sum(v.y, v.x - M);
+    else if (v.x != -INFINITY)
+      L = fmaf(v.y, exp2_hw(v.x - M), L);
   }
   for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
   float4 y = make_float4(0, 0, 0, 0);
@@ -1065,6 +1108,7 @@ int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const siz
   j.part_rows = plan.part_rows;
   j.out = out;
   j.hd = a.hd;
+  j.q8 = q8;
   size_t part0 = 0;
   for (int w = 0; w < kWidths; w++) {
     a.whole = static_cast<uint32_t>(plan.whole[w]);
