@@ -250,7 +250,9 @@ int prana_kv_read_q8(const prana_kv *kv, const size_t *first_rows, const size_t 
  * NaN too) does not reach the result. workspace: device scratch of the size
  * prana_attention_tree_workspace gives for the same sizes (it may be 0, then
  * workspace may be NULL); calls that may run at the same time (also replays of
- * two captured graphs) need one each. 8-bit: values up to 2^64 in magnitude. */
+ * two captured graphs) need one each. 8-bit: a weight counts times its V scale,
+ * with 22 bits, or to 2^-31 of the largest such product that its row sees;
+ * values up to 2^64 in magnitude, those under 2^-105 right to 2^-136 of 1. */
 int prana_attention_tree(const float *q, int kv_type, const prana_kv *kv, const size_t *past, const size_t *n_tree,
                          size_t n_seq, const uint64_t *mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
                          float *out, void *workspace, size_t workspace_bytes, prana_stream_t stream);

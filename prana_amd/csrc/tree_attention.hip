@@ -163,6 +163,14 @@ __device__ __forceinline__ void load_values(const unsigned char* p, float scale,
 // of 98, but a masked row of large scale took the other rows' bits.)
 constexpr float kTop = kLag + kPShift;  // products of weights and scales stay under 2^kTop
 constexpr float kUnseen = -3e38f;       // the reference of a row that has seen nothing
+// The scales themselves are taken times 2^32, so that x reaches from scales of
+// 2^-112 to ones past 2^57 (2^64 as values): smaller ones' products are right to
+// 2^-137, half steps of 2^-25 over 2^(80 + 32). A scale past 2^96, which only a
+// row that nothing sees should have, stops at a float's end.
+constexpr float kLift = 0x1p32f;
+__device__ __forceinline__ float lifted(float v) {
+  return fabsf(v) < INFINITY ? fminf(fmaxf(v * kLift, -0x1.fffffep127f), 0x1.fffffep127f) : v;
+}
 // x, at least -80: weights stay under 2^(80 + 15), and 2^30 of them under a float's end.
 __device__ __forceinline__ float scale_log2(float v) {
   return static_cast<float>(max(static_cast<int>(__float_as_uint(v) >> 23 & 255u) - 126, -80));
@@ -362,8 +370,11 @@ void tree_narrow_kernel(TreeArgs a) {
       *reinterpret_cast<u32x4*>(s_v + (e / (HDP / 8)) * S::kLdV + (e % (HDP / 8)) * 8) = vr[p].halves();
     }
     if constexpr (Q8) {
+      if (lane >= 32) {
+        sc = lifted(sc);
+        s_scale[wave][32 + lane] = scale_log2(sc);
+      }
       s_scale[wave][lane] = sc;
-      if (lane >= 32) s_scale[wave][32 + lane] = scale_log2(sc);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -538,7 +549,8 @@ void tree_narrow_kernel(TreeArgs a) {
     float M = s_m[0][i];
 #pragma unroll
     for (int w = 1; w < S::kWaves; w++) M = fmaxf(M, s_m[w][i]);
-    const float f = m[r] == -INFINITY ? 0.0f : exp2_hw(m[r] - M);
+    float f = m[r] == -INFINITY ? 0.0f : exp2_hw(m[r] - M);
+    if constexpr (Q8) f *= 1.0f / kLift;
 #pragma unroll
     for (int mb = 0; mb < S::kDimBlocks; mb++) {
       // a wave that saw nothing of this row holds zeros
@@ -698,8 +710,11 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
       *reinterpret_cast<u32x4*>(s_v + r * S::kLdV + d) = vr[p].halves();
     }
     if constexpr (Q8) {
+      if (tid >= BN) {
+        sc = lifted(sc);
+        if (tid < 2 * BN) s_scale[2][tid % BN] = scale_log2(sc);
+      }
       if (tid < 2 * BN) s_scale[tid / BN][tid % BN] = sc;
-      if (tid >= BN && tid < 2 * BN) s_scale[2][tid % BN] = scale_log2(sc);
     }
     __syncthreads();
     if (k0 + BN < kend) fetch(k0 + BN);
@@ -863,14 +878,15 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
       ml[1] = l;
     }
   }
+  constexpr float kDown = Q8 ? 1.0f / kLift : 1.0f;
 #pragma unroll
   for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
     for (int g = 0; g < 4; g++) {
       const uint32_t d = mb * 32 + 8 * g + 4 * h;
       if (d < hd)
-        *reinterpret_cast<float4*>(dst + d) =
-            make_float4(o[mb][4 * g] * f, o[mb][4 * g + 1] * f, o[mb][4 * g + 2] * f, o[mb][4 * g + 3] * f);
+        *reinterpret_cast<float4*>(dst + d) = make_float4(o[mb][4 * g] * kDown * f, o[mb][4 * g + 1] * kDown * f,
+                                                          o[mb][4 * g + 2] * kDown * f, o[mb][4 * g + 3] * kDown * f);
     }
 }
 

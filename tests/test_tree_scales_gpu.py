@@ -131,3 +131,18 @@ def test_scores_too_large_to_add_a_scales_exponent_to(tokens, heads, kv_heads, w
     c.scale(0, 2.0 ** r.integers(-60, 30, (past + tokens, kv_heads)))
     got = P.attention_tree(q, c.caches, [past], [tokens], heads, kv_heads, w)
     assert np.isfinite(got).all() and np.abs(got).max() <= 1.001 * c.tops()[0].max()
+
+
+@pytest.mark.parametrize("powers", [(-70,), (-90,), (-100,), (-100, -60), (-100, 57), (57,)])
+@pytest.mark.parametrize("past", [20, 3000])
+@pytest.mark.parametrize("tokens,heads,kv_heads,w", SHAPES)
+def test_scales_at_the_ends_of_their_range(tokens, heads, kv_heads, w, past, powers):
+    # (the scales lie around 2^-6; alternating ones, and the first half of the rows small)
+    r = np.random.default_rng(9)
+    q = (r.standard_normal((tokens, heads * w)) * 1.5).astype(np.float32)
+    for split in (False, True):
+        c = Caches(10, [past + tokens], kv_heads, w)
+        at = np.arange(past + tokens)
+        which = (at > len(at) // 2) if split else at % 2
+        c.scale(0, 2.0 ** np.array(powers)[np.minimum(which, len(powers) - 1)][:, None])
+        check(c, q, [past], [tokens], None, heads)
