@@ -66,6 +66,11 @@ __device__ __forceinline__ void reads_ahead() {
 // 2^x as the hardware computes it (1 ulp; results under 2^-126 are 0).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Scores of 2^22 and more (log2 units) lie half a unit and more apart: a
+// difference of them is taken before it is multiplied or shifted, or rounding
+// could carry a probability past a half's end.
+__device__ __forceinline__ bool coarse(float x) { return fabsf(x) >= 0x1p22f; }
+
 // Bit 15 of each half of the result: that half of w is an infinity or NaN
 // (its exponent, all ones, carries into the sign's place).
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) { return (w & 0x7c007c00u) + 0x04000400u; }

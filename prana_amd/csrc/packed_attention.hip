@@ -222,7 +222,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, GROUPS == 1 && HDP <= 64 ? 3 :
   for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[mb][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f;  // kept maximum (log2 units) and this lane's share of the sum
+  float m = -INFINITY, l = 0.0f;  // kept maximum (of scores before c) and this lane's share of the sum
 
   constexpr uint32_t kRound = GROUPS * BN;
   for (uint32_t r0 = 0; r0 <= tok_last_wg; r0 += kRound) {
@@ -257,17 +257,27 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, GROUPS == 1 && HDP <= 64 ? 3 :
     for (int b = 0; b < S::kKeyBlocks; b++)
 #pragma unroll
       for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[b][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-    if (__any(mx > m + kLag)) {
-      const float mn = fmaxf(m, mx), al = exp2_hw(m - mn);
-      m = mn;
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    float from = m;  // what scores are taken relative to, times c
+    if (__any((mx - m) * c > kLag || coarse(mx * c))) {
+      const bool up = (mx - m) * c > kLag;  // (each row for itself)
+      const float al = up ? exp2_hw((m - mx) * c) : 1.0f;
+      from = m = up ? mx : m;
       l *= al;
 #pragma unroll
       for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[mb][i] *= al;
+      if (__any(coarse(m * c))) {
+        const bool far = coarse(m * c);
+        from = far ? 0.0f : m;
+#pragma unroll
+        for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) s[b][i] -= far ? m : 0.0f;
+      }
     }
-    const float ms = m - kPShift;
+    const float ms = fmaf(from, c, -kPShift);
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
 #pragma unroll
@@ -320,6 +330,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, GROUPS == 1 && HDP <= 64 ? 3 :
   }
   l += __shfl_xor(l, 32, 64);
   if constexpr (GROUPS > 1) {
+    m *= c;
     // the other groups leave their sums in LDS, for the first to join
     const int row_wg = wave * 32 + n;
     __syncthreads();
@@ -487,17 +498,27 @@ __global__ __launch_bounds__(kWideGroups * 4 * kWideRows, 2) void packed_wide_ke
     float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-    if (__any(mx > m + kLag)) {
-      const float mn = fmaxf(m, mx), al = exp2_hw(m - mn);
-      m = mn;
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    float from = m;
+    if (__any((mx - m) * c > kLag || coarse(mx * c))) {
+      const bool up = (mx - m) * c > kLag;  // (each row for itself)
+      const float al = up ? exp2_hw((m - mx) * c) : 1.0f;
+      from = m = up ? mx : m;
       l *= al;
 #pragma unroll
       for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
         for (int i = 0; i < 4; i++) o[mb][i] *= al;
+      if (__any(coarse(m * c))) {
+        const bool far = coarse(m * c);
+        from = far ? 0.0f : m;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[b][i] -= far ? m : 0.0f;
+      }
     }
-    const float ms = m - kPShift;
+    const float ms = fmaf(from, c, -kPShift);
     half8 ph, pl;
 #pragma unroll
     for (int b = 0; b < 2; b++)
@@ -545,6 +566,7 @@ __global__ __launch_bounds__(kWideGroups * 4 * kWideRows, 2) void packed_wide_ke
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
+  m *= c;
   // the other groups leave their sums in LDS, for the first to join
   const int row_wg = wave * 16 + n;
   float* const s_o = reinterpret_cast<float*>(s_tiles) + row_wg * S::kLdO + 4 * g;

@@ -158,11 +158,12 @@ __device__ __forceinline__ void load_values(const unsigned char* p, float scale,
 // product then lies between 2^6 and 2^15, where two halves hold 22 bits, whatever
 // scales the keys have that the row does not see or gives no weight. With 2^x
 // above a key's scale, what is compared is score + x (log2 units); the weights
-// and their sum count from the reference. (One power of two for all rows of a
+// and their sum count from the reference, the largest score (m, before c) and
+// the rest (e) of it. (One power of two for all rows of a
 // wave, over all scales met, took 8 single tokens over up to 32767 rows 3 us less
 // of 98, but a masked row of large scale took the other rows' bits.)
 constexpr float kTop = kLag + kPShift;  // products of weights and scales stay under 2^kTop
-constexpr float kUnseen = -3e38f;       // the reference of a row that has seen nothing
+constexpr float kUnseen = -3e38f;       // in place of a row's reference when it has seen nothing
 // The scales themselves are taken times 2^32, so that x reaches from scales of
 // 2^-112 to ones past 2^57 (2^64 as values): smaller ones' products are right to
 // 2^-137, half steps of 2^-25 over 2^(80 + 32). A scale past 2^96, which only a
@@ -181,13 +182,6 @@ __device__ __forceinline__ float scale_log2(float v) {
 __device__ __forceinline__ float shift_sum(float l, float x) {
   const float half = exp2_hw(0.5f * x);
   return l * half * half;
-}
-// The reference for a largest score + x of mx. Past 2^22 that sum is rounded to
-// halves and more: two steps up keep every product under 2^kTop.
-__device__ __forceinline__ bool coarse(float mx) { return fabsf(mx) >= 0x1p22f; }
-__device__ __forceinline__ float reference(float mx) {
-  const float r = mx - kPShift;
-  return coarse(mx) ? fmaf(fabsf(r), 0x1p-22f, r) : r;
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
@@ -317,15 +311,15 @@ void tree_narrow_kernel(TreeArgs a) {
     }
   }
 
-  float c[RB], m[RB], l[RB];
+  float c[RB], m[RB], l[RB], e[RB];  // (m: the kept maximum, of scores before c; e: 8-bit)
   uint64_t word[RB];
   f32x4 o[RB][S::kDimBlocks];
 #pragma unroll
   for (int r = 0; r < RB; r++) {
     const uint32_t i = min(r * 16u + n, rows - 1) / a.group;
     word[r] = mask_word(a, sq, i);
-    m[r] = Q8 ? kUnseen : -INFINITY;
-    l[r] = 0.0f;
+    m[r] = -INFINITY;
+    l[r] = e[r] = 0.0f;
 #pragma unroll
     for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
@@ -440,42 +434,60 @@ void tree_narrow_kernel(TreeArgs a) {
           for (int j = 0; j < 4; j++)
             if (!(seen >> (b * 16 + j) & 1)) s[r][b][j] = -INFINITY;
       }
-      auto rescale = [&](float mn, float al) {
-        l[r] = Q8 ? shift_sum(l[r], m[r] - mn) : l[r] * al;
-        m[r] = mn;
+      auto row_max = [&](auto of) {  // over the row's keys
+        float x = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) x = fmaxf(x, of(b, j));
+        x = fmaxf(x, __shfl_xor(x, 16, 64));
+        return fmaxf(x, __shfl_xor(x, 32, 64));
+      };
+      auto rescale = [&](float al) {
 #pragma unroll
         for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
           for (int j = 0; j < 4; j++) o[r][mb][j] *= al;
       };
-      float ms;
+      auto relative = [&](bool far) {  // scores too large for their differences to be taken later
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[r][b][j] -= far ? m[r] : 0.0f;
+      };
+      float ms;  // what a weight counts from
       if constexpr (Q8) {
-        auto largest = [&](auto of) {  // over the row's keys, of a score and its scale's exponent
-          float x = -INFINITY;
-#pragma unroll
-          for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) x = fmaxf(x, of(s[r][b][j], vx[b][j]));
-          x = fmaxf(x, __shfl_xor(x, 16, 64));
-          return fmaxf(x, __shfl_xor(x, 32, 64));
-        };
-        const float mx = largest([&](float score, float x) { return fmaf(score, c[r], x); });
-        if (__any(mx - m[r] > kTop || coarse(mx))) {
-          const float past = largest([&](float score, float x) { return fmaf(score, c[r], -m[r]) + x; });
-          const float mn = past > kTop ? reference(mx) : m[r];
-          rescale(mn, exp2_hw(m[r] - mn));
+        const float mx = row_max([&](int b, int j) { return fmaf(s[r][b][j], c[r], vx[b][j]); });
+        ms = m[r] == -INFINITY ? kUnseen : fmaf(m[r], c[r], e[r]);
+        if (__any(mx - ms > kTop || coarse(mx))) {
+          auto past = [&](int b, int j) { return fmaf(s[r][b][j] - m[r], c[r], vx[b][j]); };
+          const bool up = row_max(past) - e[r] > kTop;
+          const float mw = m[r], ew = e[r], raw = row_max([&](int b, int j) { return s[r][b][j]; });
+          m[r] = up ? fmaxf(mw, raw) : mw;
+          e[r] = up ? row_max(past) - kPShift : ew;
+          const float x = up ? (mw - m[r]) * c[r] + (ew - e[r]) : 0.0f;
+          l[r] = shift_sum(l[r], x);
+          rescale(exp2_hw(x));
+          const bool far = coarse(m[r] * c[r]) && m[r] != -INFINITY;
+          if (__any(far)) relative(far);
+          ms = m[r] == -INFINITY ? kUnseen : far ? e[r] : fmaf(m[r], c[r], e[r]);
         }
-        ms = m[r];
       } else {
-        float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
-                         fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c[r];
-        if (__any(mx > m[r] + kLag)) {
-          const float mn = fmaxf(m[r], mx);
-          rescale(mn, mn == -INFINITY ? 1.0f : exp2_hw(m[r] - mn));  // (a row that has seen nothing yet)
+        const float mx = row_max([&](int b, int j) { return s[r][b][j]; });
+        float from = m[r];  // times c
+        if (__any((mx - m[r]) * c[r] > kLag || coarse(mx * c[r]))) {
+          const bool up = (mx - m[r]) * c[r] > kLag;  // (each row for itself)
+          const float al = up ? exp2_hw((m[r] - mx) * c[r]) : 1.0f;
+          from = m[r] = up ? mx : m[r];
+          l[r] *= al;
+          rescale(al);
+          const bool far = coarse(m[r] * c[r]) && m[r] != -INFINITY;
+          if (__any(far)) {
+            relative(far);
+            from = far ? 0.0f : m[r];
+          }
         }
-        ms = m[r] == -INFINITY ? 0.0f : m[r] - kPShift;
+        ms = from == -INFINITY ? 0.0f : fmaf(from, c[r], -kPShift);
       }
 #pragma unroll
       for (int b = 0; b < 2; b++)
@@ -535,6 +547,7 @@ void tree_narrow_kernel(TreeArgs a) {
   for (int r = 0; r < RB; r++) {
     l[r] += __shfl_xor(l[r], 16, 64);
     l[r] += __shfl_xor(l[r], 32, 64);
+    m[r] = m[r] == -INFINITY ? (Q8 ? kUnseen : m[r]) : fmaf(m[r], c[r], e[r]);
     if (g == 0) {
       s_m[wave][r * 16 + n] = m[r];
       s_l[wave][r * 16 + n] = l[r];
@@ -679,7 +692,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
     for (int j = 0; j < 16; j++) o[mb][j] = 0.0f;
-  float m = Q8 ? kUnseen : -INFINITY, l = 0.0f;
+  float m = -INFINITY, l = 0.0f, e = 0.0f;
 
   for (uint32_t k0 = kbeg; k0 < kend; k0 += BN) {
     const bool edge = k0 + BN > min(sq.past, kend);
@@ -759,48 +772,65 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
         for (int j = 0; j < 16; j++)
           if (!(seen >> (b * 32 + 8 * (j / 4) + j % 4) & 1)) s[b][j] = -INFINITY;
     }
-    auto rescale = [&](float mn, float al) {
-      l = Q8 ? shift_sum(l, m - mn) : l * al;
-      m = mn;
+    auto row_max = [&](auto of) {  // over the row's keys, of a score and the exponent of its V scale (8-bit)
+      float x = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < S::kKeyBlocks; b++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          float4 vx = make_float4(0, 0, 0, 0);
+          if constexpr (Q8) vx = *reinterpret_cast<const float4*>(&s_scale[2][b * 32 + 8 * g + 4 * h]);
+          const float v4[4] = {vx.x, vx.y, vx.z, vx.w};
+#pragma unroll
+          for (int j = 0; j < 4; j++) x = fmaxf(x, of(s[b][4 * g + j], v4[j]));
+        }
+      return fmaxf(x, __shfl_xor(x, 32, 64));
+    };
+    auto rescale = [&](float al) {
 #pragma unroll
       for (int mb = 0; mb < S::kDimBlocks; mb++)
 #pragma unroll
         for (int j = 0; j < 16; j++) o[mb][j] *= al;
     };
-    float ms;
-    if constexpr (Q8) {  // (as in the narrow kernel)
-      auto largest = [&](auto of) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < S::kKeyBlocks; b++)
-#pragma unroll
-          for (int g = 0; g < 4; g++) {
-            const float4 vx = *reinterpret_cast<const float4*>(&s_scale[2][b * 32 + 8 * g + 4 * h]);
-            const float v4[4] = {vx.x, vx.y, vx.z, vx.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) x = fmaxf(x, of(s[b][4 * g + j], v4[j]));
-          }
-        return fmaxf(x, __shfl_xor(x, 32, 64));
-      };
-      const float mx = largest([&](float score, float x) { return fmaf(score, c, x); });
-      if (__any(mx - m > kTop || coarse(mx))) {
-        const float past = largest([&](float score, float x) { return fmaf(score, c, -m) + x; });
-        const float mn = past > kTop ? reference(mx) : m;
-        rescale(mn, exp2_hw(m - mn));
-      }
-      ms = m;
-    } else {
-      float mx = s[0][0];
+    auto relative = [&](bool far) {
 #pragma unroll
       for (int b = 0; b < S::kKeyBlocks; b++)
 #pragma unroll
-        for (int j = 0; j < 16; j++) mx = fmaxf(mx, s[b][j]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-      if (__any(mx > m + kLag)) {
-        const float mn = fmaxf(m, mx);
-        rescale(mn, mn == -INFINITY ? 1.0f : exp2_hw(m - mn));
+        for (int j = 0; j < 16; j++) s[b][j] -= far ? m : 0.0f;
+    };
+    float ms;
+    if constexpr (Q8) {  // (as in the narrow kernel)
+      const float mx = row_max([&](float score, float x) { return fmaf(score, c, x); });
+      ms = m == -INFINITY ? kUnseen : fmaf(m, c, e);
+      if (__any(mx - ms > kTop || coarse(mx))) {
+        auto past = [&](float score, float x) { return fmaf(score - m, c, x); };
+        const bool up = row_max(past) - e > kTop;
+        const float mw = m, ew = e, raw = row_max([&](float score, float) { return score; });
+        m = up ? fmaxf(mw, raw) : mw;
+        e = up ? row_max(past) - kPShift : ew;
+        const float x = up ? (mw - m) * c + (ew - e) : 0.0f;
+        l = shift_sum(l, x);
+        rescale(exp2_hw(x));
+        const bool far = coarse(m * c) && m != -INFINITY;
+        if (__any(far)) relative(far);
+        ms = m == -INFINITY ? kUnseen : far ? e : fmaf(m, c, e);
       }
-      ms = m == -INFINITY ? 0.0f : m - kPShift;
+    } else {
+      const float mx = row_max([&](float score, float) { return score; });
+      float from = m;
+      if (__any((mx - m) * c > kLag || coarse(mx * c))) {
+        const bool up = (mx - m) * c > kLag;
+        const float al = up ? exp2_hw((m - mx) * c) : 1.0f;
+        from = m = up ? mx : m;
+        l *= al;
+        rescale(al);
+        const bool far = coarse(m * c) && m != -INFINITY;
+        if (__any(far)) {
+          relative(far);
+          from = far ? 0.0f : m;
+        }
+      }
+      ms = from == -INFINITY ? 0.0f : fmaf(from, c, -kPShift);
     }
 #pragma unroll
     for (int b = 0; b < S::kKeyBlocks; b++)
@@ -862,6 +892,7 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
     }
   }
   l += __shfl_xor(l, 32, 64);
+  m = m == -INFINITY ? (Q8 ? kUnseen : m) : fmaf(m, c, e);
   if (row0 + wave * 32 + n >= rows) return;
   float f;
   float* dst;

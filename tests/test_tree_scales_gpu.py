@@ -131,6 +131,7 @@ def test_scores_too_large_to_add_a_scales_exponent_to(tokens, heads, kv_heads, w
     c.scale(0, 2.0 ** r.integers(-60, 30, (past + tokens, kv_heads)))
     got = P.attention_tree(q, c.caches, [past], [tokens], heads, kv_heads, w)
     assert np.isfinite(got).all() and np.abs(got).max() <= 1.001 * c.tops()[0].max()
+    assert got.any(1).all()
 
 
 @pytest.mark.parametrize("powers", [(-70,), (-90,), (-100,), (-100, -60), (-100, 57), (57,)])
