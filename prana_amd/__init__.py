@@ -340,6 +340,11 @@ def attention_prefill(q, k, v, seq, n_heads, n_kv_heads, head_dim):
 
 
 # ---------------------------------------------------------------- serving
+def _ints(*sizes):
+    """Sizes as Python integers, whose sums and products do not wrap as numpy's do."""
+    return [[int(x) for x in s] for s in sizes]
+
+
 def _halves(a):
     a = np.ascontiguousarray(a)
     _want(a.dtype.itemsize == 2, "halves (f16 values or their bits) are expected")
@@ -369,6 +374,7 @@ class KvQ8:
     kind = KV_Q8
 
     def __init__(self, rows, n_kv_heads, head_dim):
+        (rows, n_kv_heads, head_dim), = _ints((rows, n_kv_heads, head_dim))
         self.rows, self.n_kv_heads, self.head_dim, self.width = rows, n_kv_heads, head_dim, n_kv_heads * head_dim
         self.k, self.v = (DeviceArray.from_host(np.zeros((rows, n_kv_heads * head_dim), np.int8)) for _ in "kv")
         self.k_scales, self.v_scales = (DeviceArray.from_host(np.ones((rows, n_kv_heads), np.float32)) for _ in "kv")
@@ -395,7 +401,7 @@ def _check_caches(caches, kinds, width, *per_seq):
     _want(len({c.kind for c in caches}) <= 1 and all(c.kind in kinds for c in caches), "caches of another kind")
     _want(all(c.width == width for c in caches), f"a cache's rows are not {width} values")
     _want(all(len(x) == len(caches) for x in per_seq), "one size per cache")
-    _want(all(int(x) >= 0 for sizes in per_seq for x in sizes), "a negative size")
+    _want(all(x >= 0 for sizes in per_seq for x in sizes), "a negative size")
 
 
 def kv_write_q8(caches, k, v, first_rows, n_rows):
@@ -404,6 +410,7 @@ def kv_write_q8(caches, k, v, first_rows, n_rows):
     if not caches:
         return
     k, v = np.asarray(k, np.float32), np.asarray(v, np.float32)
+    first_rows, n_rows = _ints(first_rows, n_rows)
     heads, w = caches[0].n_kv_heads, caches[0].head_dim
     _check_caches(caches, (KV_Q8,), heads * w, first_rows, n_rows)
     _want(all(c.n_kv_heads == heads for c in caches), "caches of other heads")
@@ -418,10 +425,11 @@ def kv_read_q8(caches, first_rows, n_rows, half=False):
     """Rows of KvQ8 caches (at least one cache) as values, packed: (k, v) in
     f32, or in f16."""
     _want(len(caches) > 0, "no cache")
+    first_rows, n_rows = _ints(first_rows, n_rows)
     heads, w = caches[0].n_kv_heads, caches[0].head_dim
     _check_caches(caches, (KV_Q8,), heads * w, first_rows, n_rows)
     _want(all(c.n_kv_heads == heads for c in caches), "caches of other heads")
-    dk, dv = (DeviceArray((int(sum(n_rows)), heads * w), np.float16 if half else np.float32) for _ in "kv")
+    dk, dv = (DeviceArray((sum(n_rows), heads * w), np.float16 if half else np.float32) for _ in "kv")
     check(load().prana_kv_read_q8(_kv_structs(caches), _sizes(first_rows), _sizes(n_rows), len(caches), heads, w,
                                   F16 if half else F32, dk.ptr, dv.ptr, heads * w, None))
     return dk.to_host(), dv.to_host()
@@ -433,7 +441,8 @@ def attention_packed(q, k, v, seq_lens, n_heads, n_kv_heads, head_dim):
     q, k, v = np.ascontiguousarray(q), _halves(k), _halves(v)
     kind = {np.dtype(np.float32): F32, np.dtype(np.float16): F16}.get(q.dtype)
     _want(kind is not None, "q is f32 or f16")
-    _want(all(int(n) >= 0 for n in seq_lens), "a negative size")
+    seq_lens, (n_heads, n_kv_heads, head_dim) = _ints(seq_lens, (n_heads, n_kv_heads, head_dim))
+    _want(all(n >= 0 for n in seq_lens), "a negative size")
     _want(q.shape == (sum(seq_lens), n_heads * head_dim), "q holds the rows of seq_lens, one after another")
     _want(k.shape == v.shape == (sum(seq_lens), n_kv_heads * head_dim), "k and v hold the rows of seq_lens")
     dq, dk, dv = (DeviceArray.from_host(x) for x in (q, k, v))
@@ -445,7 +454,8 @@ def attention_packed(q, k, v, seq_lens, n_heads, n_kv_heads, head_dim):
 
 def attention_tree_workspace(past, n_tree, n_heads, n_kv_heads, head_dim):
     """Bytes of device scratch attention_tree needs for these sizes."""
-    _want(len(past) == len(n_tree) and all(int(x) >= 0 for x in [*past, *n_tree]), "one size per sequence")
+    past, n_tree = _ints(past, n_tree)
+    _want(len(past) == len(n_tree) and all(x >= 0 for x in [*past, *n_tree]), "one size per sequence")
     n = C.c_size_t()
     check(load().prana_attention_tree_workspace(_sizes(past), _sizes(n_tree), len(past), n_heads, n_kv_heads,
                                                 head_dim, C.byref(n)))
@@ -457,6 +467,7 @@ def attention_tree(q, caches, past, n_tree, n_heads, n_kv_heads, head_dim, mask=
     caches: q [sum(n_tree), n_heads*head_dim] f32, mask one word per drafted
     token (bit j: it sees drafted token j of its sequence; None = a chain)."""
     q = np.asarray(q, np.float32)
+    past, n_tree, (n_heads, n_kv_heads, head_dim) = _ints(past, n_tree, (n_heads, n_kv_heads, head_dim))
     _check_caches(caches, (KV_F16, KV_Q8), n_kv_heads * head_dim, past, n_tree)
     _want(all(c.kind != KV_Q8 or c.n_kv_heads == n_kv_heads for c in caches), "caches of other heads")
     _want(q.shape == (sum(n_tree), n_heads * head_dim), "q holds the rows of n_tree, one after another")
