@@ -249,7 +249,9 @@ int prana_kv_read_q8(const prana_kv *kv, const size_t *first_rows, const size_t 
  * to q. What masked rows and rows past the drafted ones hold (infinities and
  * NaN too) does not reach the result. workspace: device scratch of the size
  * prana_attention_tree_workspace gives for the same sizes (it may be 0, then
- * workspace may be NULL); calls that may run at the same time (also replays of
+ * workspace may be NULL; no size shrinks it as it grows, so one allocated for
+ * the longest caches, most drafted tokens and sequences serves every smaller
+ * call); calls that may run at the same time (also replays of
  * two captured graphs) need one each. 8-bit: a weight counts times its V scale,
  * with 22 bits, or to 2^-31 of the largest such product that its row sees;
  * values up to 2^64 in magnitude, those under 2^-105 right to 2^-136 of 1. */

@@ -503,7 +503,8 @@ int prana_attention_tree(const float* q, int kv_type, const prana_kv* kv, const 
       return rc;
     INIT_OR_RETURN();
     return launch_attention_tree(q, kv_type == PRANA_KV_Q8, kv, past, n_tree, n_seq, mask, n_heads, n_kv_heads,
-                                 head_dim, out, static_cast<float*>(workspace), pick_stream(stream));
+                                 head_dim, out, static_cast<float*>(workspace), workspace_bytes / sizeof(float),
+                                 pick_stream(stream));
   });
 }
 

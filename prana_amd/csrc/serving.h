@@ -47,11 +47,11 @@ int launch_kv_read_q8(const prana_kv* kv, const size_t* first_rows, const size_t
                       size_t n_kv_heads, size_t head_dim, bool half, void* k, void* v, size_t ld, hipStream_t s);
 
 // ------------------------------------------------------------ tree_attention.hip
-// Floats of workspace a call with these sizes needs.
+// Floats of workspace for a call with these sizes, or smaller ones.
 size_t attention_tree_floats(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads,
                              size_t n_kv_heads, size_t head_dim);
 int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const size_t* past, const size_t* n_tree,
                           size_t n_seq, const uint64_t* mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
-                          float* out, float* workspace, hipStream_t s);
+                          float* out, float* workspace, size_t workspace_floats, hipStream_t s);
 
 }  // namespace prana

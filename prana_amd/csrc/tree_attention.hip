@@ -1134,16 +1134,37 @@ void launch_width(const TreeArgs& a, Width w, bool q8, uint32_t items, hipStream
 
 }  // namespace
 
+// No plan needs more, and more of anything needs no less: a server allocates for
+// its largest sizes once. (The plans themselves do not grow with the cache: longer
+// caches are cut into longer parts.) A sequence has at most as many parts as the
+// shortest ones make, 128 rows, or a narrow round where no width present is wider;
+// and in the launches of one width the parts make at most 2 resident() workgroups,
+// each with a tile of rows: a part has at least work / resident() rows, and who has
+// parts has more rows than one.
 size_t attention_tree_floats(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads,
                              size_t n_kv_heads, size_t head_dim) {
-  return std::max(make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim, false).floats,
-                  make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim, true).floats);
+  const size_t group = n_heads / n_kv_heads;
+  int widest = kNarrow16;
+  for (size_t i = 0; i < n_seq; i++)
+    if (n_tree[i]) widest = std::max<int>(widest, width_of(n_tree[i] * group, head_dim, false));
+  const bool narrow = widest == kNarrow16;
+  const size_t round = 32 * narrow_waves(static_cast<int>(head_dim));
+  const size_t least = narrow ? round : 128, whole = narrow ? 2 * round : least;
+  size_t most = 0, rows = 0;
+  const size_t tile[kWidths] = {16, 32, kWideRows};
+  for (int w = 0; w <= widest; w++) most += 2 * resident(static_cast<Width>(w), head_dim) * tile[w];
+  for (size_t i = 0; i < n_seq; i++) {
+    const size_t total = past[i] + n_tree[i];
+    if (total > whole) rows += n_tree[i] * n_heads * ((total + least - 1) / least);
+  }
+  return std::min(most, rows) * (head_dim + 2);
 }
 
 int launch_attention_tree(const float* q, bool q8, const prana_kv* kv, const size_t* past, const size_t* n_tree,
                           size_t n_seq, const uint64_t* mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
-                          float* out, float* workspace, hipStream_t s) {
+                          float* out, float* workspace, size_t workspace_floats, hipStream_t s) {
   const Plan plan = make_plan(past, n_tree, n_seq, n_heads, n_kv_heads, head_dim, q8);
+  if (plan.floats > workspace_floats) return fail(kErrInvalid, "attention_tree: a plan passes its bound");
   TreeArgs a{};
   a.q = q;
   a.mask = mask;
