@@ -618,6 +618,8 @@ size_t tile_rows(size_t head_dim, bool divided) {
   return head_dim > 128 ? kWideRows : divided && head_dim <= 96 ? 64 : 128;
 }
 
+size_t tile_lanes(size_t head_dim, bool divided) { return head_dim > 128 || divided ? 512 : 256; }
+
 // Whether workgroups divide the keys among groups of waves: four groups of two
 // waves (64 rows) for heads up to 96 wide, two of four for heads up to 128. That
 // shortens the longest walk over the keys, which bounds a call of few rows, but
@@ -643,15 +645,15 @@ bool divide(const std::vector<Seq>& seqs, size_t group, size_t n_kv, size_t head
 
 template <int HDP, bool HALF>
 void launch_shape(const PackedArgs& a, bool divided, uint32_t tiles, hipStream_t s) {
-  const dim3 grid(tiles * a.n_kv);
+  const dim3 grid(tiles * a.n_kv), lanes(static_cast<uint32_t>(tile_lanes(HDP, divided)));
   if constexpr (HDP <= 128) {
     constexpr int kWaves = HDP <= 96 ? 2 : 4;
     if (divided)
-      hipLaunchKernelGGL((packed_kernel<HDP, HALF, kWaves, 8 / kWaves>), grid, dim3(512), 0, s, a);
+      hipLaunchKernelGGL((packed_kernel<HDP, HALF, kWaves, 8 / kWaves>), grid, lanes, 0, s, a);
     else
-      hipLaunchKernelGGL((packed_kernel<HDP, HALF, 4, 1>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((packed_kernel<HDP, HALF, 4, 1>), grid, lanes, 0, s, a);
   } else {
-    hipLaunchKernelGGL((packed_wide_kernel<HDP, HALF>), grid, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((packed_wide_kernel<HDP, HALF>), grid, lanes, 0, s, a);
   }
 }
 
@@ -664,6 +666,12 @@ void launch_type(const PackedArgs& a, bool half, bool divided, uint32_t tiles, h
 }
 
 }  // namespace
+
+// (Workgroups divide the keys for few rows only.)
+size_t packed_lanes(size_t len, size_t n_heads, size_t n_kv_heads, size_t head_dim) {
+  const size_t rows = tile_rows(head_dim, false);
+  return (len * (n_heads / n_kv_heads) + rows - 1) / rows * n_kv_heads * tile_lanes(head_dim, false);
+}
 
 int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v, bool half, const size_t* seq_lens,
                             size_t n_seq, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t ld_q,
@@ -690,7 +698,7 @@ int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v,
   std::stable_sort(seqs.begin(), seqs.end(), [](const Seq& x, const Seq& y) { return x.len > y.len; });
   const bool divided = divide(seqs, a.group, n_kv_heads, head_dim);
   const size_t rows = tile_rows(head_dim, divided);
-  // Tiles of one grid: its lanes are to fit 32 bits (one sequence's do, by the length check).
+  // Tiles of one grid: its lanes are to fit 32 bits (one sequence's do: packed_lanes).
   const size_t most = (size_t{1} << 22) / n_kv_heads;
   for (size_t i = 0; i < seqs.size();) {
     size_t tiles = 0;

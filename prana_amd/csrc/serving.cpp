@@ -38,7 +38,8 @@ int check_attention_packed(const void* q, const uint16_t* k, const uint16_t* v, 
   if (n_seq && !seq_lens) return refuse(what, "null seq_lens");
   size_t total = 0;
   for (size_t i = 0; i < n_seq; i++) {
-    if (seq_lens[i] > kMaxRows || seq_lens[i] * n_heads > kMaxRows)
+    if (seq_lens[i] > kMaxRows || seq_lens[i] * n_heads > kMaxRows ||
+        packed_lanes(seq_lens[i], n_heads, n_kv_heads, head_dim) > 0xffffffffu)
       return refuse(what, "sequence " + std::to_string(i) + " is too long");
     total += seq_lens[i];
     if (total > 0xffffffffu) return refuse(what, "more than 2^32 - 1 rows");

@@ -36,6 +36,8 @@ int check_tree_sizes(const size_t* past, const size_t* n_tree, size_t n_seq, siz
 constexpr size_t kMaxTree = 64;  // drafted tokens of a sequence: the bits of a mask word
 
 // ------------------------------------------------------------ packed_attention.hip
+// Lanes of the launch that one sequence needs at least: they are to fit 32 bits.
+size_t packed_lanes(size_t len, size_t n_heads, size_t n_kv_heads, size_t head_dim);
 int launch_attention_packed(const void* q, const uint16_t* k, const uint16_t* v, bool half, const size_t* seq_lens,
                             size_t n_seq, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t ld_q,
                             size_t ld_kv, size_t ld_out, void* out, hipStream_t s);

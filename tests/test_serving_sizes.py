@@ -1,14 +1,22 @@
-"""CPU: sizes of the serving calls that come in small integer types, whose sums
-numpy would wrap: shapes that fit the wrapped sum are refused before the device
-is touched."""
+"""CPU: sizes of the serving calls that are refused before the device is touched:
+those that come in small integer types, whose sums numpy would wrap, where the
+shapes fit the wrapped sum, and those past what one launch can hold."""
 import numpy as np
 import pytest
 
 import prana_amd as P
-from tests.test_serving_refusals import Cache, rows
+from tests.test_serving_refusals import INVALID, Cache, message, packed, rows
 
 SMALL = np.array([200, 100], np.uint8)  # 300 rows; 44 in 8 bits
 HALVES = [rows(44, 16, np.float16)] * 2
+
+
+def test_prompts_whose_launch_would_pass_2_to_32_lanes():
+    # heads wider than 128: 512 lanes for 64 rows (of a KV head's group); 4 query heads each
+    wide = dict(hd=256, ld_q=2048, ld_kv=512, ld_out=2048)
+    assert packed(lens=((1 << 26) - 16,), q=None, **wide) == INVALID and "null buffer" in message()  # (length taken)
+    assert packed(lens=(5, 1 << 26), q=None, **wide) == INVALID and "sequence 1 is too long" in message()
+    assert packed(lens=(1 << 27,), q=None) == INVALID and "null buffer" in message()
 
 
 @pytest.mark.filterwarnings("ignore::RuntimeWarning")
