@@ -127,7 +127,9 @@ def prepare(case, seed):
         return torch.randn(*shape, device="cuda", generator=g) * sigma
 
     n = _lengths(case)
-    s = {"case": case, "lens": n, "sizes": _sizes(n)}
+    # the calls go behind what the program's stream makes of their inputs (its default stream is 0, the library's own
+    # to these calls: such a program waits for its inputs first)
+    s = {"case": case, "lens": n, "sizes": _sizes(n), "stream": torch.cuda.current_stream().cuda_stream or None}
     kvw = case["kv_heads"] * case["width"]
     if case["op"] == "prompt":
         total, qw = sum(n), case["heads"] * case["width"]
@@ -193,22 +195,22 @@ def _own(s):
         P.check(lib.prana_attention_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                            P.F32 if c["type"] == "f32" else P.F16, s["sizes"], c["seqs"], c["heads"],
                                            c["kv_heads"], c["width"], q.stride(0), k.stride(0), out.stride(0),
-                                           out.data_ptr(), None))
+                                           out.data_ptr(), s["stream"]))
         return out
     kv = _caches(P, s)
     if c["op"] == "tree":
         P.check(lib.prana_attention_tree(s["q"].data_ptr(), P.KV_F16 if c["cache"] == "f16" else P.KV_Q8, kv,
                                          s["sizes"], s["drafts"], c["seqs"], s["mask"].data_ptr(), c["heads"],
                                          c["kv_heads"], c["width"], s["out"].data_ptr(), s["work"].data_ptr(),
-                                         s["work"].numel(), None))
+                                         s["work"].numel(), s["stream"]))
         return s["out"]
     if c["mode"] == "write":
         src = s["src"]
         P.check(lib.prana_kv_write_q8(src.data_ptr(), src.data_ptr() + 2 * src.shape[1], src.shape[1], kv,
-                                      s["firsts"], s["sizes"], c["seqs"], c["kv_heads"], c["width"], None))
+                                      s["firsts"], s["sizes"], c["seqs"], c["kv_heads"], c["width"], s["stream"]))
     P.check(lib.prana_kv_read_q8(kv, s["firsts"], s["sizes"], c["seqs"], c["kv_heads"], c["width"],
                                  P.F32 if c["type"] == "f32" else P.F16, s["k_out"].data_ptr(),
-                                 s["v_out"].data_ptr(), s["k_out"].shape[1], None))
+                                 s["v_out"].data_ptr(), s["k_out"].shape[1], s["stream"]))
     return s["k_out"], s["v_out"]
 
 
