@@ -1066,44 +1066,76 @@ size_t resident(Width w, size_t hd) {
 // other sequences of the call have parts: 15.4 against 11.0).
 //
 // A kernel's launch and its joining cost a call that has sequences of several
-// widths about 8 us each, so few cache rows of a smaller width go along on the
-// wider kernel, where reading them, with most of it idle, costs less than that:
-// up to 2^26 values of an f16 cache, 2^24 of an 8-bit one (trees of 4 to 8
-// tokens in four sequences, 12/4 x 128: caches of up to 4000 25.4 us on two
-// kernels and 15.3 on one, 8-bit 28.3 and 16.5; 16 single tokens over up to
-// 20000 8-bit rows 43 us narrow and 74 wide).
+// widths about 8 us each, so those of a smaller width go along on the wider
+// kernel, most of it idle, while its longest part grows by no more than `along`
+// rows for them. One tree of 40 over 1000 rows beside 4 and 16 single tokens, us on
+// one kernel and on two, where it would grow to about
+//                     256 rows         512              1000
+//   f16    32/8 x 64                   25 29   28 29    41 40    46 40
+//          32/8 x 128   27 34  29 35   37 44   42 44    59 61    66 62
+//          8/1 x 256    39 47  39 48   56 56   56 56    86 72    90 75
+//          16/8 x 256   36 44  48 45   57 53   83 54    89 71   139 72
+//   8-bit  32/8 x 64    21 30  23 30   30 33   34 33
+//          32/8 x 128   30 34  33 35
+//          16/8 x 256   40 44  56 45
+// (Two blocks of narrow rows beside one, 8-bit, 32/8 x 64 and x 128: up to 1000 and
+// 500 rows 22 us on one kernel, 31 on two.)
+size_t along(Width wider, size_t hd, bool q8) {
+  if (wider == kNarrow32) return hd <= 64 ? 1024 : 512;
+  if (q8) return hd <= 64 ? 384 : 192;
+  return hd <= 128 ? 768 : 320;
+}
+
 Plan make_plan(const size_t* past, const size_t* n_tree, size_t n_seq, size_t n_heads, size_t n_kv, size_t hd,
                bool q8) {
   const size_t group = n_heads / n_kv;
   Plan p{};
-  size_t rows[kWidths] = {};  // cache rows of each width
+  bool has[kWidths] = {};
+  for (int w = 0; w < kWidths; w++) p.as[w] = static_cast<Width>(w);
   for (size_t i = 0; i < n_seq; i++)
-    if (n_tree[i]) rows[width_of(n_tree[i] * group, hd, q8)] += past[i] + n_tree[i];
-  const size_t few = (q8 ? size_t{1} << 24 : size_t{1} << 26) / (n_kv * hd);
-  int wider = -1;
-  for (int w = kWide; w >= 0; w--) {
-    if (!rows[w]) continue;
-    wider = wider >= 0 && rows[w] <= few ? wider : w;
-    p.as[w] = static_cast<Width>(wider);
-  }
+    if (n_tree[i]) has[width_of(n_tree[i] * group, hd, q8)] = true;
   auto width = [&](size_t i) { return p.as[width_of(n_tree[i] * group, hd, q8)]; };
   auto tiles = [&](size_t i) { return width(i) == kWide ? (n_tree[i] * group + kWideRows - 1) / kWideRows : 1; };
-  size_t work[kWidths] = {};  // cache rows times row tiles
-  for (size_t i = 0; i < n_seq; i++)
-    if (n_tree[i]) work[width(i)] += (past[i] + n_tree[i]) * tiles(i);
-  for (int w = 0; w < kWidths; w++) {
+  // The parts of the sequences on kernel w: the rows of the longest.
+  auto split = [&](int w) {
+    size_t work = 0, longest = 0;  // cache rows times row tiles
+    for (size_t i = 0; i < n_seq; i++)
+      if (n_tree[i] && width(i) == w) work += (past[i] + n_tree[i]) * tiles(i);
     const size_t round = 32 * narrow_waves(static_cast<int>(hd)), most = resident(static_cast<Width>(w), hd);
     const size_t unit = w == kWide ? 64 : round, least = w == kWide ? 128 : round;
-    size_t r = std::max(least, (work[w] * n_kv / most + unit - 1) / unit * unit);
+    size_t r = std::max(least, (work * n_kv / most + unit - 1) / unit * unit);
     p.whole[w] = w == kWide ? least : 2 * round;
     for (int tries = 0; tries < 16; tries++) {
       p.rows_per_split[w] = r;
       size_t n = 0;
-      for (size_t i = 0; i < n_seq; i++)
-        if (n_tree[i] && width(i) == w) n += p.parts(w, past[i] + n_tree[i]) * tiles(i);
+      longest = 0;
+      for (size_t i = 0; i < n_seq; i++) {
+        if (!n_tree[i] || width(i) != w) continue;
+        const size_t total = past[i] + n_tree[i], parts = p.parts(w, total);
+        n += parts * tiles(i);
+        longest = std::max(longest, parts > 1 ? r : total);
+      }
       if (n * n_kv <= most) break;
       r += std::max(unit, r / 16 / unit * unit);
     }
+    return longest;
+  };
+  int wider = -1;
+  size_t longest = 0;
+  for (int w = kWide; w >= 0; w--) {
+    if (!has[w]) continue;
+    if (wider >= 0) {
+      p.as[w] = static_cast<Width>(wider);
+      const size_t both = split(wider);
+      if (both <= longest + along(p.as[w], hd, q8)) {
+        longest = both;
+        continue;
+      }
+      p.as[w] = static_cast<Width>(w);
+      split(wider);
+    }
+    wider = w;
+    longest = split(w);
   }
   for (size_t i = 0; i < n_seq; i++) {
     if (!n_tree[i]) continue;

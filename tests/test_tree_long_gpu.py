@@ -95,3 +95,15 @@ def test_a_bound_is_passed_by_a_cache_without_one_row():
     got = P.attention_tree(q, [P.KvF16(k[lost], v[lost])], [past - 1], [1], heads, kv_heads, w)
     want, bound = SB.tree(q, ks, vs, [past], [1], None, heads, kv_heads, w)
     assert not SO.within(got, want, bound)[0]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("w,past", [(64, 6000), (64, 30000), (256, 2000), (256, 9000)])
+def test_single_tokens_beside_a_tree_on_one_kernel_and_on_two(kind, w, past):
+    # few cache rows go along on the wide kernel, more on their own
+    heads, kv_heads, lens, tokens = 4, 4, [500, past // 2, past, 7], [40, 1, 1, 2]
+    q, caches, ks, vs = make(11, kind, lens, tokens, heads, kv_heads, w)
+    got = P.attention_tree(q, caches, lens, tokens, heads, kv_heads, w)
+    want, bound = SB.tree(q, ks, vs, lens, tokens, None, heads, kv_heads, w)
+    ok, worst = SO.within(got, want, bound)
+    assert ok, worst
