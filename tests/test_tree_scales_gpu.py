@@ -147,3 +147,16 @@ def test_scales_at_the_ends_of_their_range(tokens, heads, kv_heads, w, past, pow
         which = (at > len(at) // 2) if split else at % 2
         c.scale(0, 2.0 ** np.array(powers)[np.minimum(which, len(powers) - 1)][:, None])
         check(c, q, [past], [tokens], None, heads)
+
+
+@pytest.mark.parametrize("past", [40, 3000])
+@pytest.mark.parametrize("tokens,heads,kv_heads,w", SHAPES)
+def test_scales_of_either_sign_and_none(tokens, heads, kv_heads, w, past):
+    # a value is its i8 times its scale, whatever made it
+    r = np.random.default_rng(11)
+    q = (r.standard_normal((tokens, heads * w)) * 1.5).astype(np.float32)
+    c = Caches(12, [past + tokens], kv_heads, w)
+    c.scale(0, r.choice([-1.0, 0.0, 1.0], (past + tokens, kv_heads)))
+    check(c, q, [past], [tokens], None, heads)
+    c.scale(0, np.zeros((past + tokens, kv_heads)))
+    assert not P.attention_tree(q, c.caches, [past], [tokens], heads, kv_heads, w).any()
