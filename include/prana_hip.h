@@ -193,13 +193,18 @@ int prana_attention_prefill(const float *q, const float *k, const float *v, size
  * `stream` (NULL = the library's), allocate nothing and keep nothing between
  * calls, so they may be captured into a HIP graph; a replay repeats the call
  * with the sizes and pointers it was captured with. f32 results are
- * f32-accurate (not the scalar tier's bits); an f16 result rounds its
+ * f32-accurate (not the scalar tier's bits): a row's probabilities keep 22 bits,
+ * or 2^-31 of its largest where that is more; an f16 result rounds its
  * probabilities and itself to halves. Equal calls give equal bits. Device
  * pointers lie on 16 bytes (scales on 4), row strides are multiples of 16 bytes
- * and at most 2^24 elements, head_dim is a multiple of 8 up to 256; anything
- * else is PRANA_ERR_INVALID. Outputs do not overlap inputs or one another. In
- * attention, an infinity or NaN that a row sees makes what it reaches of that
- * row infinite or NaN, and no other row's. */
+ * and at most 2^24 elements, head_dim is a multiple of 8 up to 256, a call has
+ * up to 65535 heads, 2^30 rows of a cache, 2^30 rows times heads of a prompt and
+ * of all drafted tokens (a prompt's launch up to 2^32 lanes: 2^29 where head_dim
+ * passes 128); anything else is PRANA_ERR_INVALID. Outputs do not overlap inputs
+ * or one another. In attention, an infinity or NaN that a row sees makes what it
+ * reaches of that row infinite or NaN (a K value may weigh its row out instead,
+ * where the score is -infinity), and no other row's. Prompts start at their first
+ * row: rows behind a filled cache are drafted tokens, up to 64 a call. */
 
 /* Causal attention of whole prompts: sequence s is the next seq_lens[s] rows
  * (0 allowed) of q, k, v and out, and its row i attends to its rows 0..=i. q
@@ -246,15 +251,15 @@ int prana_kv_read_q8(const prana_kv *kv, const size_t *first_rows, const size_t 
  * a chain (token i sees tokens 0..=i), so n_tree = 1 is a decode step and
  * n_tree = k the verify batch of a chain draft. A token that sees no row gets
  * zeros. q and out: device f32 [sum of n_tree][n_heads*head_dim], RoPE applied
- * to q. What masked rows and rows past the drafted ones hold (infinities and
- * NaN too) does not reach the result. workspace: device scratch of the size
- * prana_attention_tree_workspace gives for the same sizes (it may be 0, then
- * workspace may be NULL; no size shrinks it as it grows, so one allocated for
- * the longest caches, most drafted tokens and sequences serves every smaller
- * call); calls that may run at the same time (also replays of
- * two captured graphs) need one each. 8-bit: a weight counts times its V scale,
- * with 22 bits, or to 2^-31 of the largest such product that its row sees;
- * values up to 2^64 in magnitude, those under 2^-105 right to 2^-136 of 1. */
+ * to q. What masked rows and rows past the drafted ones hold (any scale,
+ * infinities and NaN too) does not reach the result. workspace: device scratch of
+ * the size prana_attention_tree_workspace gives for the same sizes (it may be 0,
+ * then workspace may be NULL). It does not shrink as past, n_tree or n_seq grow,
+ * so one for the longest caches, most drafted tokens and sequences serves every
+ * smaller call; calls that may run at the same time (also replays of two captured
+ * graphs) need one each. 8-bit: what keeps 22 bits, or 2^-31 of its row's largest,
+ * is a probability times its V scale. Values up to 2^64 in magnitude; V scales
+ * under 2^-110 are right to 2^-136 a row. */
 int prana_attention_tree(const float *q, int kv_type, const prana_kv *kv, const size_t *past, const size_t *n_tree,
                          size_t n_seq, const uint64_t *mask, size_t n_heads, size_t n_kv_heads, size_t head_dim,
                          float *out, void *workspace, size_t workspace_bytes, prana_stream_t stream);

@@ -27,7 +27,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // may point anywhere for all the compiler knows, and its generic loads count
 // as LDS accesses too, so that each wait for LDS would wait for the loads of the
 // next tile with it (4 prompts up to 1025, 8/1 x 256: 39.1 us with them, 37.3
-// without; 9 prompts up to 8192: 828, 816).
+// without; 2 prompts up to 8191, 32/8 x 128: 828, 816).
 template <class T>
 using device_t = __attribute__((address_space(1))) T;
 template <class T>

@@ -20,12 +20,16 @@
 //
 // f32 form: q * log2(e)/sqrt(w), normalised per row by a power of two, and the
 // probabilities go in as two halves each (22 bits), twice the products. The
-// f16 form rounds a probability to a half (2^-11), as its result is.
+// f16 form rounds a probability to one half (2^-11), as its result is: against 64
+// bits its results are off by 2.5e-4 (4 prompts up to 1025, 8/1 x 256) and 2.7e-4
+// (2 up to 8191, 32/8 x 128) of their norm, where rounding the result alone makes
+// 2.0e-4. Probabilities in two halves would leave that, for 41.3 us instead of 37.6
+// and 1075 instead of 810; a caller who wants them has the f32 form.
 //
-// Measured: two prompts of up to 8191, 32/8 x 128, f16: 800 us, 898 TFLOP/s (a
-// library's f16 product reaches 1155; both run at 1.5 to 1.7 GHz); matrix cores
-// busy 45 % and vector ALU 41 % of the cycles, seldom both. Nine of up to 1501,
-// 14/2 x 64, f32: 51.5 us, 316 TFLOP/s, twice that with both halves' products.
+// Measured: two prompts of up to 8191, 32/8 x 128, f16: 810 to 840 us by card, 855
+// to 885 TFLOP/s (a library's f16 product reaches 1155; both run at 1.5 to 1.7 GHz);
+// matrix cores busy 45 % and vector ALU 41 % of the cycles, seldom both. Nine of up
+// to 1501, 14/2 x 64, f32: 52.5 us, 310 TFLOP/s, twice that with both halves' products.
 // Computing scores a tile ahead (1044 us instead of 806) and groups of waves that
 // take products and softmax in turn (904 instead of 827) cost more registers and
 // barriers than they hide.

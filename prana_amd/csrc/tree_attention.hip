@@ -11,7 +11,8 @@
 // All products run on the f16 matrix cores: q * log2(e)/sqrt(w), normalised
 // per row by a power of two, and the probabilities go in as two halves each
 // (22 bits); f16 and i8 cache values are halves exactly. An 8-bit row's K scale
-// multiplies its scores, its V scale its probabilities.
+// multiplies its scores, its V scale its probabilities, whose reference then is the
+// largest such product.
 //
 // Two kernels, by the rows of a sequence and KV head:
 //   narrow (up to 32 rows): bound by reading the cache. The eight waves of a
@@ -26,18 +27,17 @@
 // the sums are rescaled.
 //
 // Measured, 32/8 heads x 128. Narrow: one token in each of 8 sequences over up
-// to 32767 8-bit rows 98 us, 4.0 TB/s of cache (a bare loop over such 128-byte
-// pieces of rows reads 5.4); the vector ALU is busy 46 % of the time, half of
-// that with turning i8 into halves, the matrix cores 16 %. Twelve waves instead
+// to 32767 8-bit rows 101 us, 3.9 TB/s of cache (a bare loop over such 128-byte
+// pieces of rows reads 5.4); the vector ALU is busy 41 % of the time, half of
+// that with turning i8 into halves, the matrix cores 15 %. Twelve waves instead
 // of eight spill (110 us); 16-byte loads of i8 gain 0.5 %. Wide: trees of up to
-// 64 in 8 sequences over up to 16385 f16 rows 196 us, 378 TFLOP/s, twice that
-// with both halves' products (a library's f16 product reaches 1155), 11 of it
-// joining; matrix cores busy 42 %, vector ALU 29 %, the rest waits for LDS and
-// at barriers. Short calls are launches and trips to memory one after another:
+// 64 in 8 sequences over up to 16385 f16 rows 194 to 203 us by card, 365 to 380
+// TFLOP/s, twice that with both halves' products (a library's f16 product reaches
+// 1155), 11 of it joining; matrix cores busy 45 %, vector ALU 33 %, the rest waits
+// for LDS and at barriers. Short calls are launches and trips to memory one after another:
 // one token over 511 rows 9 us, four trees of 13 over up to 4099 rows 12.
 #include <algorithm>
 #include <cmath>
-#include <vector>
 
 #include "common.h"
 #include "mfma_tile.h"
@@ -633,8 +633,9 @@ __global__ __launch_bounds__(kTrNT, HDP <= 128 ? 2 : 1) void tree_wide_kernel(Tr
   __shared__ __attribute__((aligned(16))) uint16_t s_k[BN * S::kLdK];
   __shared__ __attribute__((aligned(16))) uint16_t s_v[BN * S::kLdV];
   __shared__ __attribute__((aligned(16))) float s_scale[3][64];  // K scales, V scales, their scale_log2
-  // The smaller halves of q, in LDS where the registers would spill (6 trees of
-  // 48 over up to 9000 f16 rows, 24/6 x 256: 212 us in registers, 140 in LDS).
+  // The smaller halves of q, in LDS where the registers would not hold them (6 trees
+  // of 48 over up to 9000 f16 rows, 24/6 x 256: 212 us in registers, 140 in LDS, where
+  // 21 registers still spill, 14 of the 8-bit form).
   constexpr bool kLowInLds = HDP > 192;
   __shared__ __attribute__((aligned(16))) half8 s_ql[kLowInLds ? S::kStepsQK * kTrNT : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1028,10 +1029,10 @@ void launch_join(const JoinArgs& j, hipStream_t s) {
 
 // ------------------------------------------------------------ plan
 // Kernel of a sequence, by its rows per KV head. Two blocks of narrow rows only
-// over 8-bit caches of heads up to 128 wide, which leave them the registers:
-// 10 tokens in four sequences, 12/4 x 128, caches up to 4000 and 20000, take
-// 16.7 and 28.6 us there and 18.1 and 35 on the wide kernel (three quarters of
-// it idle), but 17.9 and 34 against 13.6 and 29 in f16.
+// over 8-bit caches of heads up to 128 wide, which leave them the registers (9
+// spill at 128 all the same): 10 tokens in four sequences, 12/4 x 128, caches up to
+// 4000 and 20000, take 16.7 and 28.4 us there and 19.4 and 38.5 on the wide kernel
+// (three quarters of it idle), but 17.9 and 34 against 13.6 and 29 in f16.
 enum Width { kNarrow16, kNarrow32, kWide, kWidths };
 Width width_of(size_t rows, size_t hd, bool q8) {
   return rows <= 16 ? kNarrow16 : rows <= 32 && hd <= 128 && q8 ? kNarrow32 : kWide;
