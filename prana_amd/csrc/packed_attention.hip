@@ -15,7 +15,7 @@
 //                 this product (its keys in the order the registers hold
 //                 them), and V comes out of LDS transposed to match. No
 //                 probability moves between lanes.
-// The maximum lags: it is raised, and the sums rescaled, only when a score
+// The maximum lags: a row's is raised, and its sums rescaled, only when a score
 // passes it by more than 2^8, so probabilities are at most 256.
 //
 // f32 form: q * log2(e)/sqrt(w), normalised per row by a power of two, and the

@@ -24,7 +24,7 @@
 // In both S^T = K Q^T leaves a row's scores in the lanes of one column, whose
 // registers are, as halves, the operand of O^T += V^T P^T; V comes out of LDS
 // transposed to match. The kept maximum lags the scores by up to 2^8 before
-// the sums are rescaled.
+// the sums are rescaled, each row's for itself.
 //
 // Measured, 32/8 heads x 128. Narrow: one token in each of 8 sequences over up
 // to 32767 8-bit rows 101 us, 3.9 TB/s of cache (a bare loop over such 128-byte
@@ -34,8 +34,8 @@
 // 64 in 8 sequences over up to 16385 f16 rows 194 to 203 us by card, 365 to 380
 // TFLOP/s, twice that with both halves' products (a library's f16 product reaches
 // 1155), 11 of it joining; matrix cores busy 45 %, vector ALU 33 %, the rest waits
-// for LDS and at barriers. Short calls are launches and trips to memory one after another:
-// one token over 511 rows 9 us, four trees of 13 over up to 4099 rows 12.
+// for LDS and at barriers. Short calls are launches and trips to memory one after
+// another: one token over 511 rows 9 us, four trees of 13 over up to 4099 rows 12.
 #include <algorithm>
 #include <cmath>
 
@@ -159,9 +159,9 @@ __device__ __forceinline__ void load_values(const unsigned char* p, float scale,
 // scales the keys have that the row does not see or gives no weight. With 2^x
 // above a key's scale, what is compared is score + x (log2 units); the weights
 // and their sum count from the reference, the largest score (m, before c) and
-// the rest (e) of it. (One power of two for all rows of a
-// wave, over all scales met, took 8 single tokens over up to 32767 rows 3 us less
-// of 98, but a masked row of large scale took the other rows' bits.)
+// the rest (e) of it. (8 single tokens over up to 32767 rows, 32/8 x 128: 101 us; 98
+// with one power of two for all rows of a wave, over all scales met, where a masked
+// row of large scale took the other rows' bits.)
 constexpr float kTop = kLag + kPShift;  // products of weights and scales stay under 2^kTop
 constexpr float kUnseen = -3e38f;       // in place of a row's reference when it has seen nothing
 // The scales themselves are taken times 2^32, so that x reaches from scales of
